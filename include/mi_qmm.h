@@ -36,9 +36,10 @@
 extern "C" {
 #endif
 
-#define MI_ABI_VERSION 7  /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
+#define MI_ABI_VERSION 8  /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
                              4: mi_argmax_noalloc; 5: the qmm workspace entries;
-                             6: mi_qmm_affine_qkv_norm_rope; 7: mi_sdpa_ws */
+                             6: mi_qmm_affine_qkv_norm_rope; 7: mi_sdpa_ws;
+                             8: the paged cache entries, mi_token_logprobs */
 
 enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 };
 
@@ -308,6 +309,76 @@ int mi_argmax(const void *x, int32_t *out, int64_t rows, int64_t V, int dtype, v
  * V = 151936 bf16), else MI_ERR_ARG. Same result as mi_argmax. Calls that
  * overlap on one GPU race on that array. */
 int mi_argmax_noalloc(const void *x, int32_t *out, int64_t rows, int64_t V, int dtype,
+                      void *stream);
+
+/* Serving several requests over a paged key/value cache (no counterpart in the
+ * reference, whose caches are contiguous, one request each). The pools k_pages
+ * and v_pages are T [n_pages, Hkv, page_size, D], page_size 16, 32, 64, 128 or
+ * 256, n_pages * page_size < 2^31. block_table int32 [R, table_width]: page
+ * j / page_size of request r holds its key j in row j % page_size. A slot is
+ * page * page_size + row. The tokens of a step lie request after request;
+ * cu_q int32 [R + 1] holds where each request's tokens start, and their number.
+ * All of these arrays are on the device, so a step can be captured in a graph
+ * and replayed at other lengths.
+ *
+ * mi_paged_plan: one step's bookkeeping. kv_lens[r] keys are cached and
+ * q_lens[r] tokens are new; the pages a request lacks are taken from the end of
+ * free_pages[0, *free_count) (capacity n_free), request after request, and
+ * entered into the block table. Written: cu_q; kv_after[r] = kv_lens[r] +
+ * q_lens[r]; of token t the position in its request and its slot (0 and -1 past
+ * the last token: T may exceed their number, and must not be less);
+ * *free_left, the free pages that remain; *refused, the number of refused
+ * requests. A request that needs pages and whose pages, behind those of the
+ * requests before it, exceed *free_count, or whose keys would pass its row of
+ * the table, is refused: it takes none, kv_after[r] = 0 and its slots are -1.
+ * The inputs stay as they are (the table's entries of cached keys too). 1 <= R
+ * <= 4096, table_width <= 131072. */
+int mi_paged_plan(int32_t *block_table, int64_t table_width, const int32_t *kv_lens,
+                  const int32_t *q_lens, const int32_t *free_pages, int64_t n_free,
+                  const int32_t *free_count, int64_t R, int64_t T, int64_t page_size,
+                  int32_t *cu_q, int32_t *kv_after, int32_t *positions, int32_t *slots,
+                  int32_t *free_left, int32_t *refused, void *stream);
+
+/* The attention prologue of T tokens: q [T, Hq, D] (row stride q_row_stride) ->
+ * rms_norm(q_norm) -> rope -> q_out [T, Hq, D]; k likewise -> its token's slot of
+ * k_pages; v -> copied to its slot of v_pages. A NULL norm weight skips the
+ * normalization. RoPE turns pair i < rope_dims / 2 of token t by positions[t] *
+ * inv_freq[i] (fp64, radians per position; any long-context scaling is in the
+ * table); pairs are (i, i + rope_dims / 2), or (2 i, 2 i + 1) with traditional;
+ * values from rope_dims on (a multiple of 8, at most D) are not turned. Computed
+ * in fp32 and rounded once. A token with a slot outside the pool writes no k and
+ * v; two tokens with one slot leave either's. Rows and norm weights 16- and
+ * 8-byte aligned. bf16 and fp16, D in {64, 128}. */
+int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_row_stride,
+                       int64_t k_row_stride, int64_t v_row_stride, const void *q_norm,
+                       const void *k_norm, void *q_out, void *k_pages, void *v_pages,
+                       const double *inv_freq, int rope_dims, int traditional,
+                       const int32_t *positions, const int32_t *slots, int64_t T, int64_t Hq,
+                       int64_t Hkv, int64_t D, int64_t n_pages, int64_t page_size, float eps,
+                       int dtype, void *stream);
+
+/* Causal attention of every request's new tokens over its pages: q [T, H, D] ->
+ * out [T, H, D]. Request r's tokens are rows [cu_q[r], cu_q[r + 1]) (held to T),
+ * its keys kv_lens[r] (these tokens' own among them); its token i sees keys
+ * j <= kv_lens[r] - n + i with n its tokens (a token that sees none gives 0). Rows of
+ * out behind the last request's are left as they were. Page ids outside the pool
+ * are held to it. bf16 and fp16, D in {64, 128}. */
+int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages, void *out,
+                       const int32_t *block_table, const int32_t *cu_q, const int32_t *kv_lens,
+                       int64_t T, int64_t R, int64_t table_width, int64_t H, int64_t HK, int64_t D,
+                       int64_t n_pages, int64_t page_size, float scale, int dtype, void *stream);
+
+/* Log probabilities (no counterpart in the reference, which samples greedily):
+ * logits T [rows, V] (row stride row_stride elements), lse their row's log sum
+ * exp. logprobs[r] = logits[r, tokens[r]] - lse (NaN for a token outside [0, V));
+ * entropy[r] = -sum p log p (a logit of -inf adds 0); the `top` most probable
+ * tokens, the lowest index first among equal logits: top_ids int32 [rows, top]
+ * and top_logprobs [rows, top]. All fp32. 0 <= top <= 64, top <= V <= 2^30. A row
+ * with a NaN or +inf, or of -inf alone, gives NaN (its top_ids stay in [0, V)).
+ * tokens are int32 or int64 (tokens_are_64). */
+int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_stride,
+                      const void *tokens, int tokens_are_64, int top, float *logprobs,
+                      float *entropy, int32_t *top_ids, float *top_logprobs, int dtype,
                       void *stream);
 
 #ifdef __cplusplus

@@ -25,7 +25,7 @@ import torch
 
 PKG = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("MI_QMM_LIB", PKG / "libmiqmm.so"))
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 MI_OK, MI_ERR_ARG, MI_ERR_UNSUPPORTED, MI_ERR_LAUNCH = 0, 1, 2, 3
@@ -74,6 +74,13 @@ SIGNATURES: dict[str, list] = {
     "mi_argmax_workspace_bytes": [_I64, _I64],
     "mi_argmax": [_P, _P, _I64, _I64, _I, _P, _I64, _P],
     "mi_argmax_noalloc": [_P, _P, _I64, _I64, _I, _P],
+    "mi_paged_plan": [_P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P,
+                      _P],
+    "mi_norm_rope_paged": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P,
+                           _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P],
+    "mi_paged_attention": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                           _I64, _F, _I, _P],
+    "mi_token_logprobs": [_P, _I64, _I64, _I64, _P, _I, _I, _P, _P, _P, _P, _I, _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
             "mi_gelu_mlp_f32_workspace_bytes": ctypes.c_int64,
@@ -423,6 +430,16 @@ def b_sdpa(ins, outs, p):
     if tuple(o.shape) != want or o.dtype != q.dtype or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"sdpa output must be {q.dtype} {want}")
     sdpa(q, k, v, o, Lk, Lk, float(p["scale"]), int(p.get("causal", 1)), layout)
+
+
+def paged_attention(q, k_pages, v_pages, out, table, cu_q, kv_lens, scale: float) -> None:
+    """mi_paged_attention over checked tensors."""
+    T, H, D = q.shape
+    n_pages, HK, page, _ = k_pages.shape
+    R, width = table.shape
+    _check(lib().mi_paged_attention(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(table),
+                                    _ptr(cu_q), _ptr(kv_lens), T, R, width, H, HK, D, n_pages,
+                                    page, scale, _dt(q), _stream(q)), "paged_attention")
 
 
 def b_swiglu(ins, outs, p):

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -306,6 +307,188 @@ def argmax(x, split: bool = True) -> torch.Tensor:
     o = _empty(x.shape[:-1], x, torch.int32)
     hip.b_argmax([x], [o], {"split": split})
     return o
+
+
+# -- several requests over a paged KV cache (no counterpart in the reference) ----
+#
+# Pools of pages k_pages, v_pages [n_pages, HK, page_size, D]; a block table int32
+# [R, width] of each request's pages; the tokens of a step request after request.
+
+def _i32(what: str, like: torch.Tensor, **arrays) -> None:
+    for name, t in arrays.items():
+        if t.dtype != torch.int32 or t.device != like.device or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous int32 array on {like.device}")
+
+
+class PagedPlan(NamedTuple):
+    """One step's bookkeeping, on the GPU (``paged_plan``)."""
+
+    cu_q: torch.Tensor        # int32 [R + 1]: where each request's tokens start
+    kv_lens: torch.Tensor     # int32 [R]: its keys after the step, 0 if refused
+    positions: torch.Tensor   # int32 [num_tokens]: each token's position in its request
+    slots: torch.Tensor       # int32 [num_tokens]: its cache slot, -1 if it has none
+    free_count: torch.Tensor  # int32 [1]: the free pages that remain
+    refused: torch.Tensor     # int32 [1]: requests that got no pages
+
+
+def paged_plan(block_table, kv_lens, q_lens, free_pages, free_count, page_size: int,
+               num_tokens: int) -> PagedPlan:
+    """A step's bookkeeping in one launch: request r holds kv_lens[r] keys and
+    brings q_lens[r] tokens (int32 [R]); the pages it lacks are taken from the end
+    of free_pages[:free_count] (int32 [F], int32 [1]), request after request, and
+    written into block_table (int32 [R, width]) in place. num_tokens: rows of the
+    step's token buffer, at least the sum of q_lens (rows behind it get position 0
+    and slot -1). A request whose pages are not there, or whose keys would pass
+    its row of the table, takes none and is counted in ``refused``."""
+    hip._require_gpu(block_table)
+    if block_table.dim() != 2 or kv_lens.dim() != 1 or kv_lens.shape != q_lens.shape \
+            or kv_lens.shape[0] != block_table.shape[0] or free_pages.dim() != 1 \
+            or free_count.numel() != 1:
+        raise ValueError("paged_plan takes block_table [R, width], kv_lens [R], q_lens [R], "
+                         "free_pages [F] and free_count [1]")
+    _i32("paged_plan", block_table, block_table=block_table, kv_lens=kv_lens, q_lens=q_lens,
+         free_pages=free_pages, free_count=free_count)
+    R, width = block_table.shape
+    T = int(num_tokens)
+    # one allocation for the six outputs, each from a 16-byte boundary
+    sizes = (R + 1, R, T, T, 1, 1)
+    at, starts = 0, []
+    for n in sizes:
+        starts.append(at)
+        at += (n + 3) & ~3
+    buf = block_table.new_empty(at)
+    out = PagedPlan(*(buf[s:s + n] for s, n in zip(starts, sizes)))
+    hip._check(hip.lib().mi_paged_plan(
+        block_table.data_ptr(), width, kv_lens.data_ptr(), q_lens.data_ptr(),
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), R, T, int(page_size),
+        *(t.data_ptr() for t in out), hip._stream(block_table)), "paged_plan")
+    return out
+
+
+def rope_table(dims: int, base: float = 10000.0, scale: float = 1.0, freqs=None,
+               device="cuda") -> torch.Tensor:
+    """The angle per position of each rotation pair, fp64 [dims / 2], made once and
+    kept: scale * base^(-2 i / dims), or scale / freqs[i] where ``freqs`` is given
+    (mx.fast.rope's argument: long-context scalings that stretch each wavelength
+    differently)."""
+    if freqs is not None:
+        f = torch.as_tensor(freqs, dtype=torch.float64, device=device)
+        if tuple(f.shape) != (dims // 2,):
+            raise ValueError(f"freqs must hold {dims // 2} values, got {tuple(f.shape)}")
+        return scale / f
+    i = torch.arange(dims // 2, dtype=torch.float64, device=device)
+    return scale * base ** (-2.0 * i / dims)
+
+
+def _paged_pools(what: str, q, k_pages, v_pages, D: int) -> tuple:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != D \
+            or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype \
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise ValueError(f"{what}: the pools must be contiguous {q.dtype} [pages, heads, page size, "
+                         f"{D}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    return k_pages.shape
+
+
+def norm_rope_paged(q, k, v, q_norm, k_norm, n_heads: int, n_kv_heads: int, eps: float,
+                    inv_freq, positions, slots, k_pages, v_pages,
+                    traditional: bool = False) -> torch.Tensor:
+    """The attention prologue of a step's tokens in one launch: q [T, H * D] ->
+    rms_norm(q_norm) -> rope -> [T, H, D] (returned); k -> rms_norm(k_norm) -> rope
+    and v, written to each token's slot of the pools (none where the slot is -1).
+    A norm weight of None skips the normalization. ``inv_freq``: ``rope_table``'s,
+    whose 2 * len(inv_freq) leading values of a head are turned, at the angle of
+    each token's own position. q, k, v may be column ranges of one projection."""
+    T = q.shape[0]
+    D = q.shape[-1] // n_heads
+    for name, t, h in (("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads)):
+        if t.dim() != 2 or tuple(t.shape) != (T, h * D) or t.dtype != q.dtype:
+            raise ValueError(f"norm_rope_paged: {name} must be {q.dtype} {(T, h * D)}, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+    for wt in (q_norm, k_norm):
+        if wt is not None and (tuple(wt.shape) != (D,) or wt.dtype != q.dtype
+                               or not wt.is_contiguous()):
+            raise ValueError(f"norm weight must be contiguous {q.dtype} [{D}]")
+    n_pages, hk, page, _ = _paged_pools("norm_rope_paged", q, k_pages, v_pages, D)
+    if hk != n_kv_heads or positions.shape != (T,) or slots.shape != (T,):
+        raise ValueError(f"norm_rope_paged: pools of {n_kv_heads} heads, positions and slots of "
+                         f"{T} tokens are needed")
+    _i32("norm_rope_paged", q, positions=positions, slots=slots)
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
+            or inv_freq.device != q.device:
+        raise ValueError("norm_rope_paged: inv_freq must be a float64 array (ops.rope_table)")
+    hip._require_gpu(q)
+    # rows the kernel cannot read in 16-byte pieces are copied first
+    q, k, v = (t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+               else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    out = q.new_empty((T, n_heads, D))
+    hip._check(hip.lib().mi_norm_rope_paged(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+        hip._ptr(q_norm), hip._ptr(k_norm), out.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(traditional),
+        positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv_heads, D, n_pages, page,
+        float(eps), hip._dt(q), hip._stream(q)), "norm_rope_paged")
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale: float,
+                    max_q_len: int | None = None) -> torch.Tensor:
+    """Causal GQA attention of every request's new tokens over its pages, one call
+    for requests of any lengths: q [T, H, D] -> [T, H, D]. Request r's tokens are
+    rows [cu_q[r], cu_q[r + 1]), its keys kv_lens[r], these tokens' own among them
+    (``paged_plan``'s cu_q and kv_lens). max_q_len: the most tokens a request
+    brings, where the caller knows it: it chooses the kernels, never the result's
+    meaning. Rows behind the last request's are not written."""
+    if q.dim() != 3:
+        raise ValueError(f"paged_attention: q must be [T, H, D], got {tuple(q.shape)}")
+    T, H, D = q.shape
+    n_pages, HK, page, _ = _paged_pools("paged_attention", q, k_pages, v_pages, D)
+    R = kv_lens.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] != R or cu_q.shape != (R + 1,):
+        raise ValueError("paged_attention takes block_table [R, width], cu_q [R + 1], kv_lens [R]")
+    _i32("paged_attention", q, block_table=block_table, cu_q=cu_q, kv_lens=kv_lens)
+    hip._require_gpu(q)
+    q = q.contiguous()
+    out = torch.empty_like(q)
+    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, float(scale))
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    """``token_logprobs``' results, fp32 (ids int32)."""
+
+    logprobs: torch.Tensor      # [rows]
+    entropy: torch.Tensor       # [rows]
+    top_ids: torch.Tensor       # [rows, top]
+    top_logprobs: torch.Tensor  # [rows, top]
+
+
+def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens: logits [..., V], tokens [...] -> each
+    row's log softmax at its token (NaN outside [0, V)), its entropy, and its
+    ``top`` (0 to 64) most probable tokens with their log probabilities, the lowest
+    index first among equal logits. Logits of -inf are forbidden tokens."""
+    hip._require_gpu(logits)
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if tokens.shape != lead or tokens.dtype not in (torch.int32, torch.int64) \
+            or tokens.device != logits.device:
+        raise ValueError(f"token_logprobs: tokens must be int32 or int64 {tuple(lead)} on "
+                         f"{logits.device}")
+    if V < 1 or not 0 <= top <= min(64, V):
+        raise ValueError(f"token_logprobs: top={top} of V={V} (0 to 64, at most V)")
+    if logits.stride(-1) != 1 or (logits.dim() != 2 and not logits.is_contiguous()):
+        logits = logits.contiguous()
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    tokens = tokens.contiguous()
+    rows = x.shape[0]
+    f32 = x.new_empty(rows * (2 + top), dtype=torch.float32)
+    ids = x.new_empty((*lead, top), dtype=torch.int32)
+    out = TokenLogprobs(f32[:rows].view(lead), f32[rows:2 * rows].view(lead), ids,
+                        f32[2 * rows:].view(*lead, top))
+    hip._check(hip.lib().mi_token_logprobs(
+        x.data_ptr(), rows, V, x.stride(0), tokens.data_ptr(), int(tokens.dtype == torch.int64),
+        top, out.logprobs.data_ptr(), out.entropy.data_ptr(), ids.data_ptr(),
+        out.top_logprobs.data_ptr(), hip._dt(x), hip._stream(x)), "token_logprobs")
+    return out
 
 
 def default_scale(head_dim: int) -> float:

@@ -7,7 +7,7 @@ oracle/Makefile; `build_all()` runs both.
 
 Flags: -O3, gfx950 only, packed-fp32 VALU forms disabled on the device
 (`-packed-fp32-ops`); the host pass warns that it does not know the feature,
-which is harmless. SOURCE_FLAGS adds per-file flags (mi_attn.hip: MFMA
+which is harmless. SOURCE_FLAGS adds per-file flags (the attention files: MFMA
 results in arch VGPRs).
 """
 
@@ -36,13 +36,14 @@ FLAGS = [
 ]
 
 
-# Per-source device flags. mi_attn.hip: MFMA results in arch VGPRs. By
+# Per-source device flags. The attention files: MFMA results in arch VGPRs. By
 # default the compiler kept the attention accumulators in AGPRs and copied
 # them through VGPRs for every tile's softmax rescale and stream merge
 # (272 v_accvgpr_read/write in the 64-wide form, about 40 % of its
 # loop's VALU), which also cost occupancy. Same instructions otherwise, same
 # results.
-SOURCE_FLAGS = {"mi_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+                for name in ("mi_attn.hip", "mi_paged_attn.hip")}
 
 
 def _run(cmd: list[str]) -> None:
