@@ -30,6 +30,12 @@ region kind as the o_proj cut, and layer i+1 takes that normalized output
 instead of normalizing its input again (one launch fewer per layer, same
 bits).
 
+Several requests of different lengths run together over a paged cache
+(``PagedBatch``, ``Qwen3Model.forward_paged``, ``generate_paged``; no counterpart
+in the reference): the layers and their region wrapper are the same, the tokens
+of all requests being the rows of one [1, T, hidden] input; only the attention
+prologue and the attention are the paged ones (``Attention.paged``).
+
 Only the last position's logits are computed in prefill (the caller takes
 logits[:, -1] before sampling; everything before it is dead work,
 docs/measurement.md:74-83).
@@ -108,6 +114,57 @@ class KVCache:
         self.offset = 0
 
 
+class PagedKVCache:
+    """One layer's pools of pages, of the requests of a ``PagedBatch``."""
+
+    def __init__(self, batch: "PagedBatch", shape, device, dtype):
+        self.batch = batch
+        self.keys = torch.zeros(shape, device=device, dtype=dtype)
+        self.values = torch.zeros_like(self.keys)
+
+
+class PagedBatch:
+    """``max_requests`` requests over shared pools of ``n_pages`` pages a layer.
+
+    Lengths, block table and free list live on the GPU and are changed in place,
+    so a step can be captured in a graph. ``step(q_lens, num_tokens)`` plans the
+    next one: request r brings q_lens[r] tokens (0: it waits), whose rows lie
+    request after request in a buffer of num_tokens rows; ``plan.refused`` counts
+    the requests for which pages were missing (they keep what they have, and may
+    bring their tokens again). ``finish(r)`` gives a request's pages back."""
+
+    def __init__(self, cfg: "Qwen3Config", n_layers: int, max_requests: int, n_pages: int,
+                 page_size: int, max_len: int, device, dtype=torch.bfloat16):
+        def i32(*shape):
+            return torch.zeros(shape, dtype=torch.int32, device=device)
+
+        self.page_size = page_size
+        self.block_table = i32(max_requests, -(-max_len // page_size))
+        self.lens = i32(max_requests)
+        self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=device)
+        self.free_count = i32(1) + n_pages
+        self.inv_freq = ops.rope_table(cfg.head_dim, cfg.rope_theta, device=device)
+        self.plan, self.max_q_len = None, None
+        shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
+        self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
+
+    def step(self, q_lens, num_tokens: int, max_q_len: int | None = None) -> ops.PagedPlan:
+        """max_q_len: the most tokens a request brings, where the caller knows it."""
+        p = ops.paged_plan(self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
+                           self.page_size, num_tokens)
+        self.lens.copy_(torch.where(p.kv_lens > 0, p.kv_lens, self.lens))
+        self.free_count.copy_(p.free_count)
+        self.plan, self.max_q_len = p, max_q_len
+        return p
+
+    def finish(self, r: int) -> None:
+        n = -(-int(self.lens[r]) // self.page_size)
+        at = int(self.free_count)
+        self.free_pages[at:at + n] = self.block_table[r, :n]
+        self.free_count += n
+        self.lens[r] = 0
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: Qwen3Config, mods: dict):
         super().__init__()
@@ -116,12 +173,26 @@ class Attention(nn.Module):
             setattr(self, k, v)
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
 
-    def forward(self, x, cache: KVCache):
+    def paged(self, q, k, v, cache: PagedKVCache):
+        """The planned step's attention from its q, k and v [1, T, heads * D]:
+        [1, T, H * D]."""
+        c, b = self.cfg, cache.batch
+        qr = ops.norm_rope_paged(q[0], k[0], v[0], self.q_norm.weight, self.k_norm.weight,
+                                 c.num_attention_heads, c.num_key_value_heads, c.rms_norm_eps,
+                                 b.inv_freq, b.plan.positions, b.plan.slots, cache.keys,
+                                 cache.values)
+        o = ops.paged_attention(qr, cache.keys, cache.values, b.block_table, b.plan.cu_q,
+                                b.plan.kv_lens, self.scale, b.max_q_len)
+        return o.view(1, o.shape[0], -1)
+
+    def forward(self, x, cache: KVCache | PagedKVCache):
         c = self.cfg
         B, L, _ = x.shape
         q = self.q_proj(x)
         k = self.k_proj(x)
         v = self.v_proj(x)
+        if isinstance(cache, PagedKVCache):
+            return self.o_proj(self.paged(q, k, v, cache))
         qr = ops.norm_rope(q, self.q_norm.weight, c.num_attention_heads, c.rms_norm_eps,
                            c.head_dim, c.rope_theta, cache.offset)
         ops.norm_rope(k, self.k_norm.weight, c.num_key_value_heads, c.rms_norm_eps, c.head_dim,
@@ -186,6 +257,44 @@ class Qwen3Model(nn.Module):
             h = h[:, -1:, :]
         return self.model.embed_tokens.as_linear(self.model.norm(h))
 
+    def make_batch(self, max_requests: int, n_pages: int, page_size: int = 64,
+                   max_len: int = 8192) -> PagedBatch:
+        return PagedBatch(self.cfg, len(self.model.layers), max_requests, n_pages, page_size,
+                          max_len, self.model.norm.weight.device)
+
+    def forward_paged(self, ids, batch: PagedBatch):
+        """The planned step (``batch.step``): ids [T], every request's tokens one
+        request after another -> logits [requests, vocab] of each one's last token
+        (of a request that brought none, the row means nothing)."""
+        h = self.model.embed_tokens(ids[None])
+        for layer, cache in zip(self.model.layers, batch.caches):
+            h = layer(h, cache)
+        last = (batch.plan.cu_q[1:] - 1).clamp(0, ids.shape[0] - 1)
+        h = h[0].index_select(0, last)
+        return self.model.embed_tokens.as_linear(self.model.norm(h[None]))[0]
+
+
+def generate_paged(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int, top: int = 0):
+    """Greedy tokens of several prompts at once (1-d int64 arrays, one a request of
+    an empty ``batch``): (tokens [n_tokens, R], their ``ops.TokenLogprobs`` a step).
+    One prefill step for all prompts, then decode steps; nothing waits for the GPU
+    before the end."""
+    dev = batch.lens.device
+    lens = [p.numel() for p in prompts]
+    ids = torch.cat([p.to(dev) for p in prompts])
+    batch.step(torch.tensor(lens, dtype=torch.int32, device=dev), ids.numel(), max(lens))
+    one = torch.ones(len(lens), dtype=torch.int32, device=dev)
+    tokens, logprobs = [], []
+    for i in range(n_tokens):
+        logits = model.forward_paged(ids, batch)
+        ids = ops.argmax(logits)
+        tokens.append(ids)
+        logprobs.append(ops.token_logprobs(logits, ids, top))
+        ids = ids.long()
+        if i + 1 < n_tokens:
+            batch.step(one, len(lens), 1)
+    return torch.stack(tokens), logprobs
+
 
 # ---------------------------------------------------------------------------
 # region wrapper
@@ -237,7 +346,7 @@ class Qwen3LayerRegions(SizedRegions):
         self.__dict__["_prev"] = prev
         self.__dict__["_next"] = nxt
 
-    def forward(self, x, cache: KVCache):
+    def forward(self, x, cache: KVCache | PagedKVCache):
         w = self.wrapped
         if not (x.dim() == 3 and x.dtype == torch.bfloat16 and x.is_cuda):
             return w(x, cache)
@@ -250,8 +359,8 @@ class Qwen3LayerRegions(SizedRegions):
             xn = w.input_layernorm(x)
         projs = (attn.q_proj, attn.k_proj, attn.v_proj)
         ins = [xn] + [t for m in projs for t in (m.weight, m.scales, m.biases)]
-        qr = None
-        if self._serves("qkv", ins, L):
+        qr, paged = None, isinstance(cache, PagedKVCache)
+        if not paged and self._serves("qkv", ins, L):
             # the q/k/v cut with the prologue below in its epilogue, the same
             # bits (None: shapes the fused entry does not take)
             qr = ops.qkv_norm_rope(xn, [(m.weight, m.scales, m.biases) for m in projs],
@@ -262,15 +371,19 @@ class Qwen3LayerRegions(SizedRegions):
         if qr is None:
             outs = self._try("qkv", ins, L)
             q, k, v = (m(xn) for m in projs) if outs is None else outs
+        if paged:
+            o = attn.paged(q, k, v, cache)
+        elif qr is None:
             # q/k-norm + RoPE + the KV-cache update, one launch
             qr = ops.norm_rope_qkv(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
                                    c.num_attention_heads, c.num_key_value_heads, c.rms_norm_eps,
                                    c.head_dim, c.rope_theta, cache.offset, cache.keys,
                                    cache.values, cache.offset)
-        o = ops.scaled_dot_product_attention(qr, cache.keys, cache.values, attn.scale,
-                                             "causal" if L > 1 else None,
-                                             kv_len=cache.offset + L,
-                                             out_layout=1).reshape(B, L, -1)
+        if not paged:
+            o = ops.scaled_dot_product_attention(qr, cache.keys, cache.values, attn.scale,
+                                                 "causal" if L > 1 else None,
+                                                 kv_len=cache.offset + L,
+                                                 out_layout=1).reshape(B, L, -1)
         op, pn = attn.o_proj, w.post_attention_layernorm
         outs = self._try("residual_rmsnorm", [o, op.weight, op.scales, op.biases, x, pn.weight], L)
         if outs is None:
