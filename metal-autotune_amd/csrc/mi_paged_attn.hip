@@ -11,6 +11,14 @@
 // (mi_attn_common.h). A kv head's query rows, token after token and in a token
 // its G q heads, are the columns of 32-wide blocks, so K and V are read once per
 // block and kv head and a block sees nearly one causal range.
+//
+// Requests differ in length, and only the GPU knows the lengths. The keys of
+// every block are therefore cut into chunks of one size, chosen on the GPU from
+// the lengths of all requests so that the chunks fill the chip (chunk_of), and a
+// workgroup finds its chunk by summing over the requests. A block of one chunk
+// writes its rows; the others' states go to a workspace and
+// paged_combine_kernel folds them. The chunk size, so a row's last bits, depends
+// on the lengths of the whole batch.
 #include "mi_attn_common.h"
 
 namespace mi {
@@ -18,19 +26,13 @@ namespace {
 
 constexpr int PA_WAVES = ATT_STREAMS;
 
-// The work of one workgroup beside its kv head.
-struct PagedItem {
-    int r;       // request, < 0: none
-    int q0, n;   // its first token, its tokens
-    int len;     // its keys
-    int cb;      // column block
-};
-
 struct PagedArgs {
     const void *q, *k, *v;
     void *out;
     const int *table, *cu_q, *kv_lens;
+    float *part;  // partial states, by item and kv head; null: no block is cut
     int T, R, W, H, HK, G, pages, page_log2;
+    int target;     // chunks wanted for a kv head
     float scale;    // > 0, log2 units
     uint32_t flip;  // sign bits of a negative scale, for Q
 };
@@ -50,30 +52,93 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// Item u of the column blocks of all requests in order; every wave finds it by
-// itself, 64 requests a step.
+constexpr int CHUNK_KEYS = ATT_KT * PA_WAVES;  // keys are cut in multiples of this
+
+// One request a lane: its first token, tokens, keys, column blocks and
+// CHUNK_KEYS runs of keys. (Offsets and lengths are held to the rows and the
+// table that there are.)
+struct Req {
+    int q0, n, len, blocks, runs;
+};
+__device__ __forceinline__ Req load_req(const PagedArgs &a, int r) {
+    Req q;
+    const bool in = r < a.R;
+    q.q0 = in ? min(max(a.cu_q[r], 0), a.T) : 0;
+    q.n = in ? min(max(a.cu_q[r + 1], q.q0), a.T) - q.q0 : 0;
+    q.len = in ? min(max(a.kv_lens[r], 0), a.W << a.page_log2) : 0;
+    q.blocks = (q.n * a.G + 31) >> 5;
+    q.runs = (q.len + CHUNK_KEYS - 1) / CHUNK_KEYS;
+    return q;
+}
+
+// The work of one workgroup beside its kv head.
+struct PagedItem {
+    int r;           // request, < 0: none
+    int q0, n, len;  // its first token, its tokens, its keys
+    int cb;          // column block
+    int split, ns;   // chunk of the block's keys, chunks
+    int runs;        // CHUNK_KEYS runs a chunk
+    int first;       // the block's first item
+};
+
+// Item u (BLOCK: the first item of column block u) in the order of requests, of
+// their blocks, of their chunks. Every wave finds it by itself, 64 requests a
+// step: first the runs of all blocks, which give the size of a chunk, then the
+// chunks up to its own.
+template <bool BLOCK>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
-    int before = 0;
-    for (int r0 = 0; r0 < a.R; r0 += 64) {
-        const int r = r0 + lane;
-        const bool in = r < a.R;
-        // (offsets held to the rows that there are)
-        const int c0 = in ? min(max(a.cu_q[r], 0), a.T) : 0;
-        const int c1 = in ? min(max(a.cu_q[r + 1], c0), a.T) : 0;
-        const int len = in ? min(max(a.kv_lens[r], 0), a.W << a.page_log2) : 0;
-        const int blocks = ((c1 - c0) * a.G + 31) >> 5;
-        const int end = before + wave_scan(blocks);
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(end > u);
-        if (mine) {
-            const int l = __builtin_ctzll(mine);
-            const int q0 = __builtin_amdgcn_readlane(c0, l);
-            return {r0 + l, q0, __builtin_amdgcn_readlane(c1, l) - q0,
-                    __builtin_amdgcn_readlane(len, l),
-                    u - __builtin_amdgcn_readlane(end - blocks, l)};
+    Req q = load_req(a, lane);
+    int runs = 1 << 30;
+    if (a.part) {
+        // (blocks < 2^16 and runs < 2^23: summed in two halves)
+        uint64_t total = 0;
+        for (int r0 = 0;;) {
+            const uint64_t mine = (uint64_t)(unsigned)q.blocks * (unsigned)q.runs;
+            const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
+            total += (uint64_t)(unsigned)__builtin_amdgcn_readlane(lo, 63) +
+                     ((uint64_t)(unsigned)__builtin_amdgcn_readlane(hi, 63) << 24);
+            r0 += 64;
+            if (r0 >= a.R) break;
+            q = load_req(a, r0 + lane);
+        }
+        total += a.target - 1;
+        runs = total >> 32 ? (int)(total / (unsigned)a.target)
+                           : (int)((unsigned)total / (unsigned)a.target);
+        runs = max(1, runs);
+        if (a.R > 64) q = load_req(a, lane);
+    }
+    int before = 0, items = 0;
+    for (int r0 = 0;;) {
+        const int ns = max(1, (q.runs + runs - 1) / runs);
+        const int mine = q.blocks * ns;
+        const int count = BLOCK ? q.blocks : mine;
+        const int end = before + wave_scan(count);
+        const int item_end = BLOCK ? items + wave_scan(mine) : end;
+        const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            PagedItem it;
+            it.r = r0 + l;
+            it.q0 = __builtin_amdgcn_readlane(q.q0, l);
+            it.n = __builtin_amdgcn_readlane(q.n, l);
+            it.len = __builtin_amdgcn_readlane(q.len, l);
+            it.ns = __builtin_amdgcn_readlane(ns, l);
+            it.runs = runs;
+            const int at = u - __builtin_amdgcn_readlane(end - count, l);
+            it.cb = BLOCK ? at : at / it.ns;
+            it.split = BLOCK ? 0 : at - it.cb * it.ns;
+            it.first = __builtin_amdgcn_readlane(item_end - mine, l) + it.cb * it.ns;
+            return it;
         }
         before = __builtin_amdgcn_readlane(end, 63);
+        if (BLOCK) items = __builtin_amdgcn_readlane(item_end, 63);
+        r0 += 64;
+        if (r0 >= a.R) break;
+        q = load_req(a, r0 + lane);
     }
-    return {-1, 0, 0, 0, 0};
+    PagedItem none;
+    none.r = -1;
+    return none;
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -104,6 +169,11 @@ template <int D> struct PagedLds {
     static constexpr int BYTES = SLOTS > FOLD ? SLOTS : FOLD;
 };
 
+// A chunk's state in the workspace: 32 columns of D sums, then of (l, m).
+template <int D> struct PartState {
+    static constexpr int WORDS = 32 * (D + 2);
+};
+
 // Four waves a workgroup, a column block of one kv head; wave w takes the key
 // tiles w, w + 4, ... into LDS of its own (a K and a V slot, refilled as soon as
 // their reads are in registers), and the four states are folded at the end.
@@ -116,7 +186,7 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h2 = lane >> 5, r = lane & 31;
     const int hk = blockIdx.x;
-    const PagedItem it = find_item(a, blockIdx.y, lane);
+    const PagedItem it = find_item<false>(a, blockIdx.y, lane);
     if (it.r < 0) return;  // (workgroup-uniform)
     const int lp = a.page_log2, idx = it.cb * 32 + r, cols = it.n * a.G;
     const bool ok = idx < cols;
@@ -129,7 +199,10 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     const int full = off + (it.cb * 32) / a.G + 1;
     const int bottom = min(it.cb * 32 + 31, cols - 1);
     const int last = min(off + bottom / a.G + 1, it.len);
-    const int ntiles = last > 0 ? (last + ATT_KT - 1) / ATT_KT : 0;
+    // the chunk's key tiles
+    const int all = last > 0 ? (last + ATT_KT - 1) / ATT_KT : 0;
+    const int t0 = it.split * it.runs * PA_WAVES + wave;
+    const int ntiles = it.ns > 1 ? min(all, (it.split + 1) * it.runs * PA_WAVES) : all;
     const int *row_of = a.table + (int64_t)it.r * a.W;
     const int64_t head_rows = (int64_t)1 << lp;
 
@@ -151,26 +224,26 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
         };
         // the tile's first and second 16 rows of the kv head, as row numbers
         auto rows_of = [&](int kt, int64_t &lo, int64_t &hi) __attribute__((always_inline)) {
-            const int l = ((kt - wave) / PA_WAVES) & 63, key = kt * ATT_KT;
+            const int l = ((kt - t0) / PA_WAVES) & 63, key = kt * ATT_KT;
             const int64_t mask = head_rows - 1;
             lo = (((int64_t)__builtin_amdgcn_readlane(id0, l) * a.HK + hk) << lp) + (key & mask);
             hi = (((int64_t)__builtin_amdgcn_readlane(id1, l) * a.HK + hk) << lp) +
                  ((key + 16) & mask);
         };
-        if (wave < ntiles) {
-            pages_from(wave);
+        if (t0 < ntiles) {
+            pages_from(t0);
             int64_t lo, hi;
-            rows_of(wave, lo, hi);
-            const int left = it.len - wave * ATT_KT;
+            rows_of(t0, lo, hi);
+            const int left = it.len - t0 * ATT_KT;
             dma_paged_tile<T, D, false>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left, ks, lane);
             dma_paged_tile<T, D, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left, vs, lane);
         }
-        for (int kt = wave; kt < ntiles; kt += PA_WAVES) {  // wave-uniform
+        for (int kt = t0; kt < ntiles; kt += PA_WAVES) {  // wave-uniform
             const int nx = kt + PA_WAVES;
             const bool more = nx < ntiles;
             int64_t lo = 0, hi = 0;
             if (more) {
-                if ((((nx - wave) / PA_WAVES) & 63) == 0) pages_from(nx);
+                if ((((nx - t0) / PA_WAVES) & 63) == 0) pages_from(nx);
                 rows_of(nx, lo, hi);
             }
             const int left = it.len - nx * ATT_KT;
@@ -217,9 +290,136 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     __syncthreads();
     if (wave >= D / 32) return;
     const Fold f = fold_streams<D>(part, wave, lane);
+    if (it.ns > 1) {  // (workgroup-uniform)
+        const float l = f.l + __shfl_xor(f.l, 32, 64);
+        float *o = a.part + ((int64_t)blockIdx.y * a.HK + hk) * PartState<D>::WORDS;
+        if (!ok) return;
+        float *oc = o + r * D + 32 * wave + 4 * h2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(float4 *)(oc + 8 * j) = f.o[j];
+        if (wave == 0 && h2 == 0) *(float2 *)(o + 32 * D + 2 * r) = make_float2(l, f.m);
+        return;
+    }
     const float inv = row_inv(f.l);
     if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
 #endif
+}
+
+// The chunks of four columns of a block: out = sum_s w_s O_s / sum_s w_s l_s
+// with w_s = 2^(m_s - max m). A column takes D / 4 lanes of four values; the
+// workgroup's groups of four columns take every so manyth chunk, in order, and
+// the groups are added in order.
+constexpr int COMBINE_COLS = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedArgs a) {
+#pragma clang fp contract(off)
+    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * COMBINE_COLS), IN_FLIGHT = 4;
+    __shared__ float4 acc[GROUPS][COMBINE_COLS][LANES];
+    __shared__ float2 lm[GROUPS][COMBINE_COLS];
+    const int hk = blockIdx.x;
+    const PagedItem it = find_item<true>(a, blockIdx.y, threadIdx.x & 63);
+    if (it.r < 0 || it.ns == 1) return;
+    const int left = it.n * a.G - it.cb * 32;
+    if ((int)blockIdx.z * COMBINE_COLS >= left) return;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    const int col = blockIdx.z * COMBINE_COLS + sub % COMBINE_COLS, g = sub / COMBINE_COLS;
+    const bool ok = col < left;
+    const float *base = a.part + ((int64_t)it.first * a.HK + hk) * PartState<D>::WORDS;
+    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS;
+    const float *po = base + (ok ? col : 0) * D + 4 * lane;
+    const float *pl = base + 32 * D + 2 * (ok ? col : 0);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f, m = -INFINITY;
+    for (int s0 = g; s0 < it.ns; s0 += GROUPS * IN_FLIGHT) {
+        float4 v[IN_FLIGHT];
+        float2 w[IN_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; ++i) {
+            const int s = s0 + GROUPS * i;
+            v[i] = *(const float4 *)(po + (s < it.ns ? s : g) * step);
+            w[i] = *(const float2 *)(pl + (s < it.ns ? s : g) * step);
+        }
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; ++i) {
+            if (s0 + GROUPS * i < it.ns) {
+                const MergeCoef c = merge_coef(m, w[i].y);
+                o.x = merge_one(o.x, v[i].x, c);
+                o.y = merge_one(o.y, v[i].y, c);
+                o.z = merge_one(o.z, v[i].z, c);
+                o.w = merge_one(o.w, v[i].w, c);
+                l = merge_one(l, w[i].x, c);
+                m = c.m_new;
+            }
+        }
+    }
+    acc[g][sub % COMBINE_COLS][lane] = o;
+    if (lane == 0) lm[g][sub % COMBINE_COLS] = make_float2(l, m);
+    __syncthreads();
+    if (g || !ok) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) {
+        const float4 b = acc[i][sub][lane];
+        const float2 w = lm[i][sub];
+        const MergeCoef c = merge_coef(m, w.y);
+        o.x = merge_one(o.x, b.x, c);
+        o.y = merge_one(o.y, b.y, c);
+        o.z = merge_one(o.z, b.z, c);
+        o.w = merge_one(o.w, b.w, c);
+        l = merge_one(l, w.x, c);
+        m = c.m_new;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int idx = it.cb * 32 + col, tok = idx / a.G;
+    T *orow = (T *)a.out + ((int64_t)(it.q0 + tok) * a.H + hk * a.G + (idx - tok * a.G)) * D;
+    const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    st8(orow + 4 * lane, pack4<T>(e));
+}
+
+// ---------------------------------------------------------------------------
+// dispatch
+
+// Workgroups of a launch. blocks: a bound on the column blocks (n G / 32 of a
+// request, rounded up); a chunk is one run or more, so there are at most
+// `target` chunks and the last, shorter one of every block, and no more than
+// runs of the table's rows. Few blocks: as many chunks as one round of
+// workgroups takes with those last ones; many: four rounds' worth, so that what
+// the last round leaves idle is small.
+struct PagedGrid {
+    int64_t blocks, items, target;
+    bool cut;
+};
+inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t HK, int64_t D,
+                            int64_t page) {
+    PagedGrid g;
+    g.blocks = T * G / 32 + (R < T ? R : T);
+    const int64_t slots = D == 128 ? 512 : 1024;  // workgroups the chip holds
+    const int64_t runs = ceil_div(W * page, CHUNK_KEYS);
+    const int64_t few = slots - g.blocks * HK;
+    g.target = (few >= slots / 2 ? few : 4 * slots) / HK;
+    if (g.target < 1) g.target = 1;
+    g.cut = runs > 1;
+    g.items = g.cut ? g.blocks + g.target : g.blocks;
+    if (g.items > g.blocks * runs) g.items = g.blocks * runs;
+    return g;
+}
+
+template <typename T, int D>
+int launch_paged(PagedArgs a, const PagedGrid &g, hipStream_t st) {
+    paged_wave_kernel<T, D><<<dim3((unsigned)a.HK, (unsigned)(a.part ? g.items : g.blocks)),
+                              64 * PA_WAVES, 0, st>>>(a);
+    if (a.part) {
+        const int64_t cols = (int64_t)a.T * a.G < 32 ? (int64_t)a.T * a.G : 32;
+        paged_combine_kernel<T, D><<<dim3((unsigned)a.HK, (unsigned)g.blocks,
+                                          (unsigned)ceil_div(cols, COMBINE_COLS)),
+                                     256, 0, st>>>(a);
+    }
+    return launch_status("paged attention");
+}
+
+bool page_log2_of(int64_t page, int &lp) {
+    for (lp = 4; lp <= 8; ++lp)
+        if (page == (1 << lp)) return true;
+    return false;
 }
 
 }  // namespace
@@ -227,25 +427,33 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
 
 using namespace mi;
 
+extern "C" int64_t mi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t table_width,
+                                                      int64_t H, int64_t HK, int64_t D,
+                                                      int64_t page_size) {
+    if (T <= 0 || R <= 0 || table_width <= 0 || H <= 0 || HK <= 0 || H % HK ||
+        (D != 64 && D != 128) || page_size <= 0)
+        return 0;
+    const PagedGrid g = paged_grid(T, R, table_width, H / HK, HK, D, page_size);
+    return g.cut ? g.items * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+}
+
 extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages,
                                   void *out, const int32_t *block_table, const int32_t *cu_q,
                                   const int32_t *kv_lens, int64_t T, int64_t R,
                                   int64_t table_width, int64_t H, int64_t HK, int64_t D,
                                   int64_t n_pages, int64_t page_size, float scale, int dtype,
-                                  void *stream) {
+                                  void *workspace, int64_t workspace_bytes, void *stream) {
     if (dtype != MI_BF16 && dtype != MI_F16)
         return fail(MI_ERR_UNSUPPORTED, "paged attention covers bf16 and fp16 (dtype code %d)", dtype);
     if (D != 64 && D != 128)
         return fail(MI_ERR_UNSUPPORTED, "paged attention head dim %lld", (long long)D);
-    int lp = -1;
-    for (int l = 4; l <= 8; ++l)
-        if (page_size == (1 << l)) lp = l;
-    if (lp < 0)
+    int lp;
+    if (!page_log2_of(page_size, lp))
         return fail(MI_ERR_UNSUPPORTED, "page size %lld; this build covers 16, 32, 64, 128, 256",
                     (long long)page_size);
     if (T < 0 || R < 0 || H < 1 || HK < 1 || H % HK || HK > 65535 || table_width < 1 ||
         n_pages < 1 || n_pages > (0x7fffffff >> lp) || table_width > (0x3fffffff >> lp) ||
-        T * (H / HK) > 0x3fffffff || R > 0x3fffffff)
+        T > 0x3fffffff || T * (H / HK) > 0x3fffffff || R > 0x3fffffff)
         return fail(MI_ERR_ARG, "paged attention shape T=%lld R=%lld table width %lld H=%lld HK=%lld "
                     "pages=%lld", (long long)T, (long long)R, (long long)table_width, (long long)H,
                     (long long)HK, (long long)n_pages);
@@ -254,28 +462,21 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
         return fail(MI_ERR_ARG, "null pointer");
     if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 8))
         return fail(MI_ERR_ARG, "q and the pages must be 16-byte aligned, out 8-byte aligned");
-    const int64_t G = H / HK;
-    const int64_t items = T * G / 32 + (R < T ? R : T);  // a bound on the column blocks
-    if (items > 65535)
-        return fail(MI_ERR_ARG, "paged attention: %lld column blocks", (long long)items);
+    const PagedGrid g = paged_grid(T, R, table_width, H / HK, HK, D, page_size);
+    if (g.items > 65535 || g.blocks > 65535)
+        return fail(MI_ERR_ARG, "paged attention: %lld column blocks (tokens x q heads of a kv head "
+                    "/ 32, and requests), at most 65535", (long long)g.blocks);
+    const int64_t need = g.cut ? g.items * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+    float *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16)
+                    ? (float *)workspace : nullptr;
     const float sl = scale * 1.4426950408889634f;
     // (a scale of 0 as the smallest normal: masked scores stay -inf; NaN stays NaN)
     const float mag = fabsf(sl) < 1.17549435e-38f ? 1.17549435e-38f : fabsf(sl);
-    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, (int)T, (int)R,
-                         (int)table_width, (int)H, (int)HK, (int)G, (int)n_pages, lp, mag,
-                         sl < 0.0f ? 0x80008000u : 0u};
+    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, ws, (int)T, (int)R,
+                         (int)table_width, (int)H, (int)HK, (int)(H / HK), (int)n_pages, lp,
+                         (int)g.target, mag, sl < 0.0f ? 0x80008000u : 0u};
     hipStream_t st = as_stream(stream);
-    const dim3 grid((unsigned)HK, (unsigned)items);
-    if (dtype == MI_BF16) {
-        if (D == 128)
-            paged_wave_kernel<bf16, 128><<<grid, 64 * PA_WAVES, 0, st>>>(a);
-        else
-            paged_wave_kernel<bf16, 64><<<grid, 64 * PA_WAVES, 0, st>>>(a);
-    } else {
-        if (D == 128)
-            paged_wave_kernel<f16, 128><<<grid, 64 * PA_WAVES, 0, st>>>(a);
-        else
-            paged_wave_kernel<f16, 64><<<grid, 64 * PA_WAVES, 0, st>>>(a);
-    }
-    return launch_status("paged attention");
+    if (dtype == MI_BF16)
+        return D == 128 ? launch_paged<bf16, 128>(a, g, st) : launch_paged<bf16, 64>(a, g, st);
+    return D == 128 ? launch_paged<f16, 128>(a, g, st) : launch_paged<f16, 64>(a, g, st);
 }
