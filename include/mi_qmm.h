@@ -362,7 +362,9 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
  * its keys kv_lens[r] (these tokens' own among them); its token i sees keys
  * j <= kv_lens[r] - n + i with n its tokens (a token that sees none gives 0). Rows of
  * out behind the last request's are left as they were. Page ids outside the pool
- * are held to it. bf16 and fp16, D in {64, 128}. With a workspace of
+ * are held to it. max_q_len: the most tokens a request brings, 0 if unknown; it
+ * chooses the kernels (no request of more than 32 rows of a kv head, or some),
+ * and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a workspace of
  * mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte
  * aligned, no initialization needed) long rows' keys are split over workgroups
  * and a second launch adds the parts: the same sums in another order, which
@@ -370,12 +372,13 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
  * misaligned: one workgroup a block of query rows. Calls sharing a workspace must
  * not overlap. */
 int64_t mi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t table_width, int64_t H,
-                                           int64_t HK, int64_t D, int64_t page_size);
+                                           int64_t HK, int64_t D, int64_t page_size,
+                                           int64_t max_q_len);
 int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages, void *out,
                        const int32_t *block_table, const int32_t *cu_q, const int32_t *kv_lens,
                        int64_t T, int64_t R, int64_t table_width, int64_t H, int64_t HK, int64_t D,
-                       int64_t n_pages, int64_t page_size, float scale, int dtype,
-                       void *workspace, int64_t workspace_bytes, void *stream);
+                       int64_t n_pages, int64_t page_size, int64_t max_q_len, float scale,
+                       int dtype, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Log probabilities (no counterpart in the reference, which samples greedily):
  * logits T [rows, V] (row stride row_stride elements), lse their row's log sum

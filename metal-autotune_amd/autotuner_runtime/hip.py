@@ -79,8 +79,8 @@ SIGNATURES: dict[str, list] = {
     "mi_norm_rope_paged": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P,
                            _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P],
     "mi_paged_attention": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-                           _I64, _F, _I, _P, _I64, _P],
-    "mi_paged_attention_workspace_bytes": [_I64] * 7,
+                           _I64, _I64, _F, _I, _P, _I64, _P],
+    "mi_paged_attention_workspace_bytes": [_I64] * 8,
     "mi_token_logprobs": [_P, _I64, _I64, _I64, _P, _I, _I, _P, _P, _P, _P, _I, _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
@@ -434,25 +434,27 @@ def b_sdpa(ins, outs, p):
     sdpa(q, k, v, o, Lk, Lk, float(p["scale"]), int(p.get("causal", 1)), layout)
 
 
-def paged_attention(q, k_pages, v_pages, out, table, cu_q, kv_lens, scale: float) -> None:
+def paged_attention(q, k_pages, v_pages, out, table, cu_q, kv_lens, scale: float,
+                    max_q_len: int = 0) -> None:
     """mi_paged_attention over checked tensors, with the workspace of the split
     keys' partial states."""
     T, H, D = q.shape
     n_pages, HK, page, _ = k_pages.shape
     R, width = table.shape
     stream = _stream(q)
-    nbytes = _paged_workspace_bytes(T, R, width, H, HK, D, page)
+    nbytes = _paged_workspace_bytes(T, R, width, H, HK, D, page, max_q_len)
     ws = _workspace("paged", q.device, stream, nbytes, 4 << 20) if nbytes else None
     _check(lib().mi_paged_attention(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(table),
                                     _ptr(cu_q), _ptr(kv_lens), T, R, width, H, HK, D, n_pages,
-                                    page, scale, _dt(q), _ptr(ws), nbytes, stream),
+                                    page, max_q_len, scale, _dt(q), _ptr(ws), nbytes, stream),
            "paged_attention")
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_workspace_bytes(T, R, width, H, HK, D, page) -> int:
+def _paged_workspace_bytes(T, R, width, H, HK, D, page, max_q_len) -> int:
     """mi_paged_attention_workspace_bytes, a function of these numbers alone."""
-    return int(lib().mi_paged_attention_workspace_bytes(T, R, width, H, HK, D, page))
+    return int(lib().mi_paged_attention_workspace_bytes(T, R, width, H, HK, D, page,
+                                                          max_q_len))
 
 
 def b_swiglu(ins, outs, p):

@@ -449,7 +449,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale: floa
     hip._require_gpu(q)
     q = q.contiguous()
     out = torch.empty_like(q)
-    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, float(scale))
+    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, float(scale),
+                        0 if max_q_len is None else int(max_q_len))
     return out
 
 

@@ -33,6 +33,7 @@ struct PagedArgs {
     float *part;  // partial states, by item and kv head; null: no block is cut
     int T, R, W, H, HK, G, pages, page_log2;
     int target;     // chunks wanted for a kv head
+    int wide_runs;  // the least runs of a wide block's chunk
     float scale;    // > 0, log2 units
     uint32_t flip;  // sign bits of a negative scale, for Q
 };
@@ -54,19 +55,23 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 constexpr int CHUNK_KEYS = ATT_KT * PA_WAVES;  // keys are cut in multiples of this
 
-// One request a lane: its first token, tokens, keys, column blocks and
-// CHUNK_KEYS runs of keys. (Offsets and lengths are held to the rows and the
-// table that there are.)
+// One request a lane: its first token, tokens, keys, column blocks (wide: of
+// WIDE_COLS columns) and CHUNK_KEYS runs of keys. (Offsets and lengths are held
+// to the rows and the table that there are.)
+constexpr int WIDE_COLS = 128;
 struct Req {
-    int q0, n, len, blocks, runs;
+    int q0, n, len, wide, narrow, runs;
 };
-__device__ __forceinline__ Req load_req(const PagedArgs &a, int r) {
+template <bool WIDE> __device__ __forceinline__ Req load_req(const PagedArgs &a, int r) {
     Req q;
     const bool in = r < a.R;
     q.q0 = in ? min(max(a.cu_q[r], 0), a.T) : 0;
     q.n = in ? min(max(a.cu_q[r + 1], q.q0), a.T) - q.q0 : 0;
     q.len = in ? min(max(a.kv_lens[r], 0), a.W << a.page_log2) : 0;
-    q.blocks = (q.n * a.G + 31) >> 5;
+    const int cols = q.n * a.G;
+    const bool wide = WIDE && cols > 32;
+    q.wide = wide ? (cols + WIDE_COLS - 1) / WIDE_COLS : 0;
+    q.narrow = wide ? 0 : (cols + 31) >> 5;
     q.runs = (q.len + CHUNK_KEYS - 1) / CHUNK_KEYS;
     return q;
 }
@@ -74,71 +79,80 @@ __device__ __forceinline__ Req load_req(const PagedArgs &a, int r) {
 // The work of one workgroup beside its kv head.
 struct PagedItem {
     int r;           // request, < 0: none
+    bool wide;
     int q0, n, len;  // its first token, its tokens, its keys
     int cb;          // column block
     int split, ns;   // chunk of the block's keys, chunks
     int runs;        // CHUNK_KEYS runs a chunk
-    int first;       // the block's first item
+    int part;        // the chunk's state in the workspace, in states of 32 columns
 };
 
-// Item u (BLOCK: the first item of column block u) in the order of requests, of
-// their blocks, of their chunks. Every wave finds it by itself, 64 requests a
-// step: first the runs of all blocks, which give the size of a chunk, then the
-// chunks up to its own.
-template <bool BLOCK>
+// Item u (BLOCK: the first chunk of column block u): the wide blocks' chunks
+// first, each kind in the order of requests, of their blocks (a wide request's
+// last block, which sees the most keys, first), of their chunks. Every wave
+// finds it by itself, 64 requests a step: first the runs of all blocks, which
+// give the size of a chunk, then the chunks up to its own.
+template <bool WIDE, bool BLOCK>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
-    Req q = load_req(a, lane);
+    Req q = load_req<WIDE>(a, lane);
     int runs = 1 << 30;
     if (a.part) {
         // (blocks < 2^16 and runs < 2^23: summed in two halves)
         uint64_t total = 0;
         for (int r0 = 0;;) {
-            const uint64_t mine = (uint64_t)(unsigned)q.blocks * (unsigned)q.runs;
+            const uint64_t mine = (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)q.runs;
             const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
             total += (uint64_t)(unsigned)__builtin_amdgcn_readlane(lo, 63) +
                      ((uint64_t)(unsigned)__builtin_amdgcn_readlane(hi, 63) << 24);
             r0 += 64;
             if (r0 >= a.R) break;
-            q = load_req(a, r0 + lane);
+            q = load_req<WIDE>(a, r0 + lane);
         }
         total += a.target - 1;
         runs = total >> 32 ? (int)(total / (unsigned)a.target)
                            : (int)((unsigned)total / (unsigned)a.target);
         runs = max(1, runs);
-        if (a.R > 64) q = load_req(a, lane);
     }
-    int before = 0, items = 0;
-    for (int r0 = 0;;) {
-        const int ns = max(1, (q.runs + runs - 1) / runs);
-        const int mine = q.blocks * ns;
-        const int count = BLOCK ? q.blocks : mine;
-        const int end = before + wave_scan(count);
-        const int item_end = BLOCK ? items + wave_scan(mine) : end;
-        const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            PagedItem it;
-            it.r = r0 + l;
-            it.q0 = __builtin_amdgcn_readlane(q.q0, l);
-            it.n = __builtin_amdgcn_readlane(q.n, l);
-            it.len = __builtin_amdgcn_readlane(q.len, l);
-            it.ns = __builtin_amdgcn_readlane(ns, l);
-            it.runs = runs;
-            const int at = u - __builtin_amdgcn_readlane(end - count, l);
-            it.cb = BLOCK ? at : at / it.ns;
-            it.split = BLOCK ? 0 : at - it.cb * it.ns;
-            it.first = __builtin_amdgcn_readlane(item_end - mine, l) + it.cb * it.ns;
-            return it;
+    PagedItem it;
+    it.r = -1;
+    int before = 0, states = 0;  // what u counts, and states of 32 columns
+#pragma unroll
+    for (int kind = WIDE ? 0 : 1; kind < 2; ++kind) {
+        const bool wide = kind == 0;
+        const int per = wide ? max(runs, a.wide_runs) : runs;
+        for (int r0 = 0;;) {
+            if (a.R > 64) q = load_req<WIDE>(a, r0 + lane);
+            const int ns = max(1, (q.runs + per - 1) / per);
+            const int blocks = wide ? q.wide : q.narrow;
+            const int items = blocks * ns, count = BLOCK ? blocks : items;
+            const int end = before + wave_scan(count);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
+            const int scale = wide ? WIDE_COLS / 32 : 1;
+            const int state_end = states + scale * (BLOCK ? wave_scan(items) : end - before);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                it.r = r0 + l;
+                it.wide = wide;
+                it.q0 = __builtin_amdgcn_readlane(q.q0, l);
+                it.n = __builtin_amdgcn_readlane(q.n, l);
+                it.len = __builtin_amdgcn_readlane(q.len, l);
+                it.ns = __builtin_amdgcn_readlane(ns, l);
+                it.runs = per;
+                const int at = u - __builtin_amdgcn_readlane(end - count, l);
+                const int b = BLOCK ? at : at / it.ns;
+                it.split = BLOCK ? 0 : at - b * it.ns;
+                it.cb = wide ? __builtin_amdgcn_readlane(blocks, l) - 1 - b : b;
+                it.part = __builtin_amdgcn_readlane(state_end - scale * items, l) +
+                          scale * (b * it.ns + it.split);
+                return it;
+            }
+            before = __builtin_amdgcn_readlane(end, 63);
+            states = __builtin_amdgcn_readlane(state_end, 63);
+            r0 += 64;
+            if (r0 >= a.R) break;
         }
-        before = __builtin_amdgcn_readlane(end, 63);
-        if (BLOCK) items = __builtin_amdgcn_readlane(item_end, 63);
-        r0 += 64;
-        if (r0 >= a.R) break;
-        q = load_req(a, r0 + lane);
     }
-    PagedItem none;
-    none.r = -1;
-    return none;
+    return it;
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -164,7 +178,7 @@ __device__ __forceinline__ void dma_paged_tile(const T *lo, const T *hi, int lef
 #endif
 
 template <int D> struct PagedLds {
-    static constexpr int SLOTS = PA_WAVES * 2 * Tile<D>::BYTES;
+    static constexpr int SLOTS = PA_WAVES * 2 * Tile<D>::BYTES;  // = two wide stages
     static constexpr int FOLD = PA_WAVES * Part<D>::BYTES;
     static constexpr int BYTES = SLOTS > FOLD ? SLOTS : FOLD;
 };
@@ -174,21 +188,44 @@ template <int D> struct PartState {
     static constexpr int WORDS = 32 * (D + 2);
 };
 
-// Four waves a workgroup, a column block of one kv head; wave w takes the key
-// tiles w, w + 4, ... into LDS of its own (a K and a V slot, refilled as soon as
-// their reads are in registers), and the four states are folded at the end.
-template <typename T, int D>
-__global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
+// The pages of a wave's next 64 tiles kt, kt + STEP, ..., one a lane (a tile of
+// 16-row pages has two), and a tile's first and second 16 rows of the kv head in
+// the pools.
+template <int STEP> struct TilePages {
+    const int *row;
+    int64_t hk;
+    int W, pages, lp, HK;
+    int id0, id1;
+    __device__ __forceinline__ TilePages(const PagedArgs &a, int r, int hk_)
+        : row(a.table + (int64_t)r * a.W), hk(hk_), W(a.W), pages(a.pages), lp(a.page_log2),
+          HK(a.HK), id0(0), id1(0) {}
+    __device__ __forceinline__ void load(int kt, int lane) {
+        const int key = (kt + STEP * lane) * ATT_KT;
+        id0 = min(max(row[min(key >> lp, W - 1)], 0), pages - 1);
+        id1 = min(max(row[min((key + 16) >> lp, W - 1)], 0), pages - 1);
+    }
+    // the tile `at` steps (mod 64) behind the loaded one, of first key `key`
+    __device__ __forceinline__ void rows(int at, int key, int64_t &lo, int64_t &hi) const {
+        const int64_t mask = ((int64_t)1 << lp) - 1;
+        lo = (((int64_t)__builtin_amdgcn_readlane(id0, at & 63) * HK + hk) << lp) + (key & mask);
+        hi = (((int64_t)__builtin_amdgcn_readlane(id1, at & 63) * HK + hk) << lp) +
+             ((key + 16) & mask);
+    }
+};
+
+// A narrow block: wave w takes the key tiles w, w + 4, ... of the chunk into LDS of
+// its own (a K and a V slot, refilled as soon as their reads are in registers: no
+// barrier), and the four states are folded at the end. Bound by HBM: K and V are
+// read once.
+template <typename T, int D>
+__device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem &it, int hk,
+                                             char *lds) {
     typedef Tile<D> Tl;
-    __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h2 = lane >> 5, r = lane & 31;
-    const int hk = blockIdx.x;
-    const PagedItem it = find_item<false>(a, blockIdx.y, lane);
-    if (it.r < 0) return;  // (workgroup-uniform)
-    const int lp = a.page_log2, idx = it.cb * 32 + r, cols = it.n * a.G;
+    const int idx = it.cb * 32 + r, cols = it.n * a.G;
     const bool ok = idx < cols;
     const int tok = (ok ? idx : 0) / a.G, g = (ok ? idx : 0) - tok * a.G;
     const int64_t qrow = (int64_t)(it.q0 + tok) * a.H + hk * a.G + g;
@@ -203,9 +240,6 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     const int all = last > 0 ? (last + ATT_KT - 1) / ATT_KT : 0;
     const int t0 = it.split * it.runs * PA_WAVES + wave;
     const int ntiles = it.ns > 1 ? min(all, (it.split + 1) * it.runs * PA_WAVES) : all;
-    const int *row_of = a.table + (int64_t)it.r * a.W;
-    const int64_t head_rows = (int64_t)1 << lp;
-
     char *kslot = lds + wave * 2 * Tl::BYTES, *vslot = kslot + Tl::BYTES;
     AttnState<D> st;
     attn_init(st);
@@ -213,27 +247,11 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     uint32_t flip = a.flip;
     auto run = [&](char *__restrict__ ks, char *__restrict__ vs) __attribute__((always_inline)) {
         read_q<D>((const T *)a.q + qrow * D, h2, qf);
-        // pages of the wave's next 64 tiles, one a lane (a tile of 16-row pages
-        // has two)
-        int id0 = 0, id1 = 0;
-        auto pages_from = [&](int kt) __attribute__((always_inline)) {
-            const int key = (kt + PA_WAVES * lane) * ATT_KT;
-            const int p0 = min(key >> lp, a.W - 1), p1 = min((key + 16) >> lp, a.W - 1);
-            id0 = min(max(row_of[p0], 0), a.pages - 1);
-            id1 = min(max(row_of[p1], 0), a.pages - 1);
-        };
-        // the tile's first and second 16 rows of the kv head, as row numbers
-        auto rows_of = [&](int kt, int64_t &lo, int64_t &hi) __attribute__((always_inline)) {
-            const int l = ((kt - t0) / PA_WAVES) & 63, key = kt * ATT_KT;
-            const int64_t mask = head_rows - 1;
-            lo = (((int64_t)__builtin_amdgcn_readlane(id0, l) * a.HK + hk) << lp) + (key & mask);
-            hi = (((int64_t)__builtin_amdgcn_readlane(id1, l) * a.HK + hk) << lp) +
-                 ((key + 16) & mask);
-        };
+        TilePages<PA_WAVES> pg(a, it.r, hk);
         if (t0 < ntiles) {
-            pages_from(t0);
+            pg.load(t0, lane);
             int64_t lo, hi;
-            rows_of(t0, lo, hi);
+            pg.rows(0, t0 * ATT_KT, lo, hi);
             const int left = it.len - t0 * ATT_KT;
             dma_paged_tile<T, D, false>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left, ks, lane);
             dma_paged_tile<T, D, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left, vs, lane);
@@ -243,8 +261,9 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
             const bool more = nx < ntiles;
             int64_t lo = 0, hi = 0;
             if (more) {
-                if ((((nx - t0) / PA_WAVES) & 63) == 0) pages_from(nx);
-                rows_of(nx, lo, hi);
+                const int at = (nx - t0) / PA_WAVES;
+                if ((at & 63) == 0) pg.load(nx, lane);
+                pg.rows(at, nx * ATT_KT, lo, hi);
             }
             const int left = it.len - nx * ATT_KT;
             // K (and, the first time, q) has landed once only V's loads, issued
@@ -292,7 +311,7 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     const Fold f = fold_streams<D>(part, wave, lane);
     if (it.ns > 1) {  // (workgroup-uniform)
         const float l = f.l + __shfl_xor(f.l, 32, 64);
-        float *o = a.part + ((int64_t)blockIdx.y * a.HK + hk) * PartState<D>::WORDS;
+        float *o = a.part + ((int64_t)it.part * a.HK + hk) * PartState<D>::WORDS;
         if (!ok) return;
         float *oc = o + r * D + 32 * wave + 4 * h2;
 #pragma unroll
@@ -302,6 +321,130 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
     }
     const float inv = row_inv(f.l);
     if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
+}
+
+// A wide block: wave w has the columns 32 w .. 32 w + 31 of the block's 128, and
+// all four share each stage of two key tiles, staged by DMA into one of two
+// buffers while the other is read: K and V pass through LDS once for 128 columns
+// where a narrow block's pass for 32.
+template <typename T, int D>
+__device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &it, int hk,
+                                           char *lds) {
+    typedef Tile<D> Tl;
+    constexpr int STAGE = 4 * Tl::BYTES;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h2 = lane >> 5, r = lane & 31;
+    const int cols = it.n * a.G, c0 = it.cb * WIDE_COLS + 32 * wave, idx = c0 + r;
+    const bool ok = idx < cols;
+    const int tok = (ok ? idx : 0) / a.G, g = (ok ? idx : 0) - tok * a.G;
+    const int64_t qrow = (int64_t)(it.q0 + tok) * a.H + hk * a.G + g;
+    const int off = it.len - it.n, end = off + tok + 1, full = off + c0 / a.G + 1;
+    // key tiles that the wave's columns see, and the block's
+    auto tiles_to = [&](int col) {
+        const int last = min(off + min(col, cols - 1) / a.G + 1, it.len);
+        return last > 0 ? (last + ATT_KT - 1) / ATT_KT : 0;
+    };
+    const int t0 = it.split * it.runs * PA_WAVES;
+    const int stop = it.ns > 1 ? (it.split + 1) * it.runs * PA_WAVES : 1 << 30;
+    const int t1 = min(tiles_to(it.cb * WIDE_COLS + WIDE_COLS - 1), stop);
+    const int mine = c0 < cols ? min(tiles_to(c0 + 31), stop) : 0;
+
+    AttnState<D> st;
+    attn_init(st);
+    uint4 qf[D / 16];
+    uint32_t flip = a.flip;
+    read_q<D>((const T *)a.q + qrow * D, h2, qf);
+    // stage s: key tiles t0 + 2 s, t0 + 2 s + 1; waves 0 and 1 stage K, 2 and 3 V
+    TilePages<2> pg(a, it.r, hk);
+    const T *pool = (const T *)(wave < 2 ? a.k : a.v);
+    auto issue = [&](int s, char *dst) __attribute__((always_inline)) {
+        const int kt = t0 + 2 * s + (wave & 1);
+        if ((s & 63) == 0) pg.load(kt, lane);
+        int64_t lo, hi;
+        pg.rows(s, kt * ATT_KT, lo, hi);
+        const int left = it.len - kt * ATT_KT;
+        if (wave < 2)
+            dma_paged_tile<T, D, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+        else
+            dma_paged_tile<T, D, true>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+    };
+    auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more)
+                    __attribute__((always_inline)) {
+        // every wave's DMAs of stage s have landed, and every wave is done with
+        // the buffer the next ones go to
+        att_wait_vmcnt<0>();
+        __syncthreads();
+        flip_q<D>(qf, flip);
+        if (more) issue(s + 1, nb);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int kt = t0 + 2 * s + j;
+            if (kt < mine) {  // wave-uniform
+                uint4 kf[D / 16];
+                read_k<D>(cb + j * Tl::BYTES, kf, r, h2);
+                VFrag<T, D> vf;
+                read_v<T, D>(cb + (2 + j) * Tl::BYTES, vf, lane);
+                __builtin_amdgcn_sched_barrier(0);  // (not sunk to the PV MFMAs)
+                f32x16 sc = attn_scores<T, D>(kf, qf);
+                const int k0 = kt * ATT_KT;
+                if (k0 + ATT_KT > full) attn_mask(sc, end - k0, h2);
+                uint32_t p[8];
+                attn_softmax<T, D>(st, sc, p, a.scale);
+                attn_pv<T, D>(st, p, vf);
+            }
+        }
+    };
+    const int stages = t1 > t0 ? (t1 - t0 + 1) / 2 : 0;
+    char *b0 = lds, *b1 = lds + STAGE;
+    if (stages) issue(0, b0);
+    for (int s = 0; s < stages; s += 2) {  // workgroup-uniform
+        step(b0, b1, s, s + 1 < stages);
+        if (s + 1 < stages) step(b1, b0, s + 1, s + 2 < stages);
+    }
+    if (!ok) return;
+    if (it.ns > 1) {
+        float *o = a.part + ((int64_t)(it.part + wave) * a.HK + hk) * PartState<D>::WORDS;
+        const float l = st.l + __shfl_xor(st.l, 32, 64);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(float4 *)(o + r * D + 32 * t + 4 * h2 + 8 * j) =
+                    make_float4(st.o[t][4 * j], st.o[t][4 * j + 1], st.o[t][4 * j + 2], st.o[t][4 * j + 3]);
+        if (h2 == 0) *(float2 *)(o + 32 * D + 2 * r) = make_float2(l, st.m);
+        return;
+    }
+    const float inv = row_inv(st.l);
+    T *orow = (T *)a.out + qrow * D;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e[4] = {st.o[t][4 * j] * inv, st.o[t][4 * j + 1] * inv,
+                                st.o[t][4 * j + 2] * inv, st.o[t][4 * j + 3] * inv};
+            st8(orow + 32 * t + 8 * j + 4 * h2, pack4<T>(e));
+        }
+}
+#endif
+
+// Workgroups a CU holds, a wave a SIMD each (four of the wide form with heads of 64
+// would spill).
+template <int D, bool WIDE> constexpr int paged_per_cu() { return D == 128 ? 2 : (WIDE ? 3 : 4); }
+
+// One workgroup an item and kv head. WIDE: requests of more than 32 columns are in
+// wide blocks; without it (decode) every block is narrow.
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(64 * PA_WAVES) __attribute__((amdgpu_waves_per_eu(paged_per_cu<D, WIDE>())))
+void paged_attn_kernel(PagedArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
+    const PagedItem it = find_item<WIDE, false>(a, blockIdx.y, threadIdx.x & 63);
+    if (it.r < 0) return;  // (workgroup-uniform)
+    if (WIDE && it.wide)
+        wide_block<T, D>(a, it, blockIdx.x, lds);
+    else
+        narrow_block<T, D>(a, it, blockIdx.x, lds);
 #endif
 }
 
@@ -310,24 +453,27 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_wave_kernel(PagedArgs a) 
 // workgroup's groups of four columns take every so manyth chunk, in order, and
 // the groups are added in order.
 constexpr int COMBINE_COLS = 4;
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedArgs a) {
 #pragma clang fp contract(off)
     constexpr int LANES = D / 4, GROUPS = 256 / (LANES * COMBINE_COLS), IN_FLIGHT = 4;
     __shared__ float4 acc[GROUPS][COMBINE_COLS][LANES];
     __shared__ float2 lm[GROUPS][COMBINE_COLS];
     const int hk = blockIdx.x;
-    const PagedItem it = find_item<true>(a, blockIdx.y, threadIdx.x & 63);
+    const PagedItem it = find_item<WIDE, true>(a, blockIdx.y, threadIdx.x & 63);
     if (it.r < 0 || it.ns == 1) return;
-    const int left = it.n * a.G - it.cb * 32;
+    const int cols = WIDE && it.wide ? WIDE_COLS : 32;
+    const int left = min(it.n * a.G - it.cb * cols, cols);
     if ((int)blockIdx.z * COMBINE_COLS >= left) return;
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const int col = blockIdx.z * COMBINE_COLS + sub % COMBINE_COLS, g = sub / COMBINE_COLS;
     const bool ok = col < left;
-    const float *base = a.part + ((int64_t)it.first * a.HK + hk) * PartState<D>::WORDS;
-    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS;
-    const float *po = base + (ok ? col : 0) * D + 4 * lane;
-    const float *pl = base + 32 * D + 2 * (ok ? col : 0);
+    const int c = ok ? col : 0;
+    const float *base =
+        a.part + ((int64_t)(it.part + (c >> 5)) * a.HK + hk) * PartState<D>::WORDS;
+    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS * (cols >> 5);
+    const float *po = base + (c & 31) * D + 4 * lane;
+    const float *pl = base + 32 * D + 2 * (c & 31);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f, m = -INFINITY;
     for (int s0 = g; s0 < it.ns; s0 += GROUPS * IN_FLIGHT) {
@@ -369,7 +515,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedArgs a) {
         m = c.m_new;
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int idx = it.cb * 32 + col, tok = idx / a.G;
+    const int idx = it.cb * cols + col, tok = idx / a.G;
     T *orow = (T *)a.out + ((int64_t)(it.q0 + tok) * a.H + hk * a.G + (idx - tok * a.G)) * D;
     const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     st8(orow + 4 * lane, pack4<T>(e));
@@ -378,42 +524,76 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedArgs a) {
 // ---------------------------------------------------------------------------
 // dispatch
 
-// Workgroups of a launch. blocks: a bound on the column blocks (n G / 32 of a
-// request, rounded up); a chunk is one run or more, so there are at most
-// `target` chunks and the last, shorter one of every block, and no more than
-// runs of the table's rows. Few blocks: as many chunks as one round of
+// Workgroups of a launch. wide and narrow bound the blocks of each kind (n G / 128
+// or n G / 32 of a request, rounded up). A chunk is one run or more, so there are
+// at most `target` chunks and the last, shorter one of every block, and no more
+// than a row of the table has. Few blocks: as many chunks as one round of
 // workgroups takes with those last ones; many: four rounds' worth, so that what
-// the last round leaves idle is small.
+// the last round leaves idle is small, and wide blocks, whose parts cost 66 KB
+// written and read, only past 32 runs.
 struct PagedGrid {
-    int64_t blocks, items, target;
-    bool cut;
+    int64_t wide, narrow, items, states, target, wide_runs;
+    bool cut, cut_wide;
 };
 inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t HK, int64_t D,
-                            int64_t page) {
+                            int64_t page, int64_t max_q) {
     PagedGrid g;
-    g.blocks = T * G / 32 + (R < T ? R : T);
-    const int64_t slots = D == 128 ? 512 : 1024;  // workgroups the chip holds
+    const int64_t some = R < T ? R : T;
+    if (max_q * G > 32) {
+        const int64_t most = T * G / 33 < some ? T * G / 33 : some;  // requests that can be wide
+        g.wide = T * G / WIDE_COLS + most;
+        g.narrow = some;
+    } else {
+        g.wide = 0;
+        g.narrow = T * G / 32 + some;
+    }
+    const int64_t slots = 256 * (D == 128 ? paged_per_cu<128, true>()
+                                          : g.wide ? paged_per_cu<64, true>()
+                                                   : paged_per_cu<64, false>());
     const int64_t runs = ceil_div(W * page, CHUNK_KEYS);
-    const int64_t few = slots - g.blocks * HK;
+    const int64_t few = slots - (g.wide + g.narrow) * HK;
     g.target = (few >= slots / 2 ? few : 4 * slots) / HK;
     if (g.target < 1) g.target = 1;
+    g.wide_runs = few >= slots / 2 ? 1 : 32;
     g.cut = runs > 1;
-    g.items = g.cut ? g.blocks + g.target : g.blocks;
-    if (g.items > g.blocks * runs) g.items = g.blocks * runs;
+    g.cut_wide = g.wide && runs > g.wide_runs;
+    int64_t wide = g.wide, narrow = g.narrow;  // chunks of each kind
+    if (g.cut_wide) {
+        const int64_t most = g.wide * ceil_div(runs, g.wide_runs);
+        wide = g.wide + g.target < most ? g.wide + g.target : most;
+    }
+    if (g.cut) {
+        const int64_t most = g.narrow * runs;
+        narrow = g.narrow + g.target < most ? g.narrow + g.target : most;
+    }
+    g.items = wide + narrow;
+    if (g.items > g.wide + g.narrow + g.target) g.items = g.wide + g.narrow + g.target;
+    g.states = wide * (WIDE_COLS / 32) + narrow;
     return g;
 }
+inline int64_t paged_bytes(const PagedGrid &g, int64_t HK, int64_t D) {
+    return g.cut ? g.states * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+}
 
-template <typename T, int D>
-int launch_paged(PagedArgs a, const PagedGrid &g, hipStream_t st) {
-    paged_wave_kernel<T, D><<<dim3((unsigned)a.HK, (unsigned)(a.part ? g.items : g.blocks)),
-                              64 * PA_WAVES, 0, st>>>(a);
+template <typename T, int D, bool WIDE>
+int launch_paged_w(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
+    const int64_t blocks = g.wide + g.narrow;
+    paged_attn_kernel<T, D, WIDE><<<dim3((unsigned)a.HK, (unsigned)(a.part ? g.items : blocks)),
+                                    64 * PA_WAVES, 0, st>>>(a);
     if (a.part) {
-        const int64_t cols = (int64_t)a.T * a.G < 32 ? (int64_t)a.T * a.G : 32;
-        paged_combine_kernel<T, D><<<dim3((unsigned)a.HK, (unsigned)g.blocks,
-                                          (unsigned)ceil_div(cols, COMBINE_COLS)),
-                                     256, 0, st>>>(a);
+        // (wide blocks that are never cut come first, and only they have more than
+        // 32 columns: a column group past those is never needed)
+        const int64_t most = g.cut_wide ? WIDE_COLS : 32, all = (int64_t)a.T * a.G;
+        paged_combine_kernel<T, D, WIDE>
+            <<<dim3((unsigned)a.HK, (unsigned)blocks,
+                    (unsigned)ceil_div(all < most ? all : most, COMBINE_COLS)),
+               256, 0, st>>>(a);
     }
     return launch_status("paged attention");
+}
+template <typename T, int D>
+int launch_paged(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
+    return g.wide ? launch_paged_w<T, D, true>(a, g, st) : launch_paged_w<T, D, false>(a, g, st);
 }
 
 bool page_log2_of(int64_t page, int &lp) {
@@ -429,20 +609,21 @@ using namespace mi;
 
 extern "C" int64_t mi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t table_width,
                                                       int64_t H, int64_t HK, int64_t D,
-                                                      int64_t page_size) {
+                                                      int64_t page_size, int64_t max_q_len) {
     if (T <= 0 || R <= 0 || table_width <= 0 || H <= 0 || HK <= 0 || H % HK ||
         (D != 64 && D != 128) || page_size <= 0)
         return 0;
-    const PagedGrid g = paged_grid(T, R, table_width, H / HK, HK, D, page_size);
-    return g.cut ? g.items * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+    return paged_bytes(paged_grid(T, R, table_width, H / HK, HK, D, page_size,
+                                  max_q_len > 0 && max_q_len < T ? max_q_len : T), HK, D);
 }
 
 extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages,
                                   void *out, const int32_t *block_table, const int32_t *cu_q,
                                   const int32_t *kv_lens, int64_t T, int64_t R,
                                   int64_t table_width, int64_t H, int64_t HK, int64_t D,
-                                  int64_t n_pages, int64_t page_size, float scale, int dtype,
-                                  void *workspace, int64_t workspace_bytes, void *stream) {
+                                  int64_t n_pages, int64_t page_size, int64_t max_q_len,
+                                  float scale, int dtype, void *workspace,
+                                  int64_t workspace_bytes, void *stream) {
     if (dtype != MI_BF16 && dtype != MI_F16)
         return fail(MI_ERR_UNSUPPORTED, "paged attention covers bf16 and fp16 (dtype code %d)", dtype);
     if (D != 64 && D != 128)
@@ -462,11 +643,12 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
         return fail(MI_ERR_ARG, "null pointer");
     if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 8))
         return fail(MI_ERR_ARG, "q and the pages must be 16-byte aligned, out 8-byte aligned");
-    const PagedGrid g = paged_grid(T, R, table_width, H / HK, HK, D, page_size);
-    if (g.items > 65535 || g.blocks > 65535)
-        return fail(MI_ERR_ARG, "paged attention: %lld column blocks (tokens x q heads of a kv head "
-                    "/ 32, and requests), at most 65535", (long long)g.blocks);
-    const int64_t need = g.cut ? g.items * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+    const PagedGrid g = paged_grid(T, R, table_width, H / HK, HK, D, page_size,
+                                   max_q_len > 0 && max_q_len < T ? max_q_len : T);
+    if (g.items > 65535)
+        return fail(MI_ERR_ARG, "paged attention: %lld blocks of query rows, at most 65535",
+                    (long long)g.items);
+    const int64_t need = paged_bytes(g, HK, D);
     float *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16)
                     ? (float *)workspace : nullptr;
     const float sl = scale * 1.4426950408889634f;
@@ -474,7 +656,7 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
     const float mag = fabsf(sl) < 1.17549435e-38f ? 1.17549435e-38f : fabsf(sl);
     const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, ws, (int)T, (int)R,
                          (int)table_width, (int)H, (int)HK, (int)(H / HK), (int)n_pages, lp,
-                         (int)g.target, mag, sl < 0.0f ? 0x80008000u : 0u};
+                         (int)g.target, (int)g.wide_runs, mag, sl < 0.0f ? 0x80008000u : 0u};
     hipStream_t st = as_stream(stream);
     if (dtype == MI_BF16)
         return D == 128 ? launch_paged<bf16, 128>(a, g, st) : launch_paged<bf16, 64>(a, g, st);

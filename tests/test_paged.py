@@ -65,7 +65,7 @@ def test_prologue_of_no_tokens(lib):
 
 
 def _attn(L, q=P, T=2, R=2, W=4, H=4, HK=2, D=128, pages=8, page=16, dt=hip.MI_BF16, out=P):
-    return L.mi_paged_attention(q, P, P, out, P, P, P, T, R, W, H, HK, D, pages, page, 0.1, dt,
+    return L.mi_paged_attention(q, P, P, out, P, P, P, T, R, W, H, HK, D, pages, page, 0, 0.1, dt,
                                 None, 0, None)
 
 
