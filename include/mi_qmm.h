@@ -385,13 +385,18 @@ int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages, 
  * exp. logprobs[r] = logits[r, tokens[r]] - lse (NaN for a token outside [0, V));
  * entropy[r] = -sum p log p (a logit of -inf adds 0); the `top` most probable
  * tokens, the lowest index first among equal logits: top_ids int32 [rows, top]
- * and top_logprobs [rows, top]. All fp32. 0 <= top <= 64, top <= V <= 2^30. A row
+ * and top_logprobs [rows, top]. All fp32. 0 <= top <= 64, top <= V <= 2^22. A row
  * with a NaN or +inf, or of -inf alone, gives NaN (its top_ids stay in [0, V)).
- * tokens are int32 or int64 (tokens_are_64). */
+ * tokens are int32 or int64 (tokens_are_64). Few rows are split over workgroups
+ * where a workspace of mi_token_logprobs_workspace_bytes(...) bytes (0: not split;
+ * 16-byte aligned, no initialization needed) is given, and joined by a second
+ * launch: the same results but for the sums' last bits. NULL, short or misaligned:
+ * one workgroup a row. Calls sharing a workspace must not overlap. */
+int64_t mi_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int top, int dtype);
 int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_stride,
                       const void *tokens, int tokens_are_64, int top, float *logprobs,
                       float *entropy, int32_t *top_ids, float *top_logprobs, int dtype,
-                      void *stream);
+                      void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

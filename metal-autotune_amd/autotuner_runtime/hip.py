@@ -81,13 +81,15 @@ SIGNATURES: dict[str, list] = {
     "mi_paged_attention": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                            _I64, _I64, _F, _I, _P, _I64, _P],
     "mi_paged_attention_workspace_bytes": [_I64] * 8,
-    "mi_token_logprobs": [_P, _I64, _I64, _I64, _P, _I, _I, _P, _P, _P, _P, _I, _P],
+    "mi_token_logprobs_workspace_bytes": [_I64, _I64, _I, _I],
+    "mi_token_logprobs": [_P, _I64, _I64, _I64, _P, _I, _I, _P, _P, _P, _P, _I, _P, _I64, _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
             "mi_gelu_mlp_f32_workspace_bytes": ctypes.c_int64,
             "mi_qmm_workspace_bytes": ctypes.c_int64,
             "mi_sdpa_workspace_bytes": ctypes.c_int64,
-            "mi_paged_attention_workspace_bytes": ctypes.c_int64}
+            "mi_paged_attention_workspace_bytes": ctypes.c_int64,
+            "mi_token_logprobs_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -455,6 +457,24 @@ def _paged_workspace_bytes(T, R, width, H, HK, D, page, max_q_len) -> int:
     """mi_paged_attention_workspace_bytes, a function of these numbers alone."""
     return int(lib().mi_paged_attention_workspace_bytes(T, R, width, H, HK, D, page,
                                                           max_q_len))
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace_bytes(rows, V, top, dt) -> int:
+    """mi_token_logprobs_workspace_bytes, a function of these numbers alone."""
+    return int(lib().mi_token_logprobs_workspace_bytes(rows, V, top, dt))
+
+
+def token_logprobs(x, tokens, top: int, logprobs, entropy, ids, top_logprobs) -> None:
+    """mi_token_logprobs over checked tensors, with the workspace of split rows."""
+    rows, V = x.shape
+    dt, stream = _dt(x), _stream(x)
+    nbytes = _logprobs_workspace_bytes(rows, V, top, dt)
+    ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20) if nbytes else None
+    _check(lib().mi_token_logprobs(_ptr(x), rows, V, x.stride(0), _ptr(tokens),
+                                   int(tokens.dtype == torch.int64), top, _ptr(logprobs),
+                                   _ptr(entropy), _ptr(ids), _ptr(top_logprobs), dt, _ptr(ws),
+                                   nbytes, stream), "token_logprobs")
 
 
 def b_swiglu(ins, outs, p):

@@ -485,10 +485,7 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     ids = x.new_empty((*lead, top), dtype=torch.int32)
     out = TokenLogprobs(f32[:rows].view(lead), f32[rows:2 * rows].view(lead), ids,
                         f32[2 * rows:].view(*lead, top))
-    hip._check(hip.lib().mi_token_logprobs(
-        x.data_ptr(), rows, V, x.stride(0), tokens.data_ptr(), int(tokens.dtype == torch.int64),
-        top, out.logprobs.data_ptr(), out.entropy.data_ptr(), ids.data_ptr(),
-        out.top_logprobs.data_ptr(), hip._dt(x), hip._stream(x)), "token_logprobs")
+    hip.token_logprobs(x, tokens, top, *out)
     return out
 
 

@@ -7,13 +7,19 @@
 // One pass over the row. A wave keeps S and E = sum e^d d against a reference
 // that all its lanes share and that moves only when a value passes it by 30: the
 // sums are fp32 and keep their relative precision at any offset, and moving the
-// reference by c turns E into (E - c S) e^-c. The last step refers them to the
+// reference by c turns E into (E + c S) e^c. The last step refers them to the
 // row's true maximum.
 //
-// The likeliest tokens: lane i of a wave holds the wave's i-th best value and
-// index. Values reach the list in index order and only if strictly larger than
-// its last entry, so equal values keep the lowest indices. NaN never enters; a
-// row with a NaN has NaN sums.
+// The k likeliest tokens need no list during the pass, only the maximum of every
+// chunk of 1024 values: ordered by (value descending, index ascending) they lie
+// in the k chunks whose maxima come first in that order, since a value outside
+// these has k maxima before it. So the pass leaves the maxima, and its end ranks
+// them, reads the k best chunks again and keeps what reaches the k-th maximum
+// (as good as k values in all, but for ties) in a list, a lane an entry.
+//
+// Bound by HBM at many rows (the row's one read, 11 VALU instructions a value of
+// the 13 that fit beside it); by two launches and their trips to memory at few,
+// where a row is split over workgroups.
 #include <math.h>
 
 #include "mi_common.h"
@@ -23,6 +29,9 @@ namespace {
 
 constexpr int LP_MAX_TOP = 64;   // a lane an entry
 constexpr int LP_WAVES = 4;
+constexpr int LP_CHUNK = 1024;   // values a chunk, 2 (16 bits) or 4 (fp32) 16-byte pieces a lane
+constexpr int64_t LP_MAX_V = (int64_t)1 << 22;
+constexpr int LP_MAX_CHUNKS = (int)(LP_MAX_V / LP_CHUNK) + 1;  // (the first may begin before the row)
 constexpr float LP_LOG2E = 1.4426950408889634f;
 
 // A 16-byte piece of a row as floats.
@@ -80,164 +89,302 @@ __device__ __forceinline__ void move_ref(float &s, float &e, float from, float t
     s *= f;
 }
 
+// The order of floats as the order of ints (-0 as 0); what is no value is NONE.
+constexpr int NONE = (int)0x80000000;
+__device__ __forceinline__ int key_of(float x) {
+    const int b = __builtin_bit_cast(int, x + 0.0f);
+    return x != x ? NONE : b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float of_key(int k) {
+    return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff));
+}
+
+// A wave's list: lane i < k holds the i-th best (key, index).
 struct TopList {
-    float v;  // lane i: the i-th best value
-    int id;
-    float last;  // the k-th best value (uniform)
+    int key, id;
+    int last_key, last_id;  // what a value has to come before (uniform)
 };
-__device__ __forceinline__ void top_insert(TopList &l, float v, int id, int k, int lane) {
-    const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(l.v >= v));
-    const float pv = __shfl_up(l.v, 1, 64);
-    const int pi = __shfl_up(l.id, 1, 64);
-    l.v = lane < at ? l.v : (lane == at ? v : pv);
+__device__ __forceinline__ bool before(int ka, int ia, int kb, int ib) {
+    return ka > kb || (ka == kb && ia < ib);
+}
+__device__ __forceinline__ void top_insert(TopList &l, int key, int id, int k, int lane) {
+    const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(l.key, l.id, key, id)));
+    const int pk = __shfl_up(l.key, 1, 64), pi = __shfl_up(l.id, 1, 64);
+    l.key = lane < at ? l.key : (lane == at ? key : pk);
     l.id = lane < at ? l.id : (lane == at ? id : pi);
-    l.last = readlane_f(l.v, k - 1);
+    const int lk = __builtin_amdgcn_readlane(l.key, k - 1);
+    if (lk != NONE) l.last_key = lk, l.last_id = __builtin_amdgcn_readlane(l.id, k - 1);
 }
 
-// One piece a lane (first: the index of its first value; lanes in index order).
-template <typename T, bool TOP>
-__device__ __forceinline__ void add_piece(Sums &a, TopList &l, const Piece<T> &p, int first, int k,
-                                          int lane) {
-    constexpr int N = Piece<T>::N;
-    float pm = fmaxf(p.f[0], p.f[1]);
-#pragma unroll
-    for (int i = 2; i < N; i += 2) pm = fmaxf(fmaxf(pm, p.f[i]), p.f[i + 1]);
-    a.top = fmaxf(a.top, pm);
-    if (__builtin_amdgcn_ballot_w64(pm > a.ref + 30.0f)) {
-        const float to = fmaxf(a.ref, wave_max(pm));
-        move_ref(a.s, a.e, a.ref, to);
-        a.ref = to;
+// A row as 16-byte pieces from the one that holds its first value; value i of
+// piece p is row element p N + i - skew. What lies outside the row reads as -inf.
+template <typename T> struct Row {
+    static constexpr int N = Piece<T>::N, PER = LP_CHUNK / (64 * N);  // pieces a lane and chunk
+    const T *x;
+    const char *base;
+    int skew, V;
+    __device__ __forceinline__ Row(const T *x_, int V_) : x(x_), V(V_) {
+        skew = (int)(((uintptr_t)x & 15) / sizeof(T));
+        base = (const char *)x - skew * (int)sizeof(T);
     }
+    __device__ __forceinline__ int chunks() const { return (V + skew + LP_CHUNK - 1) / LP_CHUNK; }
+    __device__ __forceinline__ int first(int chunk, int i, int lane) const {
+        return chunk * LP_CHUNK + (64 * i + lane) * N - skew;
+    }
+    // NT: a row read once, past the caches
+    template <bool NT>
+    __device__ __forceinline__ void get(int chunk, int lane, Piece<T> (&pc)[PER]) const {
+        if (chunk > 0 && (chunk + 1) * LP_CHUNK - skew <= V) {  // (uniform)
+            uint4 raw[PER];
 #pragma unroll
-    for (int i = 0; i < N; ++i) add_value(a, p.f[i]);
-    if constexpr (TOP) {
-        uint64_t mask = __builtin_amdgcn_ballot_w64(pm > l.last);
-        while (mask) {
-            const int from = __builtin_ctzll(mask);
-            float v = 0.0f;  // lane i < N: value i of that lane's piece
+            for (int i = 0; i < PER; ++i) {
+                const char *at = base + ((int64_t)chunk * LP_CHUNK + (64 * i + lane) * N) * (int)sizeof(T);
+                raw[i] = NT ? ld16_nt(at) : ld16(at);
+            }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float w = readlane_f(p.f[i], from);
-                v = lane == i ? w : v;
+            for (int i = 0; i < PER; ++i) pc[i] = open_piece<T>(raw[i]);
+        } else {  // the row's ends
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int f = first(chunk, i, lane);
+                if (f >= 0 && f + N <= V)
+                    pc[i] = open_piece<T>(ld16(base + (int64_t)(f + skew) * (int)sizeof(T)));
+                else
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        pc[i].f[e] = f + e >= 0 && f + e < V ? (float)x[f + e] : -INFINITY;
             }
-            const int base = __builtin_amdgcn_readlane(first, from);
-            uint64_t in = __builtin_amdgcn_ballot_w64(lane < N && v > l.last);
-            while (in) {
-                const int i = __builtin_ctzll(in);
-                top_insert(l, readlane_f(v, i), base + i, k, lane);
-                in &= in - 1;
-                in &= __builtin_amdgcn_ballot_w64(lane < N && v > l.last);
-            }
-            mask &= mask - 1;
-            mask &= __builtin_amdgcn_ballot_w64(pm > l.last);
         }
     }
-}
+};
 
-// One workgroup a row.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void logprob_kernel(
-    const T *__restrict__ x, int64_t row_stride, const void *__restrict__ tokens, int wide,
-    int V, int k, float *__restrict__ logprob, float *__restrict__ entropy,
-    int *__restrict__ top_ids, float *__restrict__ top_logprobs) {
-    constexpr int N = Piece<T>::N;
-    __shared__ float4 part[LP_WAVES];
-    __shared__ float lv[LP_WAVES * LP_MAX_TOP];
-    __shared__ int li[LP_WAVES * LP_MAX_TOP];
-    __shared__ float bv[LP_MAX_TOP];
-    __shared__ int bi[LP_MAX_TOP];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
-    const T *xr = x + row * row_stride;
-    // 16-byte pieces from the one that holds the row's first value; value i of
-    // piece p is row element p N + i - skew
-    const int skew = (int)(((uintptr_t)xr & 15) / sizeof(T));
-    const char *base = (const char *)xr - skew * (int)sizeof(T);
-    const int np = (V + skew + N - 1) / N;
+// The chunks c0, c0 + step, ... below c1 of a row, by one wave: its sums, and (TOP)
+// the key of each chunk's maximum at maxima[c].
+template <typename T, bool TOP, bool NT>
+__device__ __forceinline__ float4 pass(const Row<T> &row, int c0, int c1, int step, int *maxima,
+                                       int lane) {
+    constexpr int N = Row<T>::N, PER = Row<T>::PER;
     Sums a = {-3.4028235e38f, -INFINITY, 0.0f, 0.0f};
-    TopList l = {-INFINITY, 0x7fffffff, -INFINITY};
-    for (int p0 = wave * 64; p0 < np; p0 += 64 * LP_WAVES) {
-        const int p = p0 + lane, first = p * N - skew;
-        Piece<T> pc;
-        if (p > 0 && first + N <= V) {
-            pc = open_piece<T>(ld16(base + (int64_t)p * 16));
-        } else {  // the row's ends, and lanes past it
+    for (int c = c0; c < c1; c += step) {
+        Piece<T> pc[PER];
+        row.template get<NT>(c, lane, pc);
+        float pm = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                pc.f[i] = first + i >= 0 && first + i < V ? (float)xr[first + i] : -INFINITY;
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int e = 0; e < N; e += 2) pm = fmaxf(fmaxf(pm, pc[i].f[e]), pc[i].f[e + 1]);
+        a.top = fmaxf(a.top, pm);
+        if (TOP) {
+            const float cm = wave_max(pm);
+            if (lane == 0) maxima[c] = key_of(cm);
         }
-        add_piece<T, TOP>(a, l, pc, first, k, lane);
-    }
-    const float top = wave_max(a.top);
-    const float s = wave_add(a.s), e = wave_add(a.e);
-    if (lane == 0) part[wave] = make_float4(a.ref, top, s, e);
-    if constexpr (TOP) {
-        if (lane < k) lv[wave * k + lane] = l.v, li[wave * k + lane] = l.id;
-        if (threadIdx.x < k) bv[threadIdx.x] = -INFINITY, bi[threadIdx.x] = 0x7fffffff;
-    }
-    __syncthreads();
-    float m = part[0].y;
+        if (__builtin_amdgcn_ballot_w64(pm > a.ref + 30.0f)) {
+            const float to = fmaxf(a.ref, wave_max(pm));
+            move_ref(a.s, a.e, a.ref, to);
+            a.ref = to;
+        }
 #pragma unroll
-    for (int w = 1; w < LP_WAVES; ++w) m = fmaxf(m, part[w].y);
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) add_value(a, pc[i].f[e]);
+    }
+    return make_float4(a.ref, wave_max(a.top), wave_add(a.s), wave_add(a.e));
+}
+
+struct LpArgs {
+    const void *x;
+    int64_t row_stride;
+    const void *tokens;
+    int wide, V, k;
+    float *logprob, *entropy;
+    int *top_ids;
+    float *top_logprobs;
+    // rows split over workgroups: of each row its segments' sums and its chunks'
+    // maxima, nc a row
+    float4 *part;
+    int *maxima;
+    int nc, per;  // chunks a segment
+};
+
+// What follows the pass, by a workgroup of WAVES, from the row's n partial sums (ref,
+// top, s, e) and, in LDS, the keys of its chunks' maxima.
+template <int WAVES> struct TopLds {
+    int sel[LP_MAX_TOP];
+    int key[WAVES * LP_MAX_TOP], id[WAVES * LP_MAX_TOP];
+    int bkey[LP_MAX_TOP], bid[LP_MAX_TOP];
+    int count[WAVES];
+    int floor;
+};
+template <typename T, bool TOP, int WAVES>
+__device__ __forceinline__ void finish(const Row<T> &row, int64_t r, const float4 *part, int n,
+                                       const int *maxima, TopLds<WAVES> *t, const LpArgs &a) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // every wave adds the partial sums, 64 a step, in one order
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, part[i].y);
+    m = wave_max(m);
     float S = 0.0f, E = 0.0f;
-#pragma unroll
-    for (int w = 0; w < LP_WAVES; ++w) {
-        float sw = part[w].z, ew = part[w].w;
-        move_ref(sw, ew, part[w].x, m);
-        S += sw;
-        E += ew;
+    for (int i = lane; i < n; i += 64) {
+        const float4 p = part[i];
+        float s = p.z, e = p.w;
+        move_ref(s, e, p.x, m);
+        S += s;
+        E += e;
     }
+    S = wave_add(S);
+    E = wave_add(E);
     const float ls = logf(S);
     if (threadIdx.x == 0) {
-        const int64_t t = wide ? ((const int64_t *)tokens)[row] : ((const int *)tokens)[row];
-        logprob[row] = t >= 0 && t < V ? ((float)xr[t] - m) - ls : NAN;
-        entropy[row] = ls - E / S;
+        const int64_t tok = a.wide ? ((const int64_t *)a.tokens)[r] : ((const int *)a.tokens)[r];
+        a.logprob[r] = tok >= 0 && tok < row.V ? ((float)row.x[tok] - m) - ls : NAN;
+        a.entropy[r] = ls - E / S;
     }
     if constexpr (TOP) {
-        // the best k of the waves' lists, by counting what comes before each
-        const int n = LP_WAVES * k;
-        if (threadIdx.x < n) {
-            const float v = lv[threadIdx.x];
-            const int id = li[threadIdx.x];
+        const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) {
+            const int key = maxima[c];
             int rank = 0;
-            for (int i = 0; i < n; ++i)
-                rank += lv[i] > v || (lv[i] == v && (li[i] < id || (li[i] == id && i < threadIdx.x)));
-            if (rank < k) bv[rank] = v, bi[rank] = id;
+            for (int i = 0; i < nc; ++i) rank += before(maxima[i], i, key, c);
+            if (rank < need) t->sel[rank] = c;
+            if (rank == need - 1) t->floor = need == k ? key : NONE + 1;
         }
         __syncthreads();
-        if (wave == 0) {
-            // fewer than k values above -inf: the lowest indices of -inf fill up
-            int have = __builtin_popcountll(
-                __builtin_amdgcn_ballot_w64(lane < k && bi[lane] != 0x7fffffff));
-            float v = lane < k ? bv[lane] : 0.0f;
-            int id = lane < k ? bi[lane] : 0;
-            for (int i0 = 0; have < k && i0 < V; i0 += 64) {
-                const int i = i0 + lane;
-                uint64_t in = __builtin_amdgcn_ballot_w64(i < V && (float)xr[i < V ? i : 0] == -INFINITY);
-                while (in && have < k) {
-                    if (lane == have) id = i0 + __builtin_ctzll(in);
-                    in &= in - 1;
-                    ++have;
+        TopList l = {NONE, 0x7fffffff, t->floor - 1, 0};
+        for (int j = wave; j < need; j += WAVES) {
+            const int c = t->sel[j];
+            Piece<T> pc[Row<T>::PER];
+            row.template get<false>(c, lane, pc);
+#pragma unroll
+            for (int i = 0; i < Row<T>::PER; ++i)
+#pragma unroll
+                for (int e = 0; e < Row<T>::N; ++e) {
+                    const int id = row.first(c, i, lane) + e;
+                    const int key = id >= 0 && id < row.V ? key_of(pc[i].f[e]) : NONE;
+                    uint64_t in = __builtin_amdgcn_ballot_w64(before(key, id, l.last_key, l.last_id));
+                    while (in) {
+                        const int from = __builtin_ctzll(in);
+                        in &= in - 1;
+                        const int ki = __builtin_amdgcn_readlane(key, from);
+                        const int ii = __builtin_amdgcn_readlane(id, from);
+                        if (before(ki, ii, l.last_key, l.last_id)) top_insert(l, ki, ii, k, lane);
+                    }
                 }
-            }
-            if (lane < k) {
-                top_ids[row * k + lane] = id < V ? id : 0;
-                top_logprobs[row * k + lane] = (v - m) - ls;
-            }
+        }
+        // the best k of the waves' lists, by counting what comes before each entry
+        const bool mine = lane < k && l.key != NONE;
+        const int entries = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine));
+        if (lane == 0) t->count[wave] = entries;
+        if (threadIdx.x < k) t->bkey[threadIdx.x] = NONE, t->bid[threadIdx.x] = 0;
+        __syncthreads();
+        int at = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) at += t->count[w];
+            total += t->count[w];
+        }
+        if (mine) t->key[at + lane] = l.key, t->id[at + lane] = l.id;
+        __syncthreads();
+        for (int j = threadIdx.x; j < total; j += 64 * WAVES) {
+            const int key = t->key[j], id = t->id[j];
+            int rank = 0;
+            for (int i = 0; i < total; ++i) rank += before(t->key[i], t->id[i], key, id);
+            if (rank < k) t->bkey[rank] = key, t->bid[rank] = id;
+        }
+        __syncthreads();
+        if (threadIdx.x < k) {
+            const int key = t->bkey[threadIdx.x];
+            a.top_ids[r * k + threadIdx.x] = t->bid[threadIdx.x];
+            a.top_logprobs[r * k + threadIdx.x] = key == NONE ? NAN : (of_key(key) - m) - ls;
         }
     }
 }
 
-template <typename T>
-int launch_logprobs(const void *x, int64_t rows, int64_t V, int64_t stride, const void *tokens,
-                    int wide, int top, float *lp, float *ent, int32_t *ids, float *tlp,
-                    hipStream_t st) {
-    if (top)
-        logprob_kernel<T, true><<<(unsigned)rows, 64 * LP_WAVES, 0, st>>>(
-            (const T *)x, stride, tokens, wide, (int)V, top, lp, ent, ids, tlp);
-    else
-        logprob_kernel<T, false><<<(unsigned)rows, 64 * LP_WAVES, 0, st>>>(
-            (const T *)x, stride, tokens, wide, (int)V, 0, lp, ent, ids, tlp);
+// A workgroup a row.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(64 * LP_WAVES) void logprob_row_kernel(LpArgs a) {
+    __shared__ float4 part[LP_WAVES];
+    __shared__ int maxima[TOP ? LP_MAX_CHUNKS : 1];
+    __shared__ TopLds<LP_WAVES> top[1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t r = blockIdx.x;
+    const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    const float4 p = pass<T, TOP, true>(row, wave, row.chunks(), LP_WAVES, maxima, lane);
+    if (lane == 0) part[wave] = p;
+    __syncthreads();
+    finish<T, TOP, LP_WAVES>(row, r, part, LP_WAVES, maxima, top, a);
+}
+
+// A workgroup a segment of a row.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(64 * LP_WAVES) void logprob_part_kernel(LpArgs a) {
+    __shared__ float4 part[LP_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t r = blockIdx.y;
+    const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    const int c0 = blockIdx.x * a.per, end = c0 + a.per, nc = row.chunks();
+    const float4 p = pass<T, TOP, false>(row, c0 + wave, end < nc ? end : nc, LP_WAVES,
+                                         a.maxima + r * a.nc, lane);
+    if (lane == 0) part[wave] = p;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        // to the largest reference (each is finite, a segment of -inf alone too)
+        float ref = part[0].x, top = part[0].y, s = 0.0f, e = 0.0f;
+        for (int w = 1; w < LP_WAVES; ++w) ref = fmaxf(ref, part[w].x), top = fmaxf(top, part[w].y);
+        for (int w = 0; w < LP_WAVES; ++w) {
+            float sw = part[w].z, ew = part[w].w;
+            move_ref(sw, ew, part[w].x, ref);
+            s += sw;
+            e += ew;
+        }
+        a.part[r * gridDim.x + blockIdx.x] = make_float4(ref, top, s, e);
+    }
+}
+constexpr int LP_JOIN_WAVES = 8;
+template <typename T, bool TOP>
+__global__ __launch_bounds__(64 * LP_JOIN_WAVES) void logprob_join_kernel(LpArgs a, int segments) {
+    __shared__ int maxima[TOP ? LP_MAX_CHUNKS : 1];
+    __shared__ TopLds<LP_JOIN_WAVES> top[1];
+    const int64_t r = blockIdx.x;
+    const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    if (TOP) {
+        const int nc = row.chunks();
+        for (int c = threadIdx.x; c < nc; c += 64 * LP_JOIN_WAVES) maxima[c] = a.maxima[r * a.nc + c];
+        __syncthreads();
+    }
+    finish<T, TOP, LP_JOIN_WAVES>(row, r, a.part + r * segments, segments, maxima, top, a);
+}
+
+// Segments of a row: none from 512 rows on (two workgroups a CU by themselves);
+// below, about a thousand workgroups in all, of at least a chunk a wave.
+struct LpSplit {
+    int64_t nc, segments, per;
+};
+inline LpSplit lp_split(int64_t rows, int64_t V, int dtype) {
+    LpSplit s;
+    s.nc = (V + (dtype == MI_F32 ? 3 : 7) + LP_CHUNK - 1) / LP_CHUNK;
+    const int64_t most = ceil_div(s.nc, LP_WAVES), want = rows < 512 ? ceil_div(1024, rows) : 1;
+    s.per = ceil_div(s.nc, want < most ? want : most);
+    s.segments = ceil_div(s.nc, s.per);
+    return s;
+}
+inline int64_t lp_bytes(const LpSplit &s, int64_t rows, int top) {
+    return s.segments > 1 ? rows * (s.segments * 16 + (top ? s.nc * 4 : 0)) : 0;
+}
+
+template <typename T, bool TOP>
+int launch_logprobs(LpArgs a, int64_t rows, const LpSplit &s, void *ws, hipStream_t st) {
+    if (!ws) {
+        logprob_row_kernel<T, TOP><<<(unsigned)rows, 64 * LP_WAVES, 0, st>>>(a);
+        return launch_status("token logprobs");
+    }
+    a.part = (float4 *)ws;
+    a.maxima = (int *)(a.part + rows * s.segments);
+    a.nc = (int)s.nc;
+    a.per = (int)s.per;
+    logprob_part_kernel<T, TOP>
+        <<<dim3((unsigned)s.segments, (unsigned)rows), 64 * LP_WAVES, 0, st>>>(a);
+    logprob_join_kernel<T, TOP><<<(unsigned)rows, 64 * LP_JOIN_WAVES, 0, st>>>(a, (int)s.segments);
     return launch_status("token logprobs");
 }
 
@@ -246,14 +393,19 @@ int launch_logprobs(const void *x, int64_t rows, int64_t V, int64_t stride, cons
 
 using namespace mi;
 
+extern "C" int64_t mi_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int top, int dtype) {
+    if (rows <= 0 || V <= 0 || V > LP_MAX_V || top < 0) return 0;
+    return lp_bytes(lp_split(rows, V, dtype), rows, top);
+}
+
 extern "C" int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_stride,
                                  const void *tokens, int tokens_are_64, int top, float *logprobs,
                                  float *entropy, int32_t *top_ids, float *top_logprobs, int dtype,
-                                 void *stream) {
+                                 void *workspace, int64_t workspace_bytes, void *stream) {
     if (!valid_dtype(dtype)) return fail(MI_ERR_UNSUPPORTED, "dtype code %d", dtype);
-    if (rows < 0 || rows > 0x7fffffff || V < 1 || V > (1 << 30) || row_stride < 0)
-        return fail(MI_ERR_ARG, "token logprobs rows=%lld V=%lld row stride %lld", (long long)rows,
-                    (long long)V, (long long)row_stride);
+    if (rows < 0 || rows > 0x7fffffff || V < 1 || V > LP_MAX_V || row_stride < 0)
+        return fail(MI_ERR_ARG, "token logprobs rows=%lld V=%lld (1 to 2^22) row stride %lld",
+                    (long long)rows, (long long)V, (long long)row_stride);
     if (top < 0 || top > LP_MAX_TOP || top > V)
         return fail(MI_ERR_ARG, "token logprobs top=%d: 0 to %d, at most V=%lld", top, LP_MAX_TOP,
                     (long long)V);
@@ -262,10 +414,17 @@ extern "C" int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, in
         return fail(MI_ERR_ARG, "null pointer");
     if (!aligned(logits, dtype == MI_F32 ? 4 : 2))
         return fail(MI_ERR_ARG, "logits are not aligned to their type");
+    const LpSplit s = lp_split(rows, V, dtype);
+    const int64_t need = lp_bytes(s, rows, top);
+    void *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16) ? workspace
+                                                                                      : nullptr;
+    const LpArgs a = {logits, row_stride, tokens, tokens_are_64, (int)V, top, logprobs, entropy,
+                      top_ids, top_logprobs, nullptr, nullptr, 0, 0};
     hipStream_t st = as_stream(stream);
     auto run = [&](auto tag) {
-        return launch_logprobs<decltype(tag)>(logits, rows, V, row_stride, tokens, tokens_are_64,
-                                              top, logprobs, entropy, top_ids, top_logprobs, st);
+        typedef decltype(tag) T;
+        return top ? launch_logprobs<T, true>(a, rows, s, ws, st)
+                   : launch_logprobs<T, false>(a, rows, s, ws, st);
     };
     return dtype == MI_BF16 ? run(bf16{}) : dtype == MI_F16 ? run(f16{}) : run(float{});
 }

@@ -86,7 +86,8 @@ def test_attention_of_nothing(lib):
 
 
 def _lp(L, x=P, rows=2, V=100, stride=100, tokens=P, top=5, dt=hip.MI_BF16, ids=P):
-    return L.mi_token_logprobs(x, rows, V, stride, tokens, 1, top, P, P, ids, P, dt, None)
+    return L.mi_token_logprobs(x, rows, V, stride, tokens, 1, top, P, P, ids, P, dt, None, 0,
+                               None)
 
 
 @pytest.mark.parametrize("kw,code,text", [
