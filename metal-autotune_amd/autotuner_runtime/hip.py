@@ -445,10 +445,11 @@ def paged_attention(q, k_pages, v_pages, out, table, cu_q, kv_lens, scale: float
     R, width = table.shape
     stream = _stream(q)
     nbytes = _paged_workspace_bytes(T, R, width, H, HK, D, page, max_q_len)
-    ws = _workspace("paged", q.device, stream, nbytes, 4 << 20) if nbytes else None
-    _check(lib().mi_paged_attention(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(table),
-                                    _ptr(cu_q), _ptr(kv_lens), T, R, width, H, HK, D, n_pages,
-                                    page, max_q_len, scale, _dt(q), _ptr(ws), nbytes, stream),
+    ws = _workspace("paged", q.device, stream, nbytes, 4 << 20).data_ptr() if nbytes else None
+    _check(lib().mi_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                    out.data_ptr(), table.data_ptr(), cu_q.data_ptr(),
+                                    kv_lens.data_ptr(), T, R, width, H, HK, D, n_pages, page,
+                                    max_q_len, scale, _dt(q), ws, nbytes, stream),
            "paged_attention")
 
 
@@ -470,11 +471,11 @@ def token_logprobs(x, tokens, top: int, logprobs, entropy, ids, top_logprobs) ->
     rows, V = x.shape
     dt, stream = _dt(x), _stream(x)
     nbytes = _logprobs_workspace_bytes(rows, V, top, dt)
-    ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20) if nbytes else None
-    _check(lib().mi_token_logprobs(_ptr(x), rows, V, x.stride(0), _ptr(tokens),
-                                   int(tokens.dtype == torch.int64), top, _ptr(logprobs),
-                                   _ptr(entropy), _ptr(ids), _ptr(top_logprobs), dt, _ptr(ws),
-                                   nbytes, stream), "token_logprobs")
+    ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20).data_ptr() if nbytes else None
+    _check(lib().mi_token_logprobs(x.data_ptr(), rows, V, x.stride(0), tokens.data_ptr(),
+                                   tokens.dtype is torch.int64, top, logprobs.data_ptr(),
+                                   entropy.data_ptr(), ids.data_ptr(), top_logprobs.data_ptr(),
+                                   dt, ws, nbytes, stream), "token_logprobs")
 
 
 def b_swiglu(ins, outs, p):

@@ -314,10 +314,14 @@ def argmax(x, split: bool = True) -> torch.Tensor:
 # Pools of pages k_pages, v_pages [n_pages, HK, page_size, D]; a block table int32
 # [R, width] of each request's pages; the tokens of a step request after request.
 
-def _i32(what: str, like: torch.Tensor, **arrays) -> None:
-    for name, t in arrays.items():
-        if t.dtype != torch.int32 or t.device != like.device or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be a contiguous int32 array on {like.device}")
+_I32, _F32 = torch.int32, torch.float32
+
+
+def _i32(what: str, dev: int, *arrays) -> None:
+    for t in arrays:
+        if t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: lengths, tables and positions must be contiguous int32 "
+                             f"arrays on one device, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 class PagedPlan(NamedTuple):
@@ -340,29 +344,30 @@ def paged_plan(block_table, kv_lens, q_lens, free_pages, free_count, page_size: 
     step's token buffer, at least the sum of q_lens (rows behind it get position 0
     and slot -1). A request whose pages are not there, or whose keys would pass
     its row of the table, takes none and is counted in ``refused``."""
-    hip._require_gpu(block_table)
-    if block_table.dim() != 2 or kv_lens.dim() != 1 or kv_lens.shape != q_lens.shape \
-            or kv_lens.shape[0] != block_table.shape[0] or free_pages.dim() != 1 \
+    if not block_table.is_cuda:
+        hip._require_gpu(block_table)
+    shape = kv_lens.shape
+    if block_table.dim() != 2 or len(shape) != 1 or q_lens.shape != shape \
+            or shape[0] != block_table.shape[0] or free_pages.dim() != 1 \
             or free_count.numel() != 1:
         raise ValueError("paged_plan takes block_table [R, width], kv_lens [R], q_lens [R], "
                          "free_pages [F] and free_count [1]")
-    _i32("paged_plan", block_table, block_table=block_table, kv_lens=kv_lens, q_lens=q_lens,
-         free_pages=free_pages, free_count=free_count)
+    _i32("paged_plan", block_table.get_device(), block_table, kv_lens, q_lens, free_pages,
+         free_count)
     R, width = block_table.shape
     T = int(num_tokens)
-    # one allocation for the six outputs, each from a 16-byte boundary
-    sizes = (R + 1, R, T, T, 1, 1)
-    at, starts = 0, []
-    for n in sizes:
-        starts.append(at)
-        at += (n + 3) & ~3
-    buf = block_table.new_empty(at)
-    out = PagedPlan(*(buf[s:s + n] for s, n in zip(starts, sizes)))
+    if T < 0:
+        raise ValueError(f"paged_plan: num_tokens={T}")
+    # one allocation for the six outputs, which lie one after another
+    buf = block_table.new_empty(2 * (R + T) + 3)
+    at = buf.data_ptr()
     hip._check(hip.lib().mi_paged_plan(
         block_table.data_ptr(), width, kv_lens.data_ptr(), q_lens.data_ptr(),
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), R, T, int(page_size),
-        *(t.data_ptr() for t in out), hip._stream(block_table)), "paged_plan")
-    return out
+        at, at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + T),
+        at + 4 * (2 * (R + T) + 1), at + 4 * (2 * (R + T) + 2), hip._stream(block_table)),
+        "paged_plan")
+    return PagedPlan._make(torch.split_with_sizes(buf, (R + 1, R, T, T, 1, 1)))
 
 
 def rope_table(dims: int, base: float = 10000.0, scale: float = 1.0, freqs=None,
@@ -380,13 +385,15 @@ def rope_table(dims: int, base: float = 10000.0, scale: float = 1.0, freqs=None,
     return scale * base ** (-2.0 * i / dims)
 
 
-def _paged_pools(what: str, q, k_pages, v_pages, D: int) -> tuple:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != D \
-            or k_pages.dtype != q.dtype or v_pages.dtype != q.dtype \
-            or not k_pages.is_contiguous() or not v_pages.is_contiguous():
-        raise ValueError(f"{what}: the pools must be contiguous {q.dtype} [pages, heads, page size, "
-                         f"{D}], got {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    return k_pages.shape
+def _paged_pools(what: str, q, k_pages, v_pages, D: int):
+    shape, dt, dev = k_pages.shape, q.dtype, q.get_device()
+    if len(shape) != 4 or v_pages.shape != shape or shape[3] != D or k_pages.dtype is not dt \
+            or v_pages.dtype is not dt or k_pages.get_device() != dev \
+            or v_pages.get_device() != dev or not k_pages.is_contiguous() \
+            or not v_pages.is_contiguous():
+        raise ValueError(f"{what}: the pools must be contiguous {dt} [pages, heads, page size, "
+                         f"{D}] on {q.device}, got {tuple(shape)} and {tuple(v_pages.shape)}")
+    return shape
 
 
 def norm_rope_paged(q, k, v, q_norm, k_norm, n_heads: int, n_kv_heads: int, eps: float,
@@ -398,35 +405,41 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, n_heads: int, n_kv_heads: int, eps:
     A norm weight of None skips the normalization. ``inv_freq``: ``rope_table``'s,
     whose 2 * len(inv_freq) leading values of a head are turned, at the angle of
     each token's own position. q, k, v may be column ranges of one projection."""
-    T = q.shape[0]
-    D = q.shape[-1] // n_heads
-    for name, t, h in (("q", q, n_heads), ("k", k, n_kv_heads), ("v", v, n_kv_heads)):
-        if t.dim() != 2 or tuple(t.shape) != (T, h * D) or t.dtype != q.dtype:
-            raise ValueError(f"norm_rope_paged: {name} must be {q.dtype} {(T, h * D)}, got "
-                             f"{t.dtype} {tuple(t.shape)}")
+    T, width = q.shape
+    D = width // n_heads
+    dt, dev, kv = q.dtype, q.get_device(), (T, n_kv_heads * D)
+    if width != n_heads * D or k.shape != kv or v.shape != kv or k.dtype is not dt \
+            or v.dtype is not dt or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"norm_rope_paged: q, k, v must be one type on one device, [T, heads * D], "
+                         f"got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     for wt in (q_norm, k_norm):
-        if wt is not None and (tuple(wt.shape) != (D,) or wt.dtype != q.dtype
+        if wt is not None and (wt.shape != (D,) or wt.dtype is not dt or wt.get_device() != dev
                                or not wt.is_contiguous()):
-            raise ValueError(f"norm weight must be contiguous {q.dtype} [{D}]")
+            raise ValueError(f"norm weight must be contiguous {dt} [{D}] on {q.device}")
     n_pages, hk, page, _ = _paged_pools("norm_rope_paged", q, k_pages, v_pages, D)
     if hk != n_kv_heads or positions.shape != (T,) or slots.shape != (T,):
         raise ValueError(f"norm_rope_paged: pools of {n_kv_heads} heads, positions and slots of "
                          f"{T} tokens are needed")
-    _i32("norm_rope_paged", q, positions=positions, slots=slots)
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
-            or inv_freq.device != q.device:
+    _i32("norm_rope_paged", dev, positions, slots)
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 \
+            or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
         raise ValueError("norm_rope_paged: inv_freq must be a float64 array (ops.rope_table)")
-    hip._require_gpu(q)
-    # rows the kernel cannot read in 16-byte pieces are copied first
-    q, k, v = (t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-               else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    if not q.is_cuda:
+        hip._require_gpu(q)
+    (sq, uq), (sk, uk), (sv, uv) = q.stride(), k.stride(), v.stride()
+    pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (pq | pk | pv) & 15 or (sq | sk | sv) & 7 or not uq == uk == uv == 1:
+        # rows the kernel cannot read in 16-byte pieces are copied first
+        q, k, v = (t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+        (sq, _), (sk, _), (sv, _) = q.stride(), k.stride(), v.stride()
+        pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
     out = q.new_empty((T, n_heads, D))
     hip._check(hip.lib().mi_norm_rope_paged(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
-        hip._ptr(q_norm), hip._ptr(k_norm), out.data_ptr(), k_pages.data_ptr(),
+        pq, pk, pv, sq, sk, sv, None if q_norm is None else q_norm.data_ptr(),
+        None if k_norm is None else k_norm.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
         v_pages.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(traditional),
         positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv_heads, D, n_pages, page,
-        float(eps), hip._dt(q), hip._stream(q)), "norm_rope_paged")
+        eps, hip._dt(q), hip._stream(q)), "norm_rope_paged")
     return out
 
 
@@ -440,17 +453,18 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale: floa
     meaning. Rows behind the last request's are not written."""
     if q.dim() != 3:
         raise ValueError(f"paged_attention: q must be [T, H, D], got {tuple(q.shape)}")
-    T, H, D = q.shape
-    n_pages, HK, page, _ = _paged_pools("paged_attention", q, k_pages, v_pages, D)
-    R = kv_lens.shape[0]
+    _paged_pools("paged_attention", q, k_pages, v_pages, q.shape[2])
+    R, = kv_lens.shape
     if block_table.dim() != 2 or block_table.shape[0] != R or cu_q.shape != (R + 1,):
         raise ValueError("paged_attention takes block_table [R, width], cu_q [R + 1], kv_lens [R]")
-    _i32("paged_attention", q, block_table=block_table, cu_q=cu_q, kv_lens=kv_lens)
-    hip._require_gpu(q)
-    q = q.contiguous()
+    _i32("paged_attention", q.get_device(), block_table, cu_q, kv_lens)
+    if not q.is_cuda:
+        hip._require_gpu(q)
+    if not q.is_contiguous():
+        q = q.contiguous()
     out = torch.empty_like(q)
-    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, float(scale),
-                        0 if max_q_len is None else int(max_q_len))
+    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, scale,
+                        0 if max_q_len is None else max_q_len)
     return out
 
 
@@ -468,23 +482,25 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     row's log softmax at its token (NaN outside [0, V)), its entropy, and its
     ``top`` (0 to 64) most probable tokens with their log probabilities, the lowest
     index first among equal logits. Logits of -inf are forbidden tokens."""
-    hip._require_gpu(logits)
-    lead, V = logits.shape[:-1], logits.shape[-1]
-    if tokens.shape != lead or tokens.dtype not in (torch.int32, torch.int64) \
-            or tokens.device != logits.device:
+    if not logits.is_cuda:
+        hip._require_gpu(logits)
+    *lead, V = logits.shape
+    if list(tokens.shape) != lead or (tokens.dtype is not torch.int64 and tokens.dtype is not _I32) \
+            or tokens.get_device() != logits.get_device():
         raise ValueError(f"token_logprobs: tokens must be int32 or int64 {tuple(lead)} on "
                          f"{logits.device}")
-    if V < 1 or not 0 <= top <= min(64, V):
+    if V < 1 or not 0 <= top <= 64 or top > V:
         raise ValueError(f"token_logprobs: top={top} of V={V} (0 to 64, at most V)")
-    if logits.stride(-1) != 1 or (logits.dim() != 2 and not logits.is_contiguous()):
-        logits = logits.contiguous()
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    tokens = tokens.contiguous()
-    rows = x.shape[0]
-    f32 = x.new_empty(rows * (2 + top), dtype=torch.float32)
-    ids = x.new_empty((*lead, top), dtype=torch.int32)
-    out = TokenLogprobs(f32[:rows].view(lead), f32[rows:2 * rows].view(lead), ids,
-                        f32[2 * rows:].view(*lead, top))
+    x = logits
+    if x.stride(-1) != 1 or (len(lead) != 1 and not x.is_contiguous()):
+        x = x.contiguous()
+    if len(lead) != 1:
+        x = x.reshape(-1, V)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    out = TokenLogprobs(x.new_empty(lead, dtype=_F32), x.new_empty(lead, dtype=_F32),
+                        x.new_empty((*lead, top), dtype=_I32),
+                        x.new_empty((*lead, top), dtype=_F32))
     hip.token_logprobs(x, tokens, top, *out)
     return out
 

@@ -55,15 +55,19 @@ template <typename T> __device__ __forceinline__ Piece<T> open_piece(uint4 raw) 
 __device__ __forceinline__ float readlane_f(float v, int l) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
+// Over a wave, by DPP moves within its rows of 16 and their lane 0 (no trip
+// through the LDS unit).
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    v = fmaxf(v, dpp_f32<0x141>(v));
+    v = fmaxf(v, dpp_f32<0x140>(v));
+    return fmaxf(fmaxf(readlane_f(v, 0), readlane_f(v, 16)),
+                 fmaxf(readlane_f(v, 32), readlane_f(v, 48)));
 }
 __device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v = row16_sum(v);
+    return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
 }
 
 struct Sums {
@@ -131,28 +135,34 @@ template <typename T> struct Row {
     __device__ __forceinline__ int first(int chunk, int i, int lane) const {
         return chunk * LP_CHUNK + (64 * i + lane) * N - skew;
     }
-    // NT: a row read once, past the caches
+    // whether every value of the chunk's pieces is the row's
+    __device__ __forceinline__ bool whole(int chunk) const {
+        return chunk > 0 && (chunk + 1) * LP_CHUNK - skew <= V;
+    }
+    // a whole chunk; NT: a row read once, past the caches
     template <bool NT>
-    __device__ __forceinline__ void get(int chunk, int lane, Piece<T> (&pc)[PER]) const {
-        if (chunk > 0 && (chunk + 1) * LP_CHUNK - skew <= V) {  // (uniform)
-            uint4 raw[PER];
+    __device__ __forceinline__ void load(int chunk, int lane, uint4 (&raw)[PER]) const {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const char *at = base + ((int64_t)chunk * LP_CHUNK + (64 * i + lane) * N) * (int)sizeof(T);
-                raw[i] = NT ? ld16_nt(at) : ld16(at);
-            }
+        for (int i = 0; i < PER; ++i) {
+            const char *at = base + ((int64_t)chunk * LP_CHUNK + (64 * i + lane) * N) * (int)sizeof(T);
+            raw[i] = NT ? ld16_nt(at) : ld16(at);
+        }
+    }
+    __device__ __forceinline__ void open(const uint4 (&raw)[PER], Piece<T> (&pc)[PER]) const {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) pc[i] = open_piece<T>(raw[i]);
-        } else {  // the row's ends
+        for (int i = 0; i < PER; ++i) pc[i] = open_piece<T>(raw[i]);
+    }
+    // the row's ends
+    __device__ __forceinline__ void get_end(int chunk, int lane, Piece<T> (&pc)[PER]) const {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int f = first(chunk, i, lane);
-                if (f >= 0 && f + N <= V)
-                    pc[i] = open_piece<T>(ld16(base + (int64_t)(f + skew) * (int)sizeof(T)));
-                else
+        for (int i = 0; i < PER; ++i) {
+            const int f = first(chunk, i, lane);
+            if (f >= 0 && f + N <= V) {
+                pc[i] = open_piece<T>(ld16(base + (int64_t)(f + skew) * (int)sizeof(T)));
+            } else {
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        pc[i].f[e] = f + e >= 0 && f + e < V ? (float)x[f + e] : -INFINITY;
+                for (int e = 0; e < N; ++e)
+                    pc[i].f[e] = f + e >= 0 && f + e < V ? (float)x[f + e] : -INFINITY;
             }
         }
     }
@@ -165,9 +175,18 @@ __device__ __forceinline__ float4 pass(const Row<T> &row, int c0, int c1, int st
                                        int lane) {
     constexpr int N = Row<T>::N, PER = Row<T>::PER;
     Sums a = {-3.4028235e38f, -INFINITY, 0.0f, 0.0f};
+    uint4 raw[PER];  // the next chunk, on its way while this one is added
+    if (c0 < c1 && row.whole(c0)) row.template load<NT>(c0, lane, raw);
     for (int c = c0; c < c1; c += step) {
         Piece<T> pc[PER];
-        row.template get<NT>(c, lane, pc);
+        if (row.whole(c)) {  // (uniform)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) launder(raw[i]);
+            row.open(raw, pc);
+        } else {
+            row.get_end(c, lane, pc);
+        }
+        if (c + step < c1 && row.whole(c + step)) row.template load<NT>(c + step, lane, raw);
         float pm = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
@@ -215,18 +234,42 @@ template <int WAVES> struct TopLds {
     int count[WAVES];
     int floor;
 };
+// The logit of row r's token, asked for before the pass.
+template <typename T> __device__ __forceinline__ float token_logit(const Row<T> &row, int64_t r,
+                                                                   const LpArgs &a) {
+    const int64_t tok = a.wide ? ((const int64_t *)a.tokens)[r] : ((const int *)a.tokens)[r];
+    return tok >= 0 && tok < row.V ? (float)row.x[tok] : NAN;
+}
+// p0: partial sum `lane` (any where there is none)
 template <typename T, bool TOP, int WAVES>
-__device__ __forceinline__ void finish(const Row<T> &row, int64_t r, const float4 *part, int n,
-                                       const int *maxima, TopLds<WAVES> *t, const LpArgs &a) {
+__device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit, float4 p0,
+                                       const float4 *part, int n, const int *maxima,
+                                       TopLds<WAVES> *t, const LpArgs &a) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (TOP) {
+        // the chunks' ranks (maxima: padded by NONE to a multiple of 8)
+        const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) {
+            const int key = maxima[c];
+            int rank = 0;
+            for (int i = 0; i < nc; i += 8) {
+                const int4 u = *(const int4 *)(maxima + i), v = *(const int4 *)(maxima + i + 4);
+                const int e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rank += before(e[j], i + j, key, c);
+            }
+            if (rank < need) t->sel[rank] = c;
+            if (rank == need - 1) t->floor = need == k ? key : NONE + 1;
+        }
+    }
     // every wave adds the partial sums, 64 a step, in one order
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, part[i].y);
+    float m = lane < n ? p0.y : -INFINITY;
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, part[i].y);
     m = wave_max(m);
     float S = 0.0f, E = 0.0f;
     for (int i = lane; i < n; i += 64) {
-        const float4 p = part[i];
+        const float4 p = i == lane ? p0 : part[i];
         float s = p.z, e = p.w;
         move_ref(s, e, p.x, m);
         S += s;
@@ -236,25 +279,23 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, const float
     E = wave_add(E);
     const float ls = logf(S);
     if (threadIdx.x == 0) {
-        const int64_t tok = a.wide ? ((const int64_t *)a.tokens)[r] : ((const int *)a.tokens)[r];
-        a.logprob[r] = tok >= 0 && tok < row.V ? ((float)row.x[tok] - m) - ls : NAN;
+        a.logprob[r] = (logit - m) - ls;
         a.entropy[r] = ls - E / S;
     }
     if constexpr (TOP) {
         const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
-        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) {
-            const int key = maxima[c];
-            int rank = 0;
-            for (int i = 0; i < nc; ++i) rank += before(maxima[i], i, key, c);
-            if (rank < need) t->sel[rank] = c;
-            if (rank == need - 1) t->floor = need == k ? key : NONE + 1;
-        }
         __syncthreads();
         TopList l = {NONE, 0x7fffffff, t->floor - 1, 0};
         for (int j = wave; j < need; j += WAVES) {
             const int c = t->sel[j];
             Piece<T> pc[Row<T>::PER];
-            row.template get<false>(c, lane, pc);
+            if (row.whole(c)) {
+                uint4 raw[Row<T>::PER];
+                row.template load<false>(c, lane, raw);
+                row.open(raw, pc);
+            } else {
+                row.get_end(c, lane, pc);
+            }
 #pragma unroll
             for (int i = 0; i < Row<T>::PER; ++i)
 #pragma unroll
@@ -288,6 +329,7 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, const float
         for (int j = threadIdx.x; j < total; j += 64 * WAVES) {
             const int key = t->key[j], id = t->id[j];
             int rank = 0;
+#pragma unroll 4
             for (int i = 0; i < total; ++i) rank += before(t->key[i], t->id[i], key, id);
             if (rank < k) t->bkey[rank] = key, t->bid[rank] = id;
         }
@@ -304,15 +346,17 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, const float
 template <typename T, bool TOP>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprob_row_kernel(LpArgs a) {
     __shared__ float4 part[LP_WAVES];
-    __shared__ int maxima[TOP ? LP_MAX_CHUNKS : 1];
+    __shared__ __attribute__((aligned(16))) int maxima[TOP ? LP_MAX_CHUNKS + 8 : 1];
     __shared__ TopLds<LP_WAVES> top[1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t r = blockIdx.x;
     const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    const float logit = token_logit(row, r, a);
+    if (TOP && threadIdx.x < 8) maxima[row.chunks() + threadIdx.x] = NONE;
     const float4 p = pass<T, TOP, true>(row, wave, row.chunks(), LP_WAVES, maxima, lane);
     if (lane == 0) part[wave] = p;
     __syncthreads();
-    finish<T, TOP, LP_WAVES>(row, r, part, LP_WAVES, maxima, top, a);
+    finish<T, TOP, LP_WAVES>(row, r, logit, part[lane & (LP_WAVES - 1)], part, LP_WAVES, maxima, top, a);
 }
 
 // A workgroup a segment of a row.
@@ -343,16 +387,21 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprob_part_kernel(LpArgs a) {
 constexpr int LP_JOIN_WAVES = 8;
 template <typename T, bool TOP>
 __global__ __launch_bounds__(64 * LP_JOIN_WAVES) void logprob_join_kernel(LpArgs a, int segments) {
-    __shared__ int maxima[TOP ? LP_MAX_CHUNKS : 1];
+    __shared__ __attribute__((aligned(16))) int maxima[TOP ? LP_MAX_CHUNKS + 8 : 1];
     __shared__ TopLds<LP_JOIN_WAVES> top[1];
     const int64_t r = blockIdx.x;
+    const int lane = threadIdx.x & 63;
     const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    const float4 *part = a.part + r * segments;
+    const float4 p0 = part[lane < segments ? lane : 0];
+    const float logit = token_logit(row, r, a);
     if (TOP) {
         const int nc = row.chunks();
-        for (int c = threadIdx.x; c < nc; c += 64 * LP_JOIN_WAVES) maxima[c] = a.maxima[r * a.nc + c];
+        for (int c = threadIdx.x; c < nc + 8; c += 64 * LP_JOIN_WAVES)
+            maxima[c] = c < nc ? a.maxima[r * a.nc + c] : NONE;
         __syncthreads();
     }
-    finish<T, TOP, LP_JOIN_WAVES>(row, r, a.part + r * segments, segments, maxima, top, a);
+    finish<T, TOP, LP_JOIN_WAVES>(row, r, logit, p0, part, segments, maxima, top, a);
 }
 
 // Segments of a row: none from 512 rows on (two workgroups a CU by themselves);
