@@ -366,11 +366,13 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
  * chooses the kernels (no request of more than 32 rows of a kv head, or some),
  * and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a workspace of
  * mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte
- * aligned, no initialization needed) long rows' keys are split over workgroups
- * and a second launch adds the parts: the same sums in another order, which
- * depends on all requests' lengths, deterministic for them. NULL, short or
- * misaligned: one workgroup a block of query rows. Calls sharing a workspace must
- * not overlap. */
+ * aligned) long rows' keys are split over workgroups, and a row's last workgroup
+ * adds the parts: the same sums in another order, which depends on all requests'
+ * lengths, deterministic for them. The workspace's first MI_PAGED_ZERO_BYTES (a
+ * fixed prefix, whatever the sizes) are zero before its first use, and every call
+ * leaves them zero. NULL, short or misaligned: one workgroup a block of query
+ * rows. Calls sharing a workspace must not overlap. */
+#define MI_PAGED_ZERO_BYTES 262144
 int64_t mi_paged_attention_workspace_bytes(int64_t T, int64_t R, int64_t table_width, int64_t H,
                                            int64_t HK, int64_t D, int64_t page_size,
                                            int64_t max_q_len);
@@ -389,9 +391,11 @@ int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages, 
  * with a NaN or +inf, or of -inf alone, gives NaN (its top_ids stay in [0, V)).
  * tokens are int32 or int64 (tokens_are_64). Few rows are split over workgroups
  * where a workspace of mi_token_logprobs_workspace_bytes(...) bytes (0: not split;
- * 16-byte aligned, no initialization needed) is given, and joined by a second
- * launch: the same results but for the sums' last bits. NULL, short or misaligned:
- * one workgroup a row. Calls sharing a workspace must not overlap. */
+ * 16-byte aligned) is given: the same results but for the sums' last bits. Its
+ * first MI_LOGPROBS_ZERO_BYTES (a fixed prefix) are zero before its first use, and
+ * every call leaves them zero. NULL, short or misaligned: one workgroup a row.
+ * Calls sharing a workspace must not overlap. */
+#define MI_LOGPROBS_ZERO_BYTES 4096
 int64_t mi_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int top, int dtype);
 int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_stride,
                       const void *tokens, int tokens_are_64, int top, float *logprobs,

@@ -30,6 +30,7 @@ ABI_VERSION = 8
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 MI_OK, MI_ERR_ARG, MI_ERR_UNSUPPORTED, MI_ERR_LAUNCH = 0, 1, 2, 3
 MI_ACT_NONE, MI_ACT_SWIGLU, MI_ACT_GELU = 0, 1, 2
+PAGED_ZERO_BYTES, LOGPROBS_ZERO_BYTES = 262144, 4096  # MI_PAGED_ / MI_LOGPROBS_ZERO_BYTES
 
 _DT = {torch.float32: MI_F32, torch.float16: MI_F16, torch.bfloat16: MI_BF16}
 
@@ -445,7 +446,8 @@ def paged_attention(q, k_pages, v_pages, out, table, cu_q, kv_lens, scale: float
     R, width = table.shape
     stream = _stream(q)
     nbytes = _paged_workspace_bytes(T, R, width, H, HK, D, page, max_q_len)
-    ws = _workspace("paged", q.device, stream, nbytes, 4 << 20).data_ptr() if nbytes else None
+    ws = _workspace("paged", q.device, stream, nbytes, 4 << 20,
+                    zero=PAGED_ZERO_BYTES).data_ptr() if nbytes else None
     _check(lib().mi_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                                     out.data_ptr(), table.data_ptr(), cu_q.data_ptr(),
                                     kv_lens.data_ptr(), T, R, width, H, HK, D, n_pages, page,
@@ -471,7 +473,8 @@ def token_logprobs(x, tokens, top: int, logprobs, entropy, ids, top_logprobs) ->
     rows, V = x.shape
     dt, stream = _dt(x), _stream(x)
     nbytes = _logprobs_workspace_bytes(rows, V, top, dt)
-    ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20).data_ptr() if nbytes else None
+    ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20,
+                    zero=LOGPROBS_ZERO_BYTES).data_ptr() if nbytes else None
     _check(lib().mi_token_logprobs(x.data_ptr(), rows, V, x.stride(0), tokens.data_ptr(),
                                    tokens.dtype is torch.int64, top, logprobs.data_ptr(),
                                    entropy.data_ptr(), ids.data_ptr(), top_logprobs.data_ptr(),
@@ -522,8 +525,9 @@ def b_linear_f32(ins, outs, p):
 
 # Workspaces: scratch of the entries that make several launches or sum across
 # workgroups (the K-part sums of the _ws qmm entries, the split decode's partial
-# states, mi_gelu_mlp_f32's tickets and partial sums). Only the tickets need a
-# zero fill when made (mi_gelu_mlp_f32 leaves them zero after every call).
+# states, the tickets and partial results of mi_gelu_mlp_f32, mi_paged_attention
+# and mi_token_logprobs). Only the tickets need a zero fill when made (every call
+# leaves them zero).
 #
 # Eager calls share one workspace per (thread, kind, device, stream): one
 # thread's calls on one stream run in order, where a second thread may launch
@@ -558,8 +562,16 @@ def graph_workspaces():
 
 
 def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
-               zero: bool = False) -> torch.Tensor:
-    make = torch.zeros if zero else torch.empty
+               zero: bool | int = False) -> torch.Tensor:
+    """zero: all of it, or its first so many bytes, zero when made."""
+    def make(n):
+        if zero is True:
+            return torch.zeros(n, dtype=torch.uint8, device=device)
+        buf = torch.empty(n, dtype=torch.uint8, device=device)
+        if zero:
+            buf[:zero].zero_()
+        return buf
+
     if torch.cuda.is_current_stream_capturing():
         token = getattr(_scope, "token", None)
         key = (kind, device, stream, token)
@@ -567,7 +579,7 @@ def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
         if ws is None or ws.numel() < nbytes:
             if ws is not None:
                 _retired.append(ws)
-            ws = make(max(nbytes, 4096), dtype=torch.uint8, device=device)
+            ws = make(max(nbytes, 4096))
             if token is None:
                 _retired.append(ws)
             else:
@@ -580,7 +592,7 @@ def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
     ws = eager.get(key)
     if ws is None or ws.numel() < nbytes:
         size = max(nbytes, minimum, 0 if ws is None else 2 * ws.numel())
-        eager[key] = ws = make(size, dtype=torch.uint8, device=device)
+        eager[key] = ws = make(size)
     return ws
 
 

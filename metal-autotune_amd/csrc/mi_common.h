@@ -203,6 +203,33 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
+// Partial results that the last workgroup of several to finish reads. They are
+// stored with agent scope (put_part: written through, past the XCD's L2) and
+// acknowledged before the workgroup's ticket is drawn, where a release fence would
+// write back the whole L2; that order rests on the hardware: the store's vmcnt
+// falls once it is visible to the agent, and every wave waits for that count
+// before the barrier. true in every thread of the workgroup that drew the last of n
+// tickets; that one sets the counter back to 0 (tickets are zero before a call and
+// after it).
+__device__ __forceinline__ void put_part(float2 *at, float2 v) {
+    __hip_atomic_store((uint64_t *)at, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool last_of(unsigned *ticket, unsigned n) {
+    __shared__ unsigned drawn;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (drawn == n - 1)
+            __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (drawn != n - 1) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // no stale copy of a partial is read
+    return true;
+}
+
 __host__ __device__ constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline int ilog2(int v) {

@@ -18,8 +18,8 @@
 // (as good as k values in all, but for ties) in a list, a lane an entry.
 //
 // Bound by HBM at many rows (the row's one read, 11 VALU instructions a value of
-// the 13 that fit beside it); by two launches and their trips to memory at few,
-// where a row is split over workgroups.
+// the 13 that fit beside it); by the launch and its trips to memory, one after
+// another, at few, where a row is split over workgroups.
 #include <math.h>
 
 #include "mi_common.h"
@@ -28,7 +28,7 @@ namespace mi {
 namespace {
 
 constexpr int LP_MAX_TOP = 64;   // a lane an entry
-constexpr int LP_WAVES = 4;
+constexpr int LP_WAVES = 4, LP_SPLIT_WAVES = 8;  // of a workgroup that has a row, a part of one
 constexpr int LP_CHUNK = 1024;   // values a chunk, 2 (16 bits) or 4 (fp32) 16-byte pieces a lane
 constexpr int64_t LP_MAX_V = (int64_t)1 << 22;
 constexpr int LP_MAX_CHUNKS = (int)(LP_MAX_V / LP_CHUNK) + 1;  // (the first may begin before the row)
@@ -220,6 +220,7 @@ struct LpArgs {
     float *top_logprobs;
     // rows split over workgroups: of each row its segments' sums and its chunks'
     // maxima, nc a row
+    unsigned *tickets;  // a row
     float4 *part;
     int *maxima;
     int nc, per;  // chunks a segment
@@ -342,98 +343,92 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit
     }
 }
 
-// A workgroup a row.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void logprob_row_kernel(LpArgs a) {
-    __shared__ float4 part[LP_WAVES];
+// SPLIT: a workgroup a segment of a row, whose sums and maxima go to the workspace;
+// the row's last workgroup to finish goes on with them. Else a workgroup a row.
+template <typename T, bool TOP, bool SPLIT>
+__global__ __launch_bounds__(64 * (SPLIT ? LP_SPLIT_WAVES : LP_WAVES)) void logprob_kernel(LpArgs a) {
+    constexpr int WAVES = SPLIT ? LP_SPLIT_WAVES : LP_WAVES;
+    __shared__ float4 part[WAVES];
     __shared__ __attribute__((aligned(16))) int maxima[TOP ? LP_MAX_CHUNKS + 8 : 1];
-    __shared__ TopLds<LP_WAVES> top[1];
+    __shared__ TopLds<WAVES> top[1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t r = blockIdx.x;
+    const int64_t r = SPLIT ? blockIdx.y : blockIdx.x;
     const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
+    const int nc = row.chunks();
     const float logit = token_logit(row, r, a);
-    if (TOP && threadIdx.x < 8) maxima[row.chunks() + threadIdx.x] = NONE;
-    const float4 p = pass<T, TOP, true>(row, wave, row.chunks(), LP_WAVES, maxima, lane);
+    if (TOP && threadIdx.x < 8) maxima[nc + threadIdx.x] = NONE;
+    if constexpr (!SPLIT) {
+        const float4 p = pass<T, TOP, true>(row, wave, nc, WAVES, maxima, lane);
+        if (lane == 0) part[wave] = p;
+        __syncthreads();
+        finish<T, TOP, WAVES>(row, r, logit, part[lane % WAVES], part, WAVES, maxima, top, a);
+        return;
+    }
+    const int c0 = blockIdx.x * a.per, c1 = min(c0 + a.per, nc), segments = gridDim.x;
+    const float4 p = pass<T, TOP, false>(row, c0 + wave, c1, WAVES, maxima, lane);
     if (lane == 0) part[wave] = p;
     __syncthreads();
-    finish<T, TOP, LP_WAVES>(row, r, logit, part[lane & (LP_WAVES - 1)], part, LP_WAVES, maxima, top, a);
-}
-
-// A workgroup a segment of a row.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void logprob_part_kernel(LpArgs a) {
-    __shared__ float4 part[LP_WAVES];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t r = blockIdx.y;
-    const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
-    const int c0 = blockIdx.x * a.per, end = c0 + a.per, nc = row.chunks();
-    const float4 p = pass<T, TOP, false>(row, c0 + wave, end < nc ? end : nc, LP_WAVES,
-                                         a.maxima + r * a.nc, lane);
-    if (lane == 0) part[wave] = p;
-    __syncthreads();
+    int *all = a.maxima + r * a.nc;
+    float4 *sums = a.part + r * segments;
+    if (TOP)
+        for (int c = c0 + threadIdx.x; c < c1; c += 64 * WAVES)
+            __hip_atomic_store(all + c, maxima[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (threadIdx.x == 0) {
         // to the largest reference (each is finite, a segment of -inf alone too)
-        float ref = part[0].x, top = part[0].y, s = 0.0f, e = 0.0f;
-        for (int w = 1; w < LP_WAVES; ++w) ref = fmaxf(ref, part[w].x), top = fmaxf(top, part[w].y);
-        for (int w = 0; w < LP_WAVES; ++w) {
+        float ref = part[0].x, best = part[0].y, s = 0.0f, e = 0.0f;
+        for (int w = 1; w < WAVES; ++w) ref = fmaxf(ref, part[w].x), best = fmaxf(best, part[w].y);
+        for (int w = 0; w < WAVES; ++w) {
             float sw = part[w].z, ew = part[w].w;
             move_ref(sw, ew, part[w].x, ref);
             s += sw;
             e += ew;
         }
-        a.part[r * gridDim.x + blockIdx.x] = make_float4(ref, top, s, e);
+        put_part((float2 *)(sums + blockIdx.x), make_float2(ref, best));
+        put_part((float2 *)(sums + blockIdx.x) + 1, make_float2(s, e));
     }
-}
-constexpr int LP_JOIN_WAVES = 8;
-template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * LP_JOIN_WAVES) void logprob_join_kernel(LpArgs a, int segments) {
-    __shared__ __attribute__((aligned(16))) int maxima[TOP ? LP_MAX_CHUNKS + 8 : 1];
-    __shared__ TopLds<LP_JOIN_WAVES> top[1];
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x & 63;
-    const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
-    const float4 *part = a.part + r * segments;
-    const float4 p0 = part[lane < segments ? lane : 0];
-    const float logit = token_logit(row, r, a);
+    if (!last_of(a.tickets + r, segments)) return;
+    const float4 p0 = sums[lane < segments ? lane : 0];
     if (TOP) {
-        const int nc = row.chunks();
-        for (int c = threadIdx.x; c < nc + 8; c += 64 * LP_JOIN_WAVES)
-            maxima[c] = c < nc ? a.maxima[r * a.nc + c] : NONE;
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) maxima[c] = all[c];
         __syncthreads();
     }
-    finish<T, TOP, LP_JOIN_WAVES>(row, r, logit, p0, part, segments, maxima, top, a);
+    finish<T, TOP, WAVES>(row, r, logit, p0, sums, segments, maxima, top, a);
 }
 
 // Segments of a row: none from 512 rows on (two workgroups a CU by themselves);
-// below, about a thousand workgroups in all, of at least a chunk a wave.
+// below, about 512 workgroups in all, of at least a chunk a wave.
+constexpr int64_t LP_SPLIT_ROWS = 512;
+static_assert(LP_SPLIT_ROWS * 4 <= MI_LOGPROBS_ZERO_BYTES, "a ticket a row");
 struct LpSplit {
     int64_t nc, segments, per;
 };
 inline LpSplit lp_split(int64_t rows, int64_t V, int dtype) {
     LpSplit s;
     s.nc = (V + (dtype == MI_F32 ? 3 : 7) + LP_CHUNK - 1) / LP_CHUNK;
-    const int64_t most = ceil_div(s.nc, LP_WAVES), want = rows < 512 ? ceil_div(1024, rows) : 1;
+    const int64_t most = ceil_div(s.nc, LP_SPLIT_WAVES);
+    const int64_t want = rows < LP_SPLIT_ROWS ? ceil_div(512, rows) : 1;
     s.per = ceil_div(s.nc, want < most ? want : most);
     s.segments = ceil_div(s.nc, s.per);
     return s;
 }
 inline int64_t lp_bytes(const LpSplit &s, int64_t rows, int top) {
-    return s.segments > 1 ? rows * (s.segments * 16 + (top ? s.nc * 4 : 0)) : 0;
+    return s.segments > 1
+               ? MI_LOGPROBS_ZERO_BYTES + rows * (s.segments * 16 + (top ? s.nc * 4 : 0)) : 0;
 }
 
 template <typename T, bool TOP>
-int launch_logprobs(LpArgs a, int64_t rows, const LpSplit &s, void *ws, hipStream_t st) {
+int launch_logprobs(LpArgs a, int64_t rows, const LpSplit &s, char *ws, hipStream_t st) {
     if (!ws) {
-        logprob_row_kernel<T, TOP><<<(unsigned)rows, 64 * LP_WAVES, 0, st>>>(a);
+        logprob_kernel<T, TOP, false><<<(unsigned)rows, 64 * LP_WAVES, 0, st>>>(a);
         return launch_status("token logprobs");
     }
-    a.part = (float4 *)ws;
+    a.tickets = (unsigned *)ws;
+    a.part = (float4 *)(ws + MI_LOGPROBS_ZERO_BYTES);
     a.maxima = (int *)(a.part + rows * s.segments);
     a.nc = (int)s.nc;
     a.per = (int)s.per;
-    logprob_part_kernel<T, TOP>
-        <<<dim3((unsigned)s.segments, (unsigned)rows), 64 * LP_WAVES, 0, st>>>(a);
-    logprob_join_kernel<T, TOP><<<(unsigned)rows, 64 * LP_JOIN_WAVES, 0, st>>>(a, (int)s.segments);
+    logprob_kernel<T, TOP, true>
+        <<<dim3((unsigned)s.segments, (unsigned)rows), 64 * LP_SPLIT_WAVES, 0, st>>>(a);
     return launch_status("token logprobs");
 }
 
@@ -465,10 +460,10 @@ extern "C" int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, in
         return fail(MI_ERR_ARG, "logits are not aligned to their type");
     const LpSplit s = lp_split(rows, V, dtype);
     const int64_t need = lp_bytes(s, rows, top);
-    void *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16) ? workspace
-                                                                                      : nullptr;
+    char *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16)
+                   ? (char *)workspace : nullptr;
     const LpArgs a = {logits, row_stride, tokens, tokens_are_64, (int)V, top, logprobs, entropy,
-                      top_ids, top_logprobs, nullptr, nullptr, 0, 0};
+                      top_ids, top_logprobs, nullptr, nullptr, nullptr, 0, 0};
     hipStream_t st = as_stream(stream);
     auto run = [&](auto tag) {
         typedef decltype(tag) T;

@@ -16,9 +16,9 @@
 // every block are therefore cut into chunks of one size, chosen on the GPU from
 // the lengths of all requests so that the chunks fill the chip (chunk_of), and a
 // workgroup finds its chunk by summing over the requests. A block of one chunk
-// writes its rows; the others' states go to a workspace and
-// paged_combine_kernel folds them. The chunk size, so a row's last bits, depends
-// on the lengths of the whole batch.
+// writes its rows; the others' states go to a workspace, and the last workgroup of
+// a block to finish folds them, in order. The chunk size, so a row's last bits,
+// depends on the lengths of the whole batch.
 #include "mi_attn_common.h"
 
 namespace mi {
@@ -30,7 +30,8 @@ struct PagedArgs {
     const void *q, *k, *v;
     void *out;
     const int *table, *cu_q, *kv_lens;
-    float *part;  // partial states, by item and kv head; null: no block is cut
+    unsigned *tickets;  // by a block's first state and kv head
+    float *part;  // partial states, by state and kv head; null: no block is cut
     int T, R, W, H, HK, G, pages, page_log2;
     int target;     // chunks wanted for a kv head
     int wide_runs;  // the least runs of a wide block's chunk
@@ -54,6 +55,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 constexpr int CHUNK_KEYS = ATT_KT * PA_WAVES;  // keys are cut in multiples of this
+constexpr int MAX_CHUNKS = 128;  // of a block: one workgroup adds them
 
 // One request a lane: its first token, tokens, keys, column blocks (wide: of
 // WIDE_COLS columns) and CHUNK_KEYS runs of keys. (Offsets and lengths are held
@@ -84,15 +86,14 @@ struct PagedItem {
     int cb;          // column block
     int split, ns;   // chunk of the block's keys, chunks
     int runs;        // CHUNK_KEYS runs a chunk
-    int part;        // the chunk's state in the workspace, in states of 32 columns
+    int first;       // the block's first state in the workspace (of 32 columns each)
 };
 
-// Item u (BLOCK: the first chunk of column block u): the wide blocks' chunks
-// first, each kind in the order of requests, of their blocks (a wide request's
+// Item u: the wide blocks' chunks first, each kind in the order of requests, of their blocks (a wide request's
 // last block, which sees the most keys, first), of their chunks. Every wave
 // finds it by itself, 64 requests a step: first the runs of all blocks, which
 // give the size of a chunk, then the chunks up to its own.
-template <bool WIDE, bool BLOCK>
+template <bool WIDE>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
     Req q = load_req<WIDE>(a, lane);
     int runs = 1 << 30;
@@ -115,20 +116,19 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     }
     PagedItem it;
     it.r = -1;
-    int before = 0, states = 0;  // what u counts, and states of 32 columns
+    int before = 0, states = 0;  // items, and states of 32 columns
 #pragma unroll
     for (int kind = WIDE ? 0 : 1; kind < 2; ++kind) {
         const bool wide = kind == 0;
-        const int per = wide ? max(runs, a.wide_runs) : runs;
+        const int scale = wide ? WIDE_COLS / 32 : 1;
         for (int r0 = 0;;) {
             if (a.R > 64) q = load_req<WIDE>(a, r0 + lane);
+            const int per = max(max(runs, wide ? a.wide_runs : 1),
+                                (q.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
             const int ns = max(1, (q.runs + per - 1) / per);
-            const int blocks = wide ? q.wide : q.narrow;
-            const int items = blocks * ns, count = BLOCK ? blocks : items;
-            const int end = before + wave_scan(count);
+            const int blocks = wide ? q.wide : q.narrow, items = blocks * ns;
+            const int end = before + wave_scan(items);
             const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
-            const int scale = wide ? WIDE_COLS / 32 : 1;
-            const int state_end = states + scale * (BLOCK ? wave_scan(items) : end - before);
             if (past) {
                 const int l = __builtin_ctzll(past);
                 it.r = r0 + l;
@@ -137,17 +137,17 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
                 it.n = __builtin_amdgcn_readlane(q.n, l);
                 it.len = __builtin_amdgcn_readlane(q.len, l);
                 it.ns = __builtin_amdgcn_readlane(ns, l);
-                it.runs = per;
-                const int at = u - __builtin_amdgcn_readlane(end - count, l);
-                const int b = BLOCK ? at : at / it.ns;
-                it.split = BLOCK ? 0 : at - b * it.ns;
+                it.runs = __builtin_amdgcn_readlane(per, l);
+                const int before_r = __builtin_amdgcn_readlane(end - items, l);
+                const int b = (u - before_r) / it.ns;
+                it.split = u - before_r - b * it.ns;
                 it.cb = wide ? __builtin_amdgcn_readlane(blocks, l) - 1 - b : b;
-                it.part = __builtin_amdgcn_readlane(state_end - scale * items, l) +
-                          scale * (b * it.ns + it.split);
+                it.first = states + scale * (before_r - before + b * it.ns);
                 return it;
             }
-            before = __builtin_amdgcn_readlane(end, 63);
-            states = __builtin_amdgcn_readlane(state_end, 63);
+            const int all = __builtin_amdgcn_readlane(end, 63);
+            states += scale * (all - before);
+            before = all;
             r0 += 64;
             if (r0 >= a.R) break;
         }
@@ -187,6 +187,73 @@ template <int D> struct PagedLds {
 template <int D> struct PartState {
     static constexpr int WORDS = 32 * (D + 2);
 };
+
+template <int D> __device__ __forceinline__ float *part_at(const PagedArgs &a, int state, int hk) {
+    return a.part + ((int64_t)state * a.HK + hk) * PartState<D>::WORDS;
+}
+
+// A chunk's state has been put: the last workgroup of the block to come here adds
+// the chunks, out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m). A
+// column takes D / 4 lanes of four values; four columns at a time, the 256 / D
+// groups of lanes take every so manyth chunk, in order, and are added in order.
+constexpr int JOIN_COLS = 4;
+template <typename T, int D>
+__device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem &it, int hk,
+                                            int cols, char *lds) {
+#pragma clang fp contract(off)
+    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = 8;
+    if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
+    float4 *acc = (float4 *)lds;                                    // [GROUPS][JOIN_COLS][LANES]
+    float2 *lm = (float2 *)(acc + GROUPS * JOIN_COLS * LANES);      // [GROUPS][JOIN_COLS]
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    const int jc = sub % JOIN_COLS, g = sub / JOIN_COLS;
+    const int have = min(it.n * a.G - it.cb * cols, cols);
+    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS * (cols >> 5);
+    for (int c0 = 0; c0 < have; c0 += JOIN_COLS) {  // (workgroup-uniform)
+        const int col = c0 + jc, c = col < have ? col : 0;
+        const float *base = part_at<D>(a, it.first + (c >> 5), hk);
+        const float *po = base + (c & 31) * D + 4 * lane, *pl = base + 32 * D + 2 * (c & 31);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.0f, m = -INFINITY;
+        auto add = [&](const float4 &v, const float2 &w) {
+            const MergeCoef k = merge_coef(m, w.y);
+            o.x = merge_one(o.x, v.x, k);
+            o.y = merge_one(o.y, v.y, k);
+            o.z = merge_one(o.z, v.z, k);
+            o.w = merge_one(o.w, v.w, k);
+            l = merge_one(l, w.x, k);
+            m = k.m_new;
+        };
+        for (int s0 = g; s0 < it.ns; s0 += GROUPS * IN_FLIGHT) {
+            float4 v[IN_FLIGHT];
+            float2 w[IN_FLIGHT];
+#pragma unroll
+            for (int i = 0; i < IN_FLIGHT; ++i) {
+                const int s = s0 + GROUPS * i;
+                v[i] = *(const float4 *)(po + (s < it.ns ? s : g) * step);
+                w[i] = *(const float2 *)(pl + (s < it.ns ? s : g) * step);
+            }
+#pragma unroll
+            for (int i = 0; i < IN_FLIGHT; ++i)
+                if (s0 + GROUPS * i < it.ns) add(v[i], w[i]);
+        }
+        __syncthreads();
+        acc[(g * JOIN_COLS + jc) * LANES + lane] = o;
+        if (lane == 0) lm[g * JOIN_COLS + jc] = make_float2(l, m);
+        __syncthreads();
+        if (g == 0 && col < have) {
+#pragma unroll
+            for (int i = 1; i < GROUPS; ++i)
+                add(acc[(i * JOIN_COLS + jc) * LANES + lane], lm[i * JOIN_COLS + jc]);
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const int idx = it.cb * cols + col, tok = idx / a.G;
+            T *orow = (T *)a.out +
+                      ((int64_t)(it.q0 + tok) * a.H + hk * a.G + (idx - tok * a.G)) * D;
+            const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+            st8(orow + 4 * lane, pack4<T>(e));
+        }
+    }
+}
 
 #if defined(__HIP_DEVICE_COMPILE__)
 // The pages of a wave's next 64 tiles kt, kt + STEP, ..., one a lane (a tile of
@@ -307,20 +374,26 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     for (int t = 0; t < D / 32; ++t) part_put<D>(mine, st, t, lane);
     part_lm<D>(mine)[lane] = make_float2(st.l, st.m);
     __syncthreads();
-    if (wave >= D / 32) return;
-    const Fold f = fold_streams<D>(part, wave, lane);
-    if (it.ns > 1) {  // (workgroup-uniform)
-        const float l = f.l + __shfl_xor(f.l, 32, 64);
-        float *o = a.part + ((int64_t)it.part * a.HK + hk) * PartState<D>::WORDS;
-        if (!ok) return;
-        float *oc = o + r * D + 32 * wave + 4 * h2;
+    if (wave < D / 32) {
+        const Fold f = fold_streams<D>(part, wave, lane);
+        if (it.ns > 1) {  // (workgroup-uniform)
+            const float l = f.l + __shfl_xor(f.l, 32, 64);
+            float *o = part_at<D>(a, it.first + it.split, hk);
+            if (ok) {
+                float *oc = o + r * D + 32 * wave + 4 * h2;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *(float4 *)(oc + 8 * j) = f.o[j];
-        if (wave == 0 && h2 == 0) *(float2 *)(o + 32 * D + 2 * r) = make_float2(l, f.m);
-        return;
+                for (int j = 0; j < 4; ++j) {
+                    put_part((float2 *)(oc + 8 * j), make_float2(f.o[j].x, f.o[j].y));
+                    put_part((float2 *)(oc + 8 * j + 2), make_float2(f.o[j].z, f.o[j].w));
+                }
+                if (wave == 0 && h2 == 0) put_part((float2 *)(o + 32 * D + 2 * r), make_float2(l, f.m));
+            }
+        } else {
+            const float inv = row_inv(f.l);
+            if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
+        }
     }
-    const float inv = row_inv(f.l);
-    if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
+    if (it.ns > 1) join_chunks<T, D>(a, it, hk, 32, lds);
 }
 
 // A wide block: wave w has the columns 32 w .. 32 w + 31 of the block's 128, and
@@ -402,29 +475,32 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         step(b0, b1, s, s + 1 < stages);
         if (s + 1 < stages) step(b1, b0, s + 1, s + 2 < stages);
     }
-    if (!ok) return;
     if (it.ns > 1) {
-        float *o = a.part + ((int64_t)(it.part + wave) * a.HK + hk) * PartState<D>::WORDS;
+        float *o = part_at<D>(a, it.first + it.split * (WIDE_COLS / 32) + wave, hk);
         const float l = st.l + __shfl_xor(st.l, 32, 64);
+        if (ok) {
 #pragma unroll
-        for (int t = 0; t < D / 32; ++t)
+            for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *(float4 *)(o + r * D + 32 * t + 4 * h2 + 8 * j) =
-                    make_float4(st.o[t][4 * j], st.o[t][4 * j + 1], st.o[t][4 * j + 2], st.o[t][4 * j + 3]);
-        if (h2 == 0) *(float2 *)(o + 32 * D + 2 * r) = make_float2(l, st.m);
+                for (int j = 0; j < 8; ++j)
+                    put_part((float2 *)(o + r * D + 32 * t + 4 * h2 + 8 * (j / 2) + 2 * (j & 1)),
+                             make_float2(st.o[t][2 * j], st.o[t][2 * j + 1]));
+            if (h2 == 0) put_part((float2 *)(o + 32 * D + 2 * r), make_float2(l, st.m));
+        }
+        join_chunks<T, D>(a, it, hk, WIDE_COLS, lds);
         return;
     }
     const float inv = row_inv(st.l);
     T *orow = (T *)a.out + qrow * D;
+    if (ok)
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
+        for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float e[4] = {st.o[t][4 * j] * inv, st.o[t][4 * j + 1] * inv,
-                                st.o[t][4 * j + 2] * inv, st.o[t][4 * j + 3] * inv};
-            st8(orow + 32 * t + 8 * j + 4 * h2, pack4<T>(e));
-        }
+            for (int j = 0; j < 4; ++j) {
+                const float e[4] = {st.o[t][4 * j] * inv, st.o[t][4 * j + 1] * inv,
+                                    st.o[t][4 * j + 2] * inv, st.o[t][4 * j + 3] * inv};
+                st8(orow + 32 * t + 8 * j + 4 * h2, pack4<T>(e));
+            }
 }
 #endif
 
@@ -439,86 +515,13 @@ __global__ __launch_bounds__(64 * PA_WAVES) __attribute__((amdgpu_waves_per_eu(p
 void paged_attn_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
-    const PagedItem it = find_item<WIDE, false>(a, blockIdx.y, threadIdx.x & 63);
+    const PagedItem it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
     if (it.r < 0) return;  // (workgroup-uniform)
     if (WIDE && it.wide)
         wide_block<T, D>(a, it, blockIdx.x, lds);
     else
         narrow_block<T, D>(a, it, blockIdx.x, lds);
 #endif
-}
-
-// The chunks of four columns of a block: out = sum_s w_s O_s / sum_s w_s l_s
-// with w_s = 2^(m_s - max m). A column takes D / 4 lanes of four values; the
-// workgroup's groups of four columns take every so manyth chunk, in order, and
-// the groups are added in order.
-constexpr int COMBINE_COLS = 4;
-template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedArgs a) {
-#pragma clang fp contract(off)
-    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * COMBINE_COLS), IN_FLIGHT = 4;
-    __shared__ float4 acc[GROUPS][COMBINE_COLS][LANES];
-    __shared__ float2 lm[GROUPS][COMBINE_COLS];
-    const int hk = blockIdx.x;
-    const PagedItem it = find_item<WIDE, true>(a, blockIdx.y, threadIdx.x & 63);
-    if (it.r < 0 || it.ns == 1) return;
-    const int cols = WIDE && it.wide ? WIDE_COLS : 32;
-    const int left = min(it.n * a.G - it.cb * cols, cols);
-    if ((int)blockIdx.z * COMBINE_COLS >= left) return;
-    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-    const int col = blockIdx.z * COMBINE_COLS + sub % COMBINE_COLS, g = sub / COMBINE_COLS;
-    const bool ok = col < left;
-    const int c = ok ? col : 0;
-    const float *base =
-        a.part + ((int64_t)(it.part + (c >> 5)) * a.HK + hk) * PartState<D>::WORDS;
-    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS * (cols >> 5);
-    const float *po = base + (c & 31) * D + 4 * lane;
-    const float *pl = base + 32 * D + 2 * (c & 31);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.0f, m = -INFINITY;
-    for (int s0 = g; s0 < it.ns; s0 += GROUPS * IN_FLIGHT) {
-        float4 v[IN_FLIGHT];
-        float2 w[IN_FLIGHT];
-#pragma unroll
-        for (int i = 0; i < IN_FLIGHT; ++i) {
-            const int s = s0 + GROUPS * i;
-            v[i] = *(const float4 *)(po + (s < it.ns ? s : g) * step);
-            w[i] = *(const float2 *)(pl + (s < it.ns ? s : g) * step);
-        }
-#pragma unroll
-        for (int i = 0; i < IN_FLIGHT; ++i) {
-            if (s0 + GROUPS * i < it.ns) {
-                const MergeCoef c = merge_coef(m, w[i].y);
-                o.x = merge_one(o.x, v[i].x, c);
-                o.y = merge_one(o.y, v[i].y, c);
-                o.z = merge_one(o.z, v[i].z, c);
-                o.w = merge_one(o.w, v[i].w, c);
-                l = merge_one(l, w[i].x, c);
-                m = c.m_new;
-            }
-        }
-    }
-    acc[g][sub % COMBINE_COLS][lane] = o;
-    if (lane == 0) lm[g][sub % COMBINE_COLS] = make_float2(l, m);
-    __syncthreads();
-    if (g || !ok) return;
-#pragma unroll
-    for (int i = 1; i < GROUPS; ++i) {
-        const float4 b = acc[i][sub][lane];
-        const float2 w = lm[i][sub];
-        const MergeCoef c = merge_coef(m, w.y);
-        o.x = merge_one(o.x, b.x, c);
-        o.y = merge_one(o.y, b.y, c);
-        o.z = merge_one(o.z, b.z, c);
-        o.w = merge_one(o.w, b.w, c);
-        l = merge_one(l, w.x, c);
-        m = c.m_new;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int idx = it.cb * cols + col, tok = idx / a.G;
-    T *orow = (T *)a.out + ((int64_t)(it.q0 + tok) * a.H + hk * a.G + (idx - tok * a.G)) * D;
-    const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    st8(orow + 4 * lane, pack4<T>(e));
 }
 
 // ---------------------------------------------------------------------------
@@ -571,8 +574,12 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
     g.states = wide * (WIDE_COLS / 32) + narrow;
     return g;
 }
+// The tickets take a fixed prefix of the workspace, so that calls of any sizes can
+// share one whose prefix is zero.
+constexpr int64_t PAGED_TICKETS = MI_PAGED_ZERO_BYTES / 4;
 inline int64_t paged_bytes(const PagedGrid &g, int64_t HK, int64_t D) {
-    return g.cut ? g.states * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+    return g.cut && g.states * HK <= PAGED_TICKETS
+               ? MI_PAGED_ZERO_BYTES + g.states * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
 }
 
 template <typename T, int D, bool WIDE>
@@ -580,15 +587,6 @@ int launch_paged_w(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
     const int64_t blocks = g.wide + g.narrow;
     paged_attn_kernel<T, D, WIDE><<<dim3((unsigned)a.HK, (unsigned)(a.part ? g.items : blocks)),
                                     64 * PA_WAVES, 0, st>>>(a);
-    if (a.part) {
-        // (wide blocks that are never cut come first, and only they have more than
-        // 32 columns: a column group past those is never needed)
-        const int64_t most = g.cut_wide ? WIDE_COLS : 32, all = (int64_t)a.T * a.G;
-        paged_combine_kernel<T, D, WIDE>
-            <<<dim3((unsigned)a.HK, (unsigned)blocks,
-                    (unsigned)ceil_div(all < most ? all : most, COMBINE_COLS)),
-               256, 0, st>>>(a);
-    }
     return launch_status("paged attention");
 }
 template <typename T, int D>
@@ -649,12 +647,13 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
         return fail(MI_ERR_ARG, "paged attention: %lld blocks of query rows, at most 65535",
                     (long long)g.items);
     const int64_t need = paged_bytes(g, HK, D);
-    float *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16)
-                    ? (float *)workspace : nullptr;
+    char *ws = need && workspace && workspace_bytes >= need && aligned(workspace, 16)
+                   ? (char *)workspace : nullptr;
     const float sl = scale * 1.4426950408889634f;
     // (a scale of 0 as the smallest normal: masked scores stay -inf; NaN stays NaN)
     const float mag = fabsf(sl) < 1.17549435e-38f ? 1.17549435e-38f : fabsf(sl);
-    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, ws, (int)T, (int)R,
+    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, (unsigned *)ws,
+                         ws ? (float *)(ws + MI_PAGED_ZERO_BYTES) : nullptr, (int)T, (int)R,
                          (int)table_width, (int)H, (int)HK, (int)(H / HK), (int)n_pages, lp,
                          (int)g.target, (int)g.wide_runs, mag, sl < 0.0f ? 0x80008000u : 0u};
     hipStream_t st = as_stream(stream);
