@@ -387,7 +387,7 @@ int mi_paged_attention(const void *q, const void *k_pages, const void *v_pages, 
  * exp. logprobs[r] = logits[r, tokens[r]] - lse (NaN for a token outside [0, V));
  * entropy[r] = -sum p log p (a logit of -inf adds 0); the `top` most probable
  * tokens, the lowest index first among equal logits: top_ids int32 [rows, top]
- * and top_logprobs [rows, top]. All fp32. 0 <= top <= 64, top <= V <= 2^22. A row
+ * and top_logprobs [rows, top]. All fp32. 0 <= top <= 64, top <= V <= 2^20. A row
  * with a NaN or +inf, or of -inf alone, gives NaN (its top_ids stay in [0, V)).
  * tokens are int32 or int64 (tokens_are_64). Few rows are split over workgroups
  * where a workspace of mi_token_logprobs_workspace_bytes(...) bytes (0: not split;

@@ -206,14 +206,19 @@ __device__ __forceinline__ float row16_sum(float v) {
 // Partial results that the last workgroup of several to finish reads. They are
 // stored with agent scope (put_part: written through, past the XCD's L2) and
 // acknowledged before the workgroup's ticket is drawn, where a release fence would
-// write back the whole L2; that order rests on the hardware: the store's vmcnt
-// falls once it is visible to the agent, and every wave waits for that count
-// before the barrier. true in every thread of the workgroup that drew the last of n
-// tickets; that one sets the counter back to 0 (tickets are zero before a call and
-// after it).
+// write back the whole L2, and read with agent scope (get_part: past the caches),
+// where an acquire fence would empty them; that order rests on the hardware: the
+// store's vmcnt falls once it is visible to the agent, and every wave waits for
+// that count before the barrier. last_of: true in every thread of the workgroup
+// that drew the last of n tickets; that one sets the counter back to 0 (tickets are
+// zero before a call and after it).
 __device__ __forceinline__ void put_part(float2 *at, float2 v) {
     __hip_atomic_store((uint64_t *)at, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
                        __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_part(const float2 *at) {
+    return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t *)at, __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT));
 }
 __device__ __forceinline__ bool last_of(unsigned *ticket, unsigned n) {
     __shared__ unsigned drawn;
@@ -225,9 +230,7 @@ __device__ __forceinline__ bool last_of(unsigned *ticket, unsigned n) {
             __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (drawn != n - 1) return false;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // no stale copy of a partial is read
-    return true;
+    return drawn == n - 1;
 }
 
 __host__ __device__ constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

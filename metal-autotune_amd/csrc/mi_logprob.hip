@@ -30,7 +30,7 @@ namespace {
 constexpr int LP_MAX_TOP = 64;   // a lane an entry
 constexpr int LP_WAVES = 4, LP_SPLIT_WAVES = 8;  // of a workgroup that has a row, a part of one
 constexpr int LP_CHUNK = 1024;   // values a chunk, 2 (16 bits) or 4 (fp32) 16-byte pieces a lane
-constexpr int64_t LP_MAX_V = (int64_t)1 << 22;
+constexpr int64_t LP_MAX_V = (int64_t)1 << 20;
 constexpr int LP_MAX_CHUNKS = (int)(LP_MAX_V / LP_CHUNK) + 1;  // (the first may begin before the row)
 constexpr float LP_LOG2E = 1.4426950408889634f;
 
@@ -107,6 +107,7 @@ __device__ __forceinline__ float of_key(int k) {
 struct TopList {
     int key, id;
     int last_key, last_id;  // what a value has to come before (uniform)
+    float floor;            // a value that it has to reach
 };
 __device__ __forceinline__ bool before(int ka, int ia, int kb, int ib) {
     return ka > kb || (ka == kb && ia < ib);
@@ -117,7 +118,11 @@ __device__ __forceinline__ void top_insert(TopList &l, int key, int id, int k, i
     l.key = lane < at ? l.key : (lane == at ? key : pk);
     l.id = lane < at ? l.id : (lane == at ? id : pi);
     const int lk = __builtin_amdgcn_readlane(l.key, k - 1);
-    if (lk != NONE) l.last_key = lk, l.last_id = __builtin_amdgcn_readlane(l.id, k - 1);
+    if (lk != NONE) {
+        l.last_key = lk;
+        l.last_id = __builtin_amdgcn_readlane(l.id, k - 1);
+        l.floor = of_key(lk);
+    }
 }
 
 // A row as 16-byte pieces from the one that holds its first value; value i of
@@ -229,7 +234,7 @@ struct LpArgs {
 // What follows the pass, by a workgroup of WAVES, from the row's n partial sums (ref,
 // top, s, e) and, in LDS, the keys of its chunks' maxima.
 template <int WAVES> struct TopLds {
-    int sel[LP_MAX_TOP];
+    int rank[LP_MAX_CHUNKS], sel[LP_MAX_TOP];
     int key[WAVES * LP_MAX_TOP], id[WAVES * LP_MAX_TOP];
     int bkey[LP_MAX_TOP], bid[LP_MAX_TOP];
     int count[WAVES];
@@ -241,7 +246,11 @@ template <typename T> __device__ __forceinline__ float token_logit(const Row<T> 
     const int64_t tok = a.wide ? ((const int64_t *)a.tokens)[r] : ((const int *)a.tokens)[r];
     return tok >= 0 && tok < row.V ? (float)row.x[tok] : NAN;
 }
-// p0: partial sum `lane` (any where there is none)
+__device__ __forceinline__ float4 get_sums(const float4 *at) {
+    const float2 a = get_part((const float2 *)at), b = get_part((const float2 *)at + 1);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+// p0: partial sum `lane` (any where there is none; past 64 they are in part)
 template <typename T, bool TOP, int WAVES>
 __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit, float4 p0,
                                        const float4 *part, int n, const int *maxima,
@@ -249,28 +258,34 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (TOP) {
-        // the chunks' ranks (maxima: padded by NONE to a multiple of 8)
+        // the chunks' ranks: a wave compares every chunk, a lane each, with eight
+        // others at a time (maxima: padded by NONE to a multiple of 8; rank: zero)
         const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
-        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) {
-            const int key = maxima[c];
-            int rank = 0;
-            for (int i = 0; i < nc; i += 8) {
-                const int4 u = *(const int4 *)(maxima + i), v = *(const int4 *)(maxima + i + 4);
-                const int e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        for (int i = 8 * wave; i < nc; i += 8 * WAVES) {
+            const int4 u = *(const int4 *)(maxima + i), v = *(const int4 *)(maxima + i + 4);
+            const int e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            for (int c = lane; c < nc; c += 64) {
+                const int key = maxima[c];
+                int rank = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) rank += before(e[j], i + j, key, c);
+                atomicAdd(&t->rank[c], rank);
             }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) {
+            const int rank = t->rank[c];
             if (rank < need) t->sel[rank] = c;
-            if (rank == need - 1) t->floor = need == k ? key : NONE + 1;
+            if (rank == need - 1) t->floor = need == k ? maxima[c] : NONE + 1;
         }
     }
     // every wave adds the partial sums, 64 a step, in one order
     float m = lane < n ? p0.y : -INFINITY;
-    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, part[i].y);
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, get_sums(part + i).y);
     m = wave_max(m);
     float S = 0.0f, E = 0.0f;
     for (int i = lane; i < n; i += 64) {
-        const float4 p = i == lane ? p0 : part[i];
+        const float4 p = i == lane ? p0 : get_sums(part + i);
         float s = p.z, e = p.w;
         move_ref(s, e, p.x, m);
         S += s;
@@ -286,32 +301,46 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit
     if constexpr (TOP) {
         const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
         __syncthreads();
-        TopList l = {NONE, 0x7fffffff, t->floor - 1, 0};
-        for (int j = wave; j < need; j += WAVES) {
-            const int c = t->sel[j];
-            Piece<T> pc[Row<T>::PER];
-            if (row.whole(c)) {
-                uint4 raw[Row<T>::PER];
-                row.template load<false>(c, lane, raw);
-                row.open(raw, pc);
-            } else {
-                row.get_end(c, lane, pc);
+        // (a floor of NONE + 1, every value: its float is a NaN)
+        const int floor = t->floor;
+        TopList l = {NONE, 0x7fffffff, floor - 1, 0, floor == NONE + 1 ? -INFINITY : of_key(floor)};
+        constexpr int PER = Row<T>::PER, BATCH = 4;  // chunks asked for together
+        for (int j0 = wave; j0 < need; j0 += BATCH * WAVES) {
+            uint4 raw[BATCH][PER];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int j = j0 + b * WAVES;
+                if (j < need && row.whole(t->sel[j])) row.template load<false>(t->sel[j], lane, raw[b]);
             }
 #pragma unroll
-            for (int i = 0; i < Row<T>::PER; ++i)
+            for (int b = 0; b < BATCH; ++b) {
+                const int j = j0 + b * WAVES;
+                if (j >= need) break;
+                const int c = __builtin_amdgcn_readfirstlane(t->sel[j]);
+                Piece<T> pc[PER];
+                if (row.whole(c))
+                    row.open(raw[b], pc);
+                else
+                    row.get_end(c, lane, pc);
 #pragma unroll
-                for (int e = 0; e < Row<T>::N; ++e) {
-                    const int id = row.first(c, i, lane) + e;
-                    const int key = id >= 0 && id < row.V ? key_of(pc[i].f[e]) : NONE;
-                    uint64_t in = __builtin_amdgcn_ballot_w64(before(key, id, l.last_key, l.last_id));
-                    while (in) {
-                        const int from = __builtin_ctzll(in);
-                        in &= in - 1;
-                        const int ki = __builtin_amdgcn_readlane(key, from);
-                        const int ii = __builtin_amdgcn_readlane(id, from);
-                        if (before(ki, ii, l.last_key, l.last_id)) top_insert(l, ki, ii, k, lane);
+                for (int i = 0; i < PER; ++i)
+#pragma unroll
+                    for (int e = 0; e < Row<T>::N; ++e) {
+                        // (most values of a chunk: nothing reaches the list's end)
+                        if (!__builtin_amdgcn_ballot_w64(pc[i].f[e] >= l.floor)) continue;
+                        const int id = row.first(c, i, lane) + e;
+                        const int key = id >= 0 && id < row.V ? key_of(pc[i].f[e]) : NONE;
+                        uint64_t in =
+                            __builtin_amdgcn_ballot_w64(before(key, id, l.last_key, l.last_id));
+                        while (in) {
+                            const int from = __builtin_ctzll(in);
+                            in &= in - 1;
+                            const int ki = __builtin_amdgcn_readlane(key, from);
+                            const int ii = __builtin_amdgcn_readlane(id, from);
+                            if (before(ki, ii, l.last_key, l.last_id)) top_insert(l, ki, ii, k, lane);
+                        }
                     }
-                }
+            }
         }
         // the best k of the waves' lists, by counting what comes before each entry
         const bool mine = lane < k && l.key != NONE;
@@ -356,7 +385,10 @@ __global__ __launch_bounds__(64 * (SPLIT ? LP_SPLIT_WAVES : LP_WAVES)) void logp
     const Row<T> row((const T *)a.x + r * a.row_stride, a.V);
     const int nc = row.chunks();
     const float logit = token_logit(row, r, a);
-    if (TOP && threadIdx.x < 8) maxima[nc + threadIdx.x] = NONE;
+    if (TOP) {
+        if (threadIdx.x < 8) maxima[nc + threadIdx.x] = NONE;
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) top->rank[c] = 0;
+    }
     if constexpr (!SPLIT) {
         const float4 p = pass<T, TOP, true>(row, wave, nc, WAVES, maxima, lane);
         if (lane == 0) part[wave] = p;
@@ -387,9 +419,10 @@ __global__ __launch_bounds__(64 * (SPLIT ? LP_SPLIT_WAVES : LP_WAVES)) void logp
         put_part((float2 *)(sums + blockIdx.x) + 1, make_float2(s, e));
     }
     if (!last_of(a.tickets + r, segments)) return;
-    const float4 p0 = sums[lane < segments ? lane : 0];
+    const float4 p0 = get_sums(sums + (lane < segments ? lane : 0));
     if (TOP) {
-        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) maxima[c] = all[c];
+        for (int c = threadIdx.x; c < nc; c += 64 * WAVES) 
+            maxima[c] = __hip_atomic_load(all + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
     }
     finish<T, TOP, WAVES>(row, r, logit, p0, sums, segments, maxima, top, a);
@@ -448,7 +481,7 @@ extern "C" int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, in
                                  void *workspace, int64_t workspace_bytes, void *stream) {
     if (!valid_dtype(dtype)) return fail(MI_ERR_UNSUPPORTED, "dtype code %d", dtype);
     if (rows < 0 || rows > 0x7fffffff || V < 1 || V > LP_MAX_V || row_stride < 0)
-        return fail(MI_ERR_ARG, "token logprobs rows=%lld V=%lld (1 to 2^22) row stride %lld",
+        return fail(MI_ERR_ARG, "token logprobs rows=%lld V=%lld (1 to 2^20) row stride %lld",
                     (long long)rows, (long long)V, (long long)row_stride);
     if (top < 0 || top > LP_MAX_TOP || top > V)
         return fail(MI_ERR_ARG, "token logprobs top=%d: 0 to %d, at most V=%lld", top, LP_MAX_TOP,

@@ -230,8 +230,11 @@ __device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem 
 #pragma unroll
             for (int i = 0; i < IN_FLIGHT; ++i) {
                 const int s = s0 + GROUPS * i;
-                v[i] = *(const float4 *)(po + (s < it.ns ? s : g) * step);
-                w[i] = *(const float2 *)(pl + (s < it.ns ? s : g) * step);
+                const int64_t at = (s < it.ns ? s : g) * step;
+                const float2 a0 = get_part((const float2 *)(po + at));
+                const float2 a1 = get_part((const float2 *)(po + at + 2));
+                v[i] = make_float4(a0.x, a0.y, a1.x, a1.y);
+                w[i] = get_part((const float2 *)(pl + at));
             }
 #pragma unroll
             for (int i = 0; i < IN_FLIGHT; ++i)
