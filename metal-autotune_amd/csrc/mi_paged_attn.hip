@@ -158,7 +158,9 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
 #if defined(__HIP_DEVICE_COMPILE__)
 // The DMA of one key tile of K or V: rows [0, left) of it (at most 32) lie at
 // lo (rows 0..15) and hi (rows 16..31, its own 16 rows); the rest arrive as zeros.
-template <typename T, int D, bool ISV>
+// NT: non-temporal, for what is read once (decode: 48 requests of 64 to 8191 keys
+// 152 -> 136 us; wide blocks, which share keys through the L2, 97 -> 105 with it).
+template <typename T, int D, bool ISV, bool NT>
 __device__ __forceinline__ void dma_paged_tile(const T *lo, const T *hi, int left, char *dst,
                                                int lane) {
     typedef Tile<D> Tl;
@@ -172,7 +174,7 @@ __device__ __forceinline__ void dma_paged_tile(const T *lo, const T *hi, int lef
         const int c = pos ^ (ISV ? swz_v<D>(row) : swz_k<D>(row));
         const bool second = i * Tl::RPI >= 16;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(second ? r1 : r0, (lds_ptr)(dst + i * 1024), 16,
-                                                 ((row & 15) * D + 8 * c) * 2, 0, 0, 0);
+                                                 ((row & 15) * D + 8 * c) * 2, 0, 0, NT ? 2 : 0);
     }
 }
 #endif
@@ -201,7 +203,7 @@ template <typename T, int D>
 __device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem &it, int hk,
                                             int cols, char *lds) {
 #pragma clang fp contract(off)
-    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = 8;
+    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = 16;
     if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
     float4 *acc = (float4 *)lds;                                    // [GROUPS][JOIN_COLS][LANES]
     float2 *lm = (float2 *)(acc + GROUPS * JOIN_COLS * LANES);      // [GROUPS][JOIN_COLS]
@@ -323,8 +325,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             int64_t lo, hi;
             pg.rows(0, t0 * ATT_KT, lo, hi);
             const int left = it.len - t0 * ATT_KT;
-            dma_paged_tile<T, D, false>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left, ks, lane);
-            dma_paged_tile<T, D, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left, vs, lane);
+            dma_paged_tile<T, D, false, true>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left, ks, lane);
+            dma_paged_tile<T, D, true, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left, vs, lane);
         }
         for (int kt = t0; kt < ntiles; kt += PA_WAVES) {  // wave-uniform
             const int nx = kt + PA_WAVES;
@@ -346,7 +348,7 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             for (int s = 0; s < D / 16; ++s) launder(kf[s]);  // the reads have returned
             __builtin_amdgcn_sched_barrier(0);
             if (more)
-                dma_paged_tile<T, D, false>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left,
+                dma_paged_tile<T, D, false, true>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left,
                                             ks, lane);
             f32x16 s = attn_scores<T, D>(kf, qf);
             const int k0 = kt * ATT_KT;
@@ -363,7 +365,7 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             __builtin_amdgcn_sched_barrier(0);
             att_wait_lds();  // V's reads have returned
             if (more)
-                dma_paged_tile<T, D, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left,
+                dma_paged_tile<T, D, true, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left,
                                            vs, lane);
         }
     };
@@ -441,9 +443,9 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         pg.rows(s, kt * ATT_KT, lo, hi);
         const int left = it.len - kt * ATT_KT;
         if (wave < 2)
-            dma_paged_tile<T, D, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+            dma_paged_tile<T, D, false, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
         else
-            dma_paged_tile<T, D, true>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+            dma_paged_tile<T, D, true, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
     };
     auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more)
                     __attribute__((always_inline)) {
