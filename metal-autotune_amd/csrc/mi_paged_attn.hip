@@ -203,7 +203,7 @@ template <typename T, int D>
 __device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem &it, int hk,
                                             int cols, char *lds) {
 #pragma clang fp contract(off)
-    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = 16;
+    constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = D == 64 ? 8 : 16;
     if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
     float4 *acc = (float4 *)lds;                                    // [GROUPS][JOIN_COLS][LANES]
     float2 *lm = (float2 *)(acc + GROUPS * JOIN_COLS * LANES);      // [GROUPS][JOIN_COLS]
@@ -401,6 +401,45 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     if (it.ns > 1) join_chunks<T, D>(a, it, hk, 32, lds);
 }
 
+// attn_softmax over two key tiles.
+template <typename T, int D>
+__device__ __forceinline__ void softmax_pair(AttnState<D> &st, const f32x16 (&s)[2],
+                                             uint32_t (&pk)[2][8], float scale) {
+#pragma clang fp contract(off)
+    float mt[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        mt[j] = fmaxf(s[j][0], s[j][1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) mt[j] = fmaxf(fmaxf(mt[j], s[j][i]), s[j][i + 1]);
+    }
+    const float m = max_halves(fmaxf(mt[0], mt[1])) * scale;
+    const bool grow = m > st.m + 8.0f;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float m_new = grow ? m : st.m;
+        const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - m_new);
+        st.l *= corr;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[t][i] *= corr;
+        st.m = m_new;
+    }
+    const float nm = st.m == -INFINITY ? 0.0f : -st.m;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][2 * i], scale, nm));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][2 * i + 1], scale, nm));
+            pk[j][i] = pk2<T>(p0, p1);
+            sum[2 * (i & 1)] += p0;
+            sum[2 * (i & 1) + 1] += p1;
+        }
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 // A wide block: wave w has the columns 32 w .. 32 w + 31 of the block's 128, and
 // all four share each stage of two key tiles, staged by DMA into one of two
 // buffers while the other is read: K and V pass through LDS once for 128 columns
@@ -455,23 +494,29 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         __syncthreads();
         flip_q<D>(qf, flip);
         if (more) issue(s + 1, nb);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int kt = t0 + 2 * s + j;
-            if (kt < mine) {  // wave-uniform
-                uint4 kf[D / 16];
-                read_k<D>(cb + j * Tl::BYTES, kf, r, h2);
-                VFrag<T, D> vf;
-                read_v<T, D>(cb + (2 + j) * Tl::BYTES, vf, lane);
-                __builtin_amdgcn_sched_barrier(0);  // (not sunk to the PV MFMAs)
-                f32x16 sc = attn_scores<T, D>(kf, qf);
-                const int k0 = kt * ATT_KT;
-                if (k0 + ATT_KT > full) attn_mask(sc, end - k0, h2);
-                uint32_t p[8];
-                attn_softmax<T, D>(st, sc, p, a.scale);
-                attn_pv<T, D>(st, p, vf);
-            }
+        const int kt = t0 + 2 * s;
+        if (kt >= mine) return;  // (wave-uniform)
+        // both tiles: two chains of score MFMAs, one running maximum
+        f32x16 sc[2];
+        {
+            uint4 kf[D / 16];
+            read_k<D>(cb, kf, r, h2);
+            sc[0] = attn_scores<T, D>(kf, qf);
+            read_k<D>(cb + Tl::BYTES, kf, r, h2);
+            sc[1] = attn_scores<T, D>(kf, qf);
         }
+        VFrag<T, D> vf;
+        read_v<T, D>(cb + 2 * Tl::BYTES, vf, lane);
+        const int k0 = kt * ATT_KT;
+        if (k0 + 2 * ATT_KT > full) {
+            attn_mask(sc[0], end - k0, h2);
+            attn_mask(sc[1], end - k0 - ATT_KT, h2);
+        }
+        uint32_t p[2][8];
+        softmax_pair<T, D>(st, sc, p, a.scale);
+        attn_pv<T, D>(st, p[0], vf);
+        read_v<T, D>(cb + 3 * Tl::BYTES, vf, lane);
+        attn_pv<T, D>(st, p[1], vf);
     };
     const int stages = t1 > t0 ? (t1 - t0 + 1) / 2 : 0;
     char *b0 = lds, *b1 = lds + STAGE;
