@@ -89,10 +89,21 @@ struct PagedItem {
     int first;       // the block's first state in the workspace (of 32 columns each)
 };
 
-// Item u: the wide blocks' chunks first, each kind in the order of requests, of their blocks (a wide request's
-// last block, which sees the most keys, first), of their chunks. Every wave
-// finds it by itself, 64 requests a step: first the runs of all blocks, which
-// give the size of a chunk, then the chunks up to its own.
+// The wide blocks of a lane's request that see at least L runs of keys, its last
+// ones: block cb's last token is min((128 cb + 127) / G, n - 1), which sees len - n
+// keys and those up to its own.
+__device__ __forceinline__ int blocks_from(const PagedArgs &a, const Req &q, int L) {
+    const int y = (L - 1) * CHUNK_KEYS - (q.len - q.n);  // the first token that does
+    if (y >= q.n && L > 0) return 0;
+    return y <= 0 || L == 0 ? q.wide : q.wide - min(y * a.G / WIDE_COLS, q.wide - 1);
+}
+
+// Item u: the wide blocks' chunks first, then the narrow ones', in the order of
+// requests, of their blocks, of their chunks; but the wide ones of at most 64
+// requests from those that see the most keys to those that see the fewest, since
+// a long one that starts last would run on alone (four prompts of 2048 tokens: 203
+// -> 165 us). Every wave finds its item by itself, 64 requests a step: first the
+// runs of all blocks, which give the size of a chunk, then the chunks up to its own.
 template <bool WIDE>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
     Req q = load_req<WIDE>(a, lane);
@@ -121,6 +132,39 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     for (int kind = WIDE ? 0 : 1; kind < 2; ++kind) {
         const bool wide = kind == 0;
         const int scale = wide ? WIDE_COLS / 32 : 1;
+        if (wide && a.R <= 64) {
+            const int per = max(max(runs, a.wide_runs), (q.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
+            const int ns = max(1, (q.runs + per - 1) / per);
+            const int end = wave_scan(q.wide * ns);
+            before = __builtin_amdgcn_readlane(end, 63);
+            states = scale * before;
+            if (u >= before) continue;
+            // the largest L of which more than u items see at least L runs
+            int lo = 0, hi = ((a.W << a.page_log2) + CHUNK_KEYS - 1) / CHUNK_KEYS + 1, above = 0;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                const int n = __builtin_amdgcn_readlane(wave_scan(blocks_from(a, q, mid) * ns), 63);
+                if (n > u)
+                    lo = mid;
+                else
+                    hi = mid, above = n;
+            }
+            const int have = blocks_from(a, q, lo), at = (have - blocks_from(a, q, lo + 1)) * ns;
+            const int upto = above + wave_scan(at);
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > u));
+            it.r = l;
+            it.wide = true;
+            it.q0 = __builtin_amdgcn_readlane(q.q0, l);
+            it.n = __builtin_amdgcn_readlane(q.n, l);
+            it.len = __builtin_amdgcn_readlane(q.len, l);
+            it.ns = __builtin_amdgcn_readlane(ns, l);
+            it.runs = __builtin_amdgcn_readlane(per, l);
+            const int p = u - __builtin_amdgcn_readlane(upto - at, l), b = p / it.ns;
+            it.split = p - b * it.ns;
+            it.cb = __builtin_amdgcn_readlane(q.wide - have, l) + b;
+            it.first = scale * (__builtin_amdgcn_readlane(end - q.wide * ns, l) + it.cb * it.ns);
+            return it;
+        }
         for (int r0 = 0;;) {
             if (a.R > 64) q = load_req<WIDE>(a, r0 + lane);
             const int per = max(max(runs, wide ? a.wide_runs : 1),
