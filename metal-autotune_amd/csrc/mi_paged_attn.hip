@@ -78,13 +78,21 @@ template <bool WIDE> __device__ __forceinline__ Req load_req(const PagedArgs &a,
     return q;
 }
 
+// Runs that the lane's request's blocks read on average (a wide request's first
+// block sees fewer keys than its last).
+__device__ __forceinline__ int mean_runs(const PagedArgs &a, const Req &q) {
+    const int first = q.len - q.n + min(WIDE_COLS / a.G + 1, q.n);
+    return q.wide ? (q.runs + (max(first, 0) + CHUNK_KEYS - 1) / CHUNK_KEYS + 1) / 2 : q.runs;
+}
+
 // The work of one workgroup beside its kv head.
 struct PagedItem {
     int r;           // request, < 0: none
     bool wide;
     int q0, n, len;  // its first token, its tokens, its keys
     int cb;          // column block
-    int split, ns;   // chunk of the block's keys, chunks
+    int split, ns;   // chunk of the block's keys, chunks (a request's earlier wide
+                     // blocks have fewer than its last: split >= ns is no work)
     int runs;        // CHUNK_KEYS runs a chunk
     int first;       // the block's first state in the workspace (of 32 columns each)
 };
@@ -112,7 +120,7 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
         // (blocks < 2^16 and runs < 2^23: summed in two halves)
         uint64_t total = 0;
         for (int r0 = 0;;) {
-            const uint64_t mine = (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)q.runs;
+            const uint64_t mine = (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)mean_runs(a, q);
             const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
             total += (uint64_t)(unsigned)__builtin_amdgcn_readlane(lo, 63) +
                      ((uint64_t)(unsigned)__builtin_amdgcn_readlane(hi, 63) << 24);
@@ -229,23 +237,26 @@ template <int D> struct PagedLds {
     static constexpr int BYTES = SLOTS > FOLD ? SLOTS : FOLD;
 };
 
-// A chunk's state in the workspace: 32 columns of D sums, then of (l, m).
+// A chunk's state in the workspace, of 32 columns, in whole lines of a wave's
+// stores (written past the caches, pieces of a line cost a line each): a narrow
+// block's is columns of D sums, then of (l, m); a wide one's is the registers' pairs
+// by lane, then (l, m) by lane.
 template <int D> struct PartState {
-    static constexpr int WORDS = 32 * (D + 2);
+    static constexpr int WORDS = 32 * D + 128;
 };
 
 template <int D> __device__ __forceinline__ float *part_at(const PagedArgs &a, int state, int hk) {
     return a.part + ((int64_t)state * a.HK + hk) * PartState<D>::WORDS;
 }
 
-// A chunk's state has been put: the last workgroup of the block to come here adds
+// A narrow block's chunk has been put: the last workgroup of it to come here adds
 // the chunks, out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m). A
 // column takes D / 4 lanes of four values; four columns at a time, the 256 / D
 // groups of lanes take every so manyth chunk, in order, and are added in order.
 constexpr int JOIN_COLS = 4;
 template <typename T, int D>
-__device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem &it, int hk,
-                                            int cols, char *lds) {
+__device__ __forceinline__ void join_narrow(const PagedArgs &a, const PagedItem &it, int hk,
+                                            int have, char *lds) {
 #pragma clang fp contract(off)
     constexpr int LANES = D / 4, GROUPS = 256 / (LANES * JOIN_COLS), IN_FLIGHT = D == 64 ? 8 : 16;
     if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
@@ -253,12 +264,11 @@ __device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem 
     float2 *lm = (float2 *)(acc + GROUPS * JOIN_COLS * LANES);      // [GROUPS][JOIN_COLS]
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const int jc = sub % JOIN_COLS, g = sub / JOIN_COLS;
-    const int have = min(it.n * a.G - it.cb * cols, cols);
-    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS * (cols >> 5);
+    const int64_t step = (int64_t)a.HK * PartState<D>::WORDS;
     for (int c0 = 0; c0 < have; c0 += JOIN_COLS) {  // (workgroup-uniform)
         const int col = c0 + jc, c = col < have ? col : 0;
-        const float *base = part_at<D>(a, it.first + (c >> 5), hk);
-        const float *po = base + (c & 31) * D + 4 * lane, *pl = base + 32 * D + 2 * (c & 31);
+        const float *base = part_at<D>(a, it.first, hk);
+        const float *po = base + c * D + 4 * lane, *pl = base + 32 * D + 2 * c;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.0f, m = -INFINITY;
         auto add = [&](const float4 &v, const float2 &w) {
@@ -295,7 +305,7 @@ __device__ __forceinline__ void join_chunks(const PagedArgs &a, const PagedItem 
             for (int i = 1; i < GROUPS; ++i)
                 add(acc[(i * JOIN_COLS + jc) * LANES + lane], lm[i * JOIN_COLS + jc]);
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const int idx = it.cb * cols + col, tok = idx / a.G;
+            const int idx = it.cb * 32 + col, tok = idx / a.G;
             T *orow = (T *)a.out +
                       ((int64_t)(it.q0 + tok) * a.H + hk * a.G + (idx - tok * a.G)) * D;
             const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
@@ -423,26 +433,30 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     for (int t = 0; t < D / 32; ++t) part_put<D>(mine, st, t, lane);
     part_lm<D>(mine)[lane] = make_float2(st.l, st.m);
     __syncthreads();
-    if (wave < D / 32) {
-        const Fold f = fold_streams<D>(part, wave, lane);
-        if (it.ns > 1) {  // (workgroup-uniform)
-            const float l = f.l + __shfl_xor(f.l, 32, 64);
-            float *o = part_at<D>(a, it.first + it.split, hk);
-            if (ok) {
-                float *oc = o + r * D + 32 * wave + 4 * h2;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    put_part((float2 *)(oc + 8 * j), make_float2(f.o[j].x, f.o[j].y));
-                    put_part((float2 *)(oc + 8 * j + 2), make_float2(f.o[j].z, f.o[j].w));
-                }
-                if (wave == 0 && h2 == 0) put_part((float2 *)(o + 32 * D + 2 * r), make_float2(l, f.m));
-            }
-        } else {
-            const float inv = row_inv(f.l);
-            if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
-        }
+    Fold f;
+    if (wave < D / 32) f = fold_streams<D>(part, wave, lane);
+    if (it.ns == 1) {  // (workgroup-uniform)
+        if (wave >= D / 32) return;
+        const float inv = row_inv(f.l);
+        if (ok) store_fold<T>(f, inv, (T *)a.out + qrow * D, wave, h2);
+        return;
     }
-    if (it.ns > 1) join_chunks<T, D>(a, it, hk, 32, lds);
+    __syncthreads();  // every wave has folded; the state by columns, then out
+    float *cols_at = (float *)lds;  // [32][D], [32] (l, m)
+    if (wave < D / 32) {
+        const float l = f.l + __shfl_xor(f.l, 32, 64);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(float4 *)(cols_at + r * D + 32 * wave + 8 * j + 4 * h2) = f.o[j];
+        if (wave == 0 && h2 == 0) *(float2 *)(cols_at + 32 * D + 2 * r) = make_float2(l, f.m);
+    }
+    __syncthreads();
+    float *o = part_at<D>(a, it.first + it.split, hk);
+    const int have = min(cols - it.cb * 32, 32);
+    for (int i = 2 * threadIdx.x; i < have * D; i += 128 * PA_WAVES)
+        put_part((float2 *)(o + i), *(float2 *)(cols_at + i));
+    if ((int)threadIdx.x < have)
+        put_part((float2 *)(o + 32 * D) + threadIdx.x, *(float2 *)(cols_at + 32 * D + 2 * threadIdx.x));
+    join_narrow<T, D>(a, it, hk, have, lds);
 }
 
 // attn_softmax over two key tiles.
@@ -570,19 +584,32 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         if (s + 1 < stages) step(b1, b0, s + 1, s + 2 < stages);
     }
     if (it.ns > 1) {
-        float *o = part_at<D>(a, it.first + it.split * (WIDE_COLS / 32) + wave, hk);
-        const float l = st.l + __shfl_xor(st.l, 32, 64);
-        if (ok) {
+        // the state out; the last workgroup of the block to come here folds all of
+        // them, in order, each wave its own columns'
+        constexpr int PAIRS = D / 32 * 8;
+        float2 *o = (float2 *)part_at<D>(a, it.first + it.split * (WIDE_COLS / 32) + wave, hk) + lane;
 #pragma unroll
-            for (int t = 0; t < D / 32; ++t)
+        for (int i = 0; i < PAIRS; ++i)
+            put_part(o + 64 * i, make_float2(st.o[i / 8][2 * (i % 8)], st.o[i / 8][2 * (i % 8) + 1]));
+        put_part(o + 64 * PAIRS, make_float2(st.l, st.m));
+        if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
+        attn_init(st);
+        for (int s = 0; s < it.ns; ++s) {
+            const float2 *p =
+                (const float2 *)part_at<D>(a, it.first + s * (WIDE_COLS / 32) + wave, hk) + lane;
+            float2 v[PAIRS + 1];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    put_part((float2 *)(o + r * D + 32 * t + 4 * h2 + 8 * (j / 2) + 2 * (j & 1)),
-                             make_float2(st.o[t][2 * j], st.o[t][2 * j + 1]));
-            if (h2 == 0) put_part((float2 *)(o + 32 * D + 2 * r), make_float2(l, st.m));
+            for (int i = 0; i <= PAIRS; ++i) v[i] = get_part(p + 64 * i);
+            const MergeCoef c = merge_coef(st.m, v[PAIRS].y);
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                const int t = i / 8, e = 2 * (i % 8);
+                st.o[t][e] = merge_one(st.o[t][e], v[i].x, c);
+                st.o[t][e + 1] = merge_one(st.o[t][e + 1], v[i].y, c);
+            }
+            st.l = merge_one(st.l, v[PAIRS].x, c);
+            st.m = c.m_new;
         }
-        join_chunks<T, D>(a, it, hk, WIDE_COLS, lds);
-        return;
     }
     const float inv = row_inv(st.l);
     T *orow = (T *)a.out + qrow * D;
@@ -609,12 +636,22 @@ __global__ __launch_bounds__(64 * PA_WAVES) __attribute__((amdgpu_waves_per_eu(p
 void paged_attn_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
-    const PagedItem it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
+    PagedItem it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
     if (it.r < 0) return;  // (workgroup-uniform)
-    if (WIDE && it.wide)
+    if (WIDE && it.wide) {
+        if (it.ns > 1) {
+            // the block's own chunks, of equal sizes
+            const int last = min((it.cb * WIDE_COLS + WIDE_COLS - 1) / a.G, it.n - 1);
+            const int keys = max(it.len - it.n + last + 1, 1);
+            const int runs = (keys + CHUNK_KEYS - 1) / CHUNK_KEYS;
+            it.ns = (runs + it.runs - 1) / it.runs;
+            it.runs = (runs + it.ns - 1) / it.ns;
+            if (it.split >= it.ns) return;
+        }
         wide_block<T, D>(a, it, blockIdx.x, lds);
-    else
+    } else {
         narrow_block<T, D>(a, it, blockIdx.x, lds);
+    }
 #endif
 }
 
@@ -626,8 +663,10 @@ void paged_attn_kernel(PagedArgs a) {
 // at most `target` chunks and the last, shorter one of every block, and no more
 // than a row of the table has. Few blocks: as many chunks as one round of
 // workgroups takes with those last ones; many: four rounds' worth, so that what
-// the last round leaves idle is small, and wide blocks, whose parts cost 66 KB
-// written and read, only past 32 runs.
+// the last round leaves idle is small. Wide blocks, whose parts cost 66 KB written
+// and read, are then cut only where they fill less than two rounds, past 32 runs
+// (20 requests, four of 256 to 512 tokens and up to 4096 keys: 90 us; from 8 runs
+// on, 103; 8192 tokens of one prompt uncut 562 us, cut past 32 runs 694).
 struct PagedGrid {
     int64_t wide, narrow, items, states, target, wide_runs;
     bool cut, cut_wide;
@@ -651,20 +690,21 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
     const int64_t few = slots - (g.wide + g.narrow) * HK;
     g.target = (few >= slots / 2 ? few : 4 * slots) / HK;
     if (g.target < 1) g.target = 1;
-    g.wide_runs = few >= slots / 2 ? 1 : 32;
+    g.wide_runs = few >= slots / 2 ? 1 : g.wide * HK < 2 * slots ? 32 : 1 << 23;
     g.cut = runs > 1;
     g.cut_wide = g.wide && runs > g.wide_runs;
     int64_t wide = g.wide, narrow = g.narrow;  // chunks of each kind
     if (g.cut_wide) {
-        const int64_t most = g.wide * ceil_div(runs, g.wide_runs);
-        wide = g.wide + g.target < most ? g.wide + g.target : most;
+        // (the chunks are counted by a request's last block, their size comes from
+        // the mean: up to twice as many)
+        const int64_t most = g.wide * ceil_div(runs, g.wide_runs), some = g.wide + 2 * g.target;
+        wide = some < most ? some : most;
     }
     if (g.cut) {
         const int64_t most = g.narrow * runs;
         narrow = g.narrow + g.target < most ? g.narrow + g.target : most;
     }
     g.items = wide + narrow;
-    if (g.items > g.wide + g.narrow + g.target) g.items = g.wide + g.narrow + g.target;
     g.states = wide * (WIDE_COLS / 32) + narrow;
     return g;
 }
@@ -673,7 +713,7 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
 constexpr int64_t PAGED_TICKETS = MI_PAGED_ZERO_BYTES / 4;
 inline int64_t paged_bytes(const PagedGrid &g, int64_t HK, int64_t D) {
     return g.cut && g.states * HK <= PAGED_TICKETS
-               ? MI_PAGED_ZERO_BYTES + g.states * HK * 32 * (D + 2) * (int64_t)sizeof(float) : 0;
+               ? MI_PAGED_ZERO_BYTES + g.states * HK * (32 * D + 128) * (int64_t)sizeof(float) : 0;
 }
 
 template <typename T, int D, bool WIDE>
