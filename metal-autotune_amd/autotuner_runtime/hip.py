@@ -468,7 +468,7 @@ def _logprobs_workspace_bytes(rows, V, top, dt) -> int:
     return int(lib().mi_token_logprobs_workspace_bytes(rows, V, top, dt))
 
 
-def token_logprobs(x, tokens, top: int, logprobs, entropy, ids, top_logprobs) -> None:
+def token_logprobs(x, tokens, wide: bool, top: int, logprobs, entropy, ids, top_logprobs) -> None:
     """mi_token_logprobs over checked tensors, with the workspace of split rows."""
     rows, V = x.shape
     dt, stream = _dt(x), _stream(x)
@@ -476,7 +476,7 @@ def token_logprobs(x, tokens, top: int, logprobs, entropy, ids, top_logprobs) ->
     ws = _workspace("logprobs", x.device, stream, nbytes, 1 << 20,
                     zero=LOGPROBS_ZERO_BYTES).data_ptr() if nbytes else None
     _check(lib().mi_token_logprobs(x.data_ptr(), rows, V, x.stride(0), tokens.data_ptr(),
-                                   tokens.dtype is torch.int64, top, logprobs.data_ptr(),
+                                   wide, top, logprobs.data_ptr(),
                                    entropy.data_ptr(), ids.data_ptr(), top_logprobs.data_ptr(),
                                    dt, ws, nbytes, stream), "token_logprobs")
 

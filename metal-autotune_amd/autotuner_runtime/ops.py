@@ -484,24 +484,27 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     index first among equal logits. Logits of -inf are forbidden tokens."""
     if not logits.is_cuda:
         hip._require_gpu(logits)
-    *lead, V = logits.shape
-    if list(tokens.shape) != lead or (tokens.dtype is not torch.int64 and tokens.dtype is not _I32) \
+    shape = logits.shape
+    lead, V = shape[:-1], shape[-1]
+    wide = tokens.dtype is torch.int64
+    if tokens.shape != lead or not (wide or tokens.dtype is _I32) \
             or tokens.get_device() != logits.get_device():
         raise ValueError(f"token_logprobs: tokens must be int32 or int64 {tuple(lead)} on "
                          f"{logits.device}")
-    if V < 1 or not 0 <= top <= 64 or top > V:
+    if not 0 <= top <= 64 or top > V or V < 1:
         raise ValueError(f"token_logprobs: top={top} of V={V} (0 to 64, at most V)")
     x = logits
-    if x.stride(-1) != 1 or (len(lead) != 1 and not x.is_contiguous()):
+    if not x.is_contiguous() and (x.stride(-1) != 1 or len(lead) != 1):
         x = x.contiguous()
     if len(lead) != 1:
         x = x.reshape(-1, V)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    out = TokenLogprobs(x.new_empty(lead, dtype=_F32), x.new_empty(lead, dtype=_F32),
+    logprobs = x.new_empty(lead, dtype=_F32)
+    out = TokenLogprobs(logprobs, torch.empty_like(logprobs),
                         x.new_empty((*lead, top), dtype=_I32),
-                        x.new_empty((*lead, top), dtype=_F32))
-    hip.token_logprobs(x, tokens, top, *out)
+                        logprobs.new_empty((*lead, top)))
+    hip.token_logprobs(x, tokens, wide, top, *out)
     return out
 
 
