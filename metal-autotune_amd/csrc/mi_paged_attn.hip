@@ -26,10 +26,23 @@ namespace {
 
 constexpr int PA_WAVES = ATT_STREAMS;
 
+// The work of one workgroup beside its kv head.
+struct PagedItem {
+    int r;           // request, < 0: none
+    int wide;
+    int q0, n, len;  // its first token, its tokens, its keys
+    int cb;          // column block
+    int split, ns;   // chunk of the block's keys, chunks (a request's earlier wide
+                     // blocks have fewer than its last: split >= ns is no work)
+    int runs;        // CHUNK_KEYS runs a chunk
+    int first;       // the block's first state in the workspace (of 32 columns each)
+};
+
 struct PagedArgs {
     const void *q, *k, *v;
     void *out;
     const int *table, *cu_q, *kv_lens;
+    PagedItem *items;   // made by paged_items_kernel; null: each workgroup finds its own
     unsigned *tickets;  // by a block's first state and kv head
     float *part;  // partial states, by state and kv head; null: no block is cut
     int T, R, W, H, HK, G, pages, page_log2;
@@ -85,18 +98,6 @@ __device__ __forceinline__ int mean_runs(const PagedArgs &a, const Req &q) {
     return q.wide ? (q.runs + (max(first, 0) + CHUNK_KEYS - 1) / CHUNK_KEYS + 1) / 2 : q.runs;
 }
 
-// The work of one workgroup beside its kv head.
-struct PagedItem {
-    int r;           // request, < 0: none
-    bool wide;
-    int q0, n, len;  // its first token, its tokens, its keys
-    int cb;          // column block
-    int split, ns;   // chunk of the block's keys, chunks (a request's earlier wide
-                     // blocks have fewer than its last: split >= ns is no work)
-    int runs;        // CHUNK_KEYS runs a chunk
-    int first;       // the block's first state in the workspace (of 32 columns each)
-};
-
 // The wide blocks of a lane's request that see at least L runs of keys, its last
 // ones: block cb's last token is min((128 cb + 127) / G, n - 1), which sees len - n
 // keys and those up to its own.
@@ -106,27 +107,28 @@ __device__ __forceinline__ int blocks_from(const PagedArgs &a, const Req &q, int
     return y <= 0 || L == 0 ? q.wide : q.wide - min(y * a.G / WIDE_COLS, q.wide - 1);
 }
 
-// Item u: the wide blocks' chunks first, then the narrow ones', in the order of
-// requests, of their blocks, of their chunks; but the wide ones of at most 64
-// requests from those that see the most keys to those that see the fewest, since
-// a long one that starts last would run on alone (four prompts of 2048 tokens: 203
-// -> 165 us). Every wave finds its item by itself, 64 requests a step: first the
+// Item u: the wide blocks' chunks, then the narrow ones' whole chunks, then what is
+// left of them, each in the order of requests, of their blocks, of their chunks;
+// but the wide ones of at most 64 requests from those that see the most keys to
+// those that see the fewest: what starts last should be short. Every wave finds its item by itself, 64 requests a step: first the
 // runs of all blocks, which give the size of a chunk, then the chunks up to its own.
 template <bool WIDE>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
     Req q = load_req<WIDE>(a, lane);
-    int runs = 1 << 30;
+    int runs = 1 << 30, longest = 0;
     if (a.part) {
         // (blocks < 2^16 and runs < 2^23: summed in two halves)
         uint64_t total = 0;
         for (int r0 = 0;;) {
+            const Req next = a.R > r0 + 64 ? load_req<WIDE>(a, r0 + 64 + lane) : q;
+            longest = max(longest, q.runs);
             const uint64_t mine = (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)mean_runs(a, q);
             const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
             total += (uint64_t)(unsigned)__builtin_amdgcn_readlane(lo, 63) +
                      ((uint64_t)(unsigned)__builtin_amdgcn_readlane(hi, 63) << 24);
             r0 += 64;
             if (r0 >= a.R) break;
-            q = load_req<WIDE>(a, r0 + lane);
+            q = next;
         }
         total += a.target - 1;
         runs = total >> 32 ? (int)(total / (unsigned)a.target)
@@ -135,9 +137,9 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     }
     PagedItem it;
     it.r = -1;
-    int before = 0, states = 0;  // items, and states of 32 columns
+    int before = 0, states = 0, narrow_states = 0;  // items, and states of 32 columns
 #pragma unroll
-    for (int kind = WIDE ? 0 : 1; kind < 2; ++kind) {
+    for (int kind = WIDE ? 0 : 1; kind < 3; ++kind) {
         const bool wide = kind == 0;
         const int scale = wide ? WIDE_COLS / 32 : 1;
         if (wide && a.R <= 64) {
@@ -173,13 +175,20 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             it.first = scale * (__builtin_amdgcn_readlane(end - q.wide * ns, l) + it.cb * it.ns);
             return it;
         }
+        if (kind == 1) {
+            narrow_states = states;
+            if (!__builtin_amdgcn_ballot_w64(longest >= runs)) continue;  // none is cut
+        }
+        if (kind == 2) states = narrow_states;
+        if (a.R > 64) q = load_req<WIDE>(a, lane);
         for (int r0 = 0;;) {
-            if (a.R > 64) q = load_req<WIDE>(a, r0 + lane);
+            const Req next = a.R > r0 + 64 ? load_req<WIDE>(a, r0 + 64 + lane) : q;
             const int per = max(max(runs, wide ? a.wide_runs : 1),
                                 (q.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
-            const int ns = max(1, (q.runs + per - 1) / per);
-            const int blocks = wide ? q.wide : q.narrow, items = blocks * ns;
-            const int end = before + wave_scan(items);
+            const int ns = max(1, (q.runs + per - 1) / per), whole = q.runs / per;
+            const int blocks = wide ? q.wide : q.narrow;
+            const int some = wide ? ns : kind == 1 ? whole : ns - whole, items = blocks * some;
+            const int end = before + wave_scan(items), state_end = states + wave_scan(scale * blocks * ns);
             const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
             if (past) {
                 const int l = __builtin_ctzll(past);
@@ -190,18 +199,18 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
                 it.len = __builtin_amdgcn_readlane(q.len, l);
                 it.ns = __builtin_amdgcn_readlane(ns, l);
                 it.runs = __builtin_amdgcn_readlane(per, l);
-                const int before_r = __builtin_amdgcn_readlane(end - items, l);
-                const int b = (u - before_r) / it.ns;
-                it.split = u - before_r - b * it.ns;
+                const int at = u - __builtin_amdgcn_readlane(end - items, l);
+                const int each = __builtin_amdgcn_readlane(some, l), b = at / each;
+                it.split = at - b * each + (kind == 2 ? __builtin_amdgcn_readlane(whole, l) : 0);
                 it.cb = wide ? __builtin_amdgcn_readlane(blocks, l) - 1 - b : b;
-                it.first = states + scale * (before_r - before + b * it.ns);
+                it.first = __builtin_amdgcn_readlane(state_end - scale * blocks * ns, l) + scale * b * it.ns;
                 return it;
             }
-            const int all = __builtin_amdgcn_readlane(end, 63);
-            states += scale * (all - before);
-            before = all;
+            before = __builtin_amdgcn_readlane(end, 63);
+            states = __builtin_amdgcn_readlane(state_end, 63);
             r0 += 64;
             if (r0 >= a.R) break;
+            q = next;
         }
     }
     return it;
@@ -629,6 +638,14 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
 // would spill).
 template <int D, bool WIDE> constexpr int paged_per_cu() { return D == 128 ? 2 : (WIDE ? 3 : 4); }
 
+// A wave an item: found once for all kv heads.
+template <bool WIDE> __global__ __launch_bounds__(256) void paged_items_kernel(PagedArgs a, int items) {
+    const int u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (u >= items) return;
+    const PagedItem it = find_item<WIDE>(a, u, threadIdx.x & 63);
+    if ((threadIdx.x & 63) == 0) a.items[u] = it;
+}
+
 // One workgroup an item and kv head. WIDE: requests of more than 32 columns are in
 // wide blocks; without it (decode) every block is narrow.
 template <typename T, int D, bool WIDE>
@@ -636,7 +653,18 @@ __global__ __launch_bounds__(64 * PA_WAVES) __attribute__((amdgpu_waves_per_eu(p
 void paged_attn_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
-    PagedItem it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
+    PagedItem it;
+    if (a.items) {
+        const int *p = (const int *)(a.items + blockIdx.y);
+        int f[sizeof(PagedItem) / 4];
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(PagedItem) / 4); ++i) f[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(PagedItem) / 4); ++i) f[i] = __builtin_amdgcn_readfirstlane(f[i]);
+        it = __builtin_bit_cast(PagedItem, f);
+    } else {
+        it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
+    }
     if (it.r < 0) return;  // (workgroup-uniform)
     if (WIDE && it.wide) {
         if (it.ns > 1) {
@@ -662,14 +690,14 @@ void paged_attn_kernel(PagedArgs a) {
 // or n G / 32 of a request, rounded up). A chunk is one run or more, so there are
 // at most `target` chunks and the last, shorter one of every block, and no more
 // than a row of the table has. Few blocks: as many chunks as one round of
-// workgroups takes with those last ones; many: four rounds' worth, so that what
-// the last round leaves idle is small. Wide blocks, whose parts cost 66 KB written
+// workgroups takes with those last ones; many: one and a half rounds' worth, the
+// shorter ones last (64 requests of 4096 keys: 171 us, with four rounds' 183). Wide blocks, whose parts cost 66 KB written
 // and read, are then cut only where they fill less than two rounds, past 32 runs
 // (20 requests, four of 256 to 512 tokens and up to 4096 keys: 90 us; from 8 runs
 // on, 103; 8192 tokens of one prompt uncut 562 us, cut past 32 runs 694).
 struct PagedGrid {
     int64_t wide, narrow, items, states, target, wide_runs;
-    bool cut, cut_wide;
+    bool cut, cut_wide, listed;
 };
 inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t HK, int64_t D,
                             int64_t page, int64_t max_q) {
@@ -688,7 +716,7 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
                                                    : paged_per_cu<64, false>());
     const int64_t runs = ceil_div(W * page, CHUNK_KEYS);
     const int64_t few = slots - (g.wide + g.narrow) * HK;
-    g.target = (few >= slots / 2 ? few : 4 * slots) / HK;
+    g.target = (few >= slots / 2 ? few : 3 * slots / 2) / HK;
     if (g.target < 1) g.target = 1;
     g.wide_runs = few >= slots / 2 ? 1 : g.wide * HK < 2 * slots ? 32 : 1 << 23;
     g.cut = runs > 1;
@@ -705,21 +733,34 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
         narrow = g.narrow + g.target < most ? g.narrow + g.target : most;
     }
     g.items = wide + narrow;
+    // Past 192 requests a workgroup would sum over them for longer than a launch
+    // takes that lists the items once (1000 requests of 300 keys: 222 us, without
+    // 423; 300 of 600: 128, 140; 129 of 1000: 96, 90).
+    g.listed = R > 192;
     g.states = wide * (WIDE_COLS / 32) + narrow;
     return g;
 }
 // The tickets take a fixed prefix of the workspace, so that calls of any sizes can
 // share one whose prefix is zero.
 constexpr int64_t PAGED_TICKETS = MI_PAGED_ZERO_BYTES / 4;
+inline int64_t paged_list_bytes(const PagedGrid &g) {
+    return g.listed ? ceil_div(g.items * (int64_t)sizeof(PagedItem), 256) * 256 : 0;
+}
+inline bool paged_cuts(const PagedGrid &g, int64_t HK) {
+    return g.cut && g.states * HK <= PAGED_TICKETS;
+}
 inline int64_t paged_bytes(const PagedGrid &g, int64_t HK, int64_t D) {
-    return g.cut && g.states * HK <= PAGED_TICKETS
-               ? MI_PAGED_ZERO_BYTES + g.states * HK * (32 * D + 128) * (int64_t)sizeof(float) : 0;
+    const int64_t states =
+        paged_cuts(g, HK) ? g.states * HK * (32 * D + 128) * (int64_t)sizeof(float) : 0;
+    return states || g.listed ? MI_PAGED_ZERO_BYTES + paged_list_bytes(g) + states : 0;
 }
 
 template <typename T, int D, bool WIDE>
 int launch_paged_w(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
-    const int64_t blocks = g.wide + g.narrow;
-    paged_attn_kernel<T, D, WIDE><<<dim3((unsigned)a.HK, (unsigned)(a.part ? g.items : blocks)),
+    const int64_t items = a.part ? g.items : g.wide + g.narrow;
+    if (a.items)
+        paged_items_kernel<WIDE><<<(unsigned)ceil_div(items, 4), 256, 0, st>>>(a, (int)items);
+    paged_attn_kernel<T, D, WIDE><<<dim3((unsigned)a.HK, (unsigned)items),
                                     64 * PA_WAVES, 0, st>>>(a);
     return launch_status("paged attention");
 }
@@ -786,8 +827,10 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
     const float sl = scale * 1.4426950408889634f;
     // (a scale of 0 as the smallest normal: masked scores stay -inf; NaN stays NaN)
     const float mag = fabsf(sl) < 1.17549435e-38f ? 1.17549435e-38f : fabsf(sl);
-    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens, (unsigned *)ws,
-                         ws ? (float *)(ws + MI_PAGED_ZERO_BYTES) : nullptr, (int)T, (int)R,
+    char *lists = ws ? ws + MI_PAGED_ZERO_BYTES : nullptr;
+    const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens,
+                         ws && g.listed ? (PagedItem *)lists : nullptr, (unsigned *)ws,
+                         ws && paged_cuts(g, HK) ? (float *)(lists + paged_list_bytes(g)) : nullptr, (int)T, (int)R,
                          (int)table_width, (int)H, (int)HK, (int)(H / HK), (int)n_pages, lp,
                          (int)g.target, (int)g.wide_runs, mag, sl < 0.0f ? 0x80008000u : 0u};
     hipStream_t st = as_stream(stream);

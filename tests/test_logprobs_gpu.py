@@ -143,6 +143,39 @@ def test_no_answer_is_nan():
     assert torch.equal(r.logprobs[0], want.logprobs[0])
 
 
+def test_without_a_workspace(monkeypatch):
+    """The C entry without scratch: a workgroup a row, the same answers."""
+    from autotuner_runtime import hip
+
+    x, tok = logits(8, 3, 40001, BF)
+    want = check(x, tok, 7)
+    need = hip._logprobs_workspace_bytes
+    for short in (lambda *a: 0, lambda *a: need(*a) - 1):
+        monkeypatch.setattr(hip, "_logprobs_workspace_bytes", short)
+        got = check(x, tok, 7)
+        assert torch.equal(got.top_ids, want.top_ids)
+
+
+def test_repeats_and_graphs():
+    """The same bits from call to call, and from a graph replayed over new logits."""
+    from autotuner_runtime import hip
+
+    x, tok = logits(9, 3, 65537, BF)
+    y, _ = logits(10, 3, 65537, BF)
+    want = [ops.token_logprobs(v, tok, 5) for v in (x, y)]
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with hip.graph_workspaces(), torch.cuda.graph(graph):
+        out = ops.token_logprobs(static, tok, 5)
+    for i in (0, 1, 1, 0, 1):
+        static.copy_((x, y)[i])
+        ops.token_logprobs(y, tok, 5)  # eager work between
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i])), i
+
+
 def test_refusals():
     x, tok = logits(7, 3, 100, BF)
     for top in (-1, 65, 101):

@@ -312,6 +312,95 @@ def test_attention_of_many_requests():
     run_attention(kv.tolist(), n_q.tolist(), 4, 2, 64, 16, BF)
 
 
+@pytest.mark.parametrize("R", [65, 193, 260])
+def test_attention_of_many_requests_of_all_lengths(R):
+    """Rows that are cut among rows that are not, prompts among single tokens, by
+    64 requests a step and from a list of the work."""
+    rng = np.random.default_rng(R)
+    kv = rng.integers(1, 90, R)
+    n_q = np.minimum(rng.integers(0, 3, R), kv)
+    kv[[3, R // 2, R - 1]] = [2500, 700, 1301]
+    n_q[[3, R // 2, R - 1]] = [1, 200, 33]
+    kv[20], n_q[20] = 120, 120
+    run_attention(kv.tolist(), n_q.tolist(), 8, 2, 64, 32, BF)
+    run_attention(kv.tolist(), n_q.tolist(), 8, 2, 128, 16, FP, max_q_len=200)
+
+
+def test_attention_without_a_workspace(monkeypatch):
+    """The C entry without scratch: a workgroup a block, the same rows within
+    rounding; scratch one byte short takes that path too."""
+    kv, n_q = [3000, 10, 700], [1, 1, 90]
+    want = run_attention(kv, n_q, 8, 2, 128, 64, BF)
+    need = hip._paged_workspace_bytes
+    for short in (lambda *a: 0, lambda *a: need(*a) - 1):
+        monkeypatch.setattr(hip, "_paged_workspace_bytes", short)
+        got = run_attention(kv, n_q, 8, 2, 128, 64, BF)
+        assert float((got.float() - want.float()).abs().max()) < 0.05
+    many = [50] * 300
+    run_attention(many, [1] * 300, 4, 2, 64, 16, BF)
+
+
+def test_attention_kernel_hint_changes_no_meaning():
+    """max_q_len chooses kernels: too small, too large and absent give the rows."""
+    for hint in (1, 7, 500, None):
+        run_attention([400, 33, 260], [130, 1, 40], 8, 2, 64, 32, BF, max_q_len=hint)
+
+
+def test_attention_on_streams_and_threads():
+    """Two streams and two threads at once, each with scratch of its own."""
+    import threading
+
+    g = gen_of(31)
+    kv, n_q = [2900, 500], [1, 1]
+    kp, vp, table, ks, vs = make_cache(g, kv, 64, 4, 128, BF)
+    qs = [rnd(g, 2, 16, 128) for _ in range(4)]
+    cu, lens = i32([0, 1, 2]), i32(kv)
+    want = [ops.paged_attention(q, kp, vp, table, cu, lens, 0.1, 1) for q in qs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = ops.paged_attention(qs[i], kp, vp, table, cu, lens, 0.1, 1)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_attention_in_graphs_at_other_lengths():
+    """Two graphs of one shape, captured in scopes of their own and replayed in
+    turn and at once, at lengths that change between replays."""
+    g = gen_of(32)
+    kv = [3000, 700]
+    kp, vp, table, ks, vs = make_cache(g, kv, 64, 2, 64, BF)
+    q = rnd(g, 2, 8, 64)
+    cu, lens = i32([0, 1, 2]), i32(kv)
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    ops.paged_attention(q, kp, vp, table, cu, lens, 0.125, 1)
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with hip.graph_workspaces(), torch.cuda.graph(graph):
+            outs.append(ops.paged_attention(q, kp, vp, table, cu, lens, 0.125, 1))
+        graphs.append(graph)
+    for now in ([3000, 700], [100, 1], [2049, 640], [3000, 700]):
+        lens.copy_(i32(now))
+        want = ops.paged_attention(q, kp, vp, table, cu, lens, 0.125, 1)
+        check_attention(want, *attention_64(q, [k[:n] for k, n in zip(ks, now)],
+                                            [v[:n] for v, n in zip(vs, now)], [1, 1], 0.125), BF)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
 def test_attention_leaves_rows_behind_the_last_request():
     """Rows of the token buffer that no request has are not written, and a cu_q
     that passes the buffer is held to it."""
