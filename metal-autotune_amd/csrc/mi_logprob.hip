@@ -17,7 +17,7 @@
 // them, reads the k best chunks again and keeps what reaches the k-th maximum
 // (as good as k values in all, but for ties) in a list, a lane an entry.
 //
-// Bound by HBM at many rows (the row's one read, 11 VALU instructions a value of
+// Bound by HBM at many rows (the row's one read, 9.5 VALU instructions a value of
 // the 13 that fit beside it); by the launch and its trips to memory, one after
 // another, at few, where a row is split over workgroups.
 #include <math.h>
@@ -32,7 +32,7 @@ constexpr int LP_WAVES = 4, LP_SPLIT_WAVES = 8;  // of a workgroup that has a ro
 constexpr int LP_CHUNK = 1024;   // values a chunk, 2 (16 bits) or 4 (fp32) 16-byte pieces a lane
 constexpr int64_t LP_MAX_V = (int64_t)1 << 20;
 constexpr int LP_MAX_CHUNKS = (int)(LP_MAX_V / LP_CHUNK) + 1;  // (the first may begin before the row)
-constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 
 // A 16-byte piece of a row as floats.
 template <typename T> struct Piece {
@@ -70,27 +70,39 @@ __device__ __forceinline__ float wave_add(float v) {
     return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
 }
 
+// What a wave sums is in units of log2: t = x log2 e - C with C = rint(ref log2 e) an
+// integer, p = 2^t, S = sum p, E = sum p t: one fma a value, rounded as finely as t
+// is small, and a step from one C to another scales by a power of two. References
+// beyond 1e30 (a mask's lowest value, where x log2 e overflows; -FLT_MAX before the
+// first value) take t = (x - ref) log2 e instead.
 struct Sums {
     float ref;   // shared by the wave
     float top;   // the lane's largest value
     float s, e;  // the lane's sums against ref
 };
-
-// d and e^d of one value against a reference, added. (e^d = 0 for d below -104:
-// the floor keeps a forbidden token's -inf out of 0 * d; NaN reaches s.)
-__device__ __forceinline__ void add_value(Sums &a, float x) {
-    const float d = x - a.ref;
-    const float p = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+__device__ __forceinline__ bool far(float ref) { return !(fabsf(ref) <= 1e30f); }
+__device__ __forceinline__ float units(float ref) { return __builtin_rintf(ref * LP_LOG2E); }
+// (2^t = 0 for t below -150: the floor keeps a forbidden token's -inf out of 0 * t;
+// NaN reaches s.)
+__device__ __forceinline__ void add_value(Sums &a, float t) {
+    const float p = __builtin_amdgcn_exp2f(t);
     a.s += p;
-    a.e = __builtin_fmaf(p, fmaxf(d, -200.0f), a.e);
+    a.e = __builtin_fmaf(p, fmaxf(t, -300.0f), a.e);
 }
-__device__ __forceinline__ void move_ref(float &s, float &e, float from, float to) {
-    const float c = from - to;
-    const float f = __builtin_amdgcn_exp2f(c * LP_LOG2E);
-    // (a reference at a mask's lowest value, or -FLT_MAX before the first: c s may
-    // overflow, and what it is weighted with has vanished)
+// Sums against a reference c units higher.
+__device__ __forceinline__ void move_sums(float &s, float &e, float c) {
+    const float f = __builtin_amdgcn_exp2f(c);
+    // (c s may overflow where what it is weighted with has vanished)
     e = f == 0.0f ? 0.0f : __builtin_fmaf(c, s, e) * f;
     s *= f;
+}
+__device__ __forceinline__ void move_ref(float &s, float &e, float from, float to) {
+    move_sums(s, e, far(from) || far(to) ? (from - to) * LP_LOG2E : units(from) - units(to));
+}
+// ... against the row's maximum itself.
+__device__ __forceinline__ void move_to(float &s, float &e, float from, float m) {
+    move_sums(s, e, far(from) || far(m) ? (from - m) * LP_LOG2E
+                                        : __builtin_fmaf(-m, LP_LOG2E, units(from)));
 }
 
 // The order of floats as the order of ints (-0 as 0); what is no value is NONE.
@@ -142,7 +154,7 @@ template <typename T> struct Row {
     }
     // whether every value of the chunk's pieces is the row's
     __device__ __forceinline__ bool whole(int chunk) const {
-        return chunk > 0 && (chunk + 1) * LP_CHUNK - skew <= V;
+        return (chunk > 0 || skew == 0) && (chunk + 1) * LP_CHUNK - skew <= V;
     }
     // a whole chunk; NT: a row read once, past the caches
     template <bool NT>
@@ -157,60 +169,94 @@ template <typename T> struct Row {
 #pragma unroll
         for (int i = 0; i < PER; ++i) pc[i] = open_piece<T>(raw[i]);
     }
-    // the row's ends
+    // the row's ends: the pieces within it as 16 bytes, the one across an end value by
+    // value (all of these loads in flight together)
     __device__ __forceinline__ void get_end(int chunk, int lane, Piece<T> (&pc)[PER]) const {
+        uint4 raw[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int f = first(chunk, i, lane);
+            if (f >= 0 && f + N <= V) raw[i] = ld16(base + (int64_t)(f + skew) * (int)sizeof(T));
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int f = first(chunk, i, lane);
             if (f >= 0 && f + N <= V) {
-                pc[i] = open_piece<T>(ld16(base + (int64_t)(f + skew) * (int)sizeof(T)));
-            } else {
+                pc[i] = open_piece<T>(raw[i]);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) pc[i].f[e] = -INFINITY;
+            if (f + N > 0 && f < V) {
+                T v[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = x[min(max(f + e, 0), V - 1)];
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    pc[i].f[e] = f + e >= 0 && f + e < V ? (float)x[f + e] : -INFINITY;
+                    if (f + e >= 0 && f + e < V) pc[i].f[e] = (float)v[e];
             }
         }
     }
 };
 
-// The chunks c0, c0 + step, ... below c1 of a row, by one wave: its sums, and (TOP)
-// the key of each chunk's maximum at maxima[c].
-template <typename T, bool TOP, bool NT>
-__device__ __forceinline__ float4 pass(const Row<T> &row, int c0, int c1, int step, int *maxima,
-                                       int lane) {
+// One chunk added to a wave's sums; (TOP) the key of its maximum at maxima[c].
+template <typename T, bool TOP>
+__device__ __forceinline__ void add_chunk(Sums &a, const Piece<T> (&pc)[Row<T>::PER], int c,
+                                          int *maxima, int lane) {
     constexpr int N = Row<T>::N, PER = Row<T>::PER;
+    float pm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) pm = fmaxf(fmaxf(pm, pc[i].f[e]), pc[i].f[e + 1]);
+    a.top = fmaxf(a.top, pm);
+    if (TOP) {
+        const float cm = wave_max(pm);
+        if (lane == 0) maxima[c] = key_of(cm);
+    }
+    if (__builtin_amdgcn_ballot_w64(pm > a.ref + 30.0f)) {
+        const float to = fmaxf(a.ref, wave_max(pm));
+        move_ref(a.s, a.e, a.ref, to);
+        a.ref = to;
+    }
+    if (far(a.ref)) {  // (uniform)
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) add_value(a, (pc[i].f[e] - a.ref) * LP_LOG2E);
+    } else {
+        const float c2 = units(a.ref);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) add_value(a, __builtin_fmaf(pc[i].f[e], LP_LOG2E, -c2));
+    }
+}
+
+// The chunks c0, c0 + STEP, ... below c1 of a row, by one wave. The row's ends come
+// after the whole chunks, in a loop of their own: among them, the waits for their
+// loads would stop the next chunk's, which are on their way while one is added.
+template <typename T, bool TOP, bool NT, int STEP>
+__device__ __forceinline__ float4 pass(const Row<T> &row, int c0, int c1, int *maxima, int lane) {
+    constexpr int PER = Row<T>::PER;
     Sums a = {-3.4028235e38f, -INFINITY, 0.0f, 0.0f};
-    uint4 raw[PER];  // the next chunk, on its way while this one is added
-    if (c0 < c1 && row.whole(c0)) row.template load<NT>(c0, lane, raw);
-    for (int c = c0; c < c1; c += step) {
+    const int w0 = c0 + (row.skew && c0 == 0 ? STEP : 0), w1 = min(c1, (row.V + row.skew) / LP_CHUNK);
+    uint4 raw[PER];
+    if (w0 < w1) row.template load<NT>(w0, lane, raw);
+    for (int c = w0; c < w1; c += STEP) {
         Piece<T> pc[PER];
-        if (row.whole(c)) {  // (uniform)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) launder(raw[i]);
-            row.open(raw, pc);
-        } else {
-            row.get_end(c, lane, pc);
-        }
-        if (c + step < c1 && row.whole(c + step)) row.template load<NT>(c + step, lane, raw);
-        float pm = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int e = 0; e < N; e += 2) pm = fmaxf(fmaxf(pm, pc[i].f[e]), pc[i].f[e + 1]);
-        a.top = fmaxf(a.top, pm);
-        if (TOP) {
-            const float cm = wave_max(pm);
-            if (lane == 0) maxima[c] = key_of(cm);
-        }
-        if (__builtin_amdgcn_ballot_w64(pm > a.ref + 30.0f)) {
-            const float to = fmaxf(a.ref, wave_max(pm));
-            move_ref(a.s, a.e, a.ref, to);
-            a.ref = to;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int e = 0; e < N; ++e) add_value(a, pc[i].f[e]);
+        for (int i = 0; i < PER; ++i) launder(raw[i]);
+        row.open(raw, pc);
+        if (c + STEP < w1) row.template load<NT>(c + STEP, lane, raw);
+        add_chunk<T, TOP>(a, pc, c, maxima, lane);
+    }
+    for (int j = 0; j < 2; ++j) {
+        const int c = j ? row.chunks() - 1 : 0;
+        if (c < c0 || c >= c1 || (c - c0) % STEP || row.whole(c) || (j && c == 0)) continue;
+        Piece<T> pc[PER];
+        row.get_end(c, lane, pc);
+        add_chunk<T, TOP>(a, pc, c, maxima, lane);
     }
     return make_float4(a.ref, wave_max(a.top), wave_add(a.s), wave_add(a.e));
 }
@@ -287,7 +333,7 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit
     for (int i = lane; i < n; i += 64) {
         const float4 p = i == lane ? p0 : get_sums(part + i);
         float s = p.z, e = p.w;
-        move_ref(s, e, p.x, m);
+        move_to(s, e, p.x, m);
         S += s;
         E += e;
     }
@@ -296,7 +342,7 @@ __device__ __forceinline__ void finish(const Row<T> &row, int64_t r, float logit
     const float ls = logf(S);
     if (threadIdx.x == 0) {
         a.logprob[r] = (logit - m) - ls;
-        a.entropy[r] = ls - E / S;
+        a.entropy[r] = ls - LP_LN2 * (E / S);
     }
     if constexpr (TOP) {
         const int k = a.k, nc = row.chunks(), need = k < nc ? k : nc;
@@ -390,14 +436,14 @@ __global__ __launch_bounds__(64 * (SPLIT ? LP_SPLIT_WAVES : LP_WAVES)) void logp
         for (int c = threadIdx.x; c < nc; c += 64 * WAVES) top->rank[c] = 0;
     }
     if constexpr (!SPLIT) {
-        const float4 p = pass<T, TOP, true>(row, wave, nc, WAVES, maxima, lane);
+        const float4 p = pass<T, TOP, true, WAVES>(row, wave, nc, maxima, lane);
         if (lane == 0) part[wave] = p;
         __syncthreads();
         finish<T, TOP, WAVES>(row, r, logit, part[lane % WAVES], part, WAVES, maxima, top, a);
         return;
     }
     const int c0 = blockIdx.x * a.per, c1 = min(c0 + a.per, nc), segments = gridDim.x;
-    const float4 p = pass<T, TOP, false>(row, c0 + wave, c1, WAVES, maxima, lane);
+    const float4 p = pass<T, TOP, false, WAVES>(row, c0 + wave, c1, maxima, lane);
     if (lane == 0) part[wave] = p;
     __syncthreads();
     int *all = a.maxima + r * a.nc;
