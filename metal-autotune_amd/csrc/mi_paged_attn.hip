@@ -103,7 +103,7 @@ __device__ __forceinline__ int mean_runs(const PagedArgs &a, const Req &q) {
 // keys and those up to its own.
 __device__ __forceinline__ int blocks_from(const PagedArgs &a, const Req &q, int L) {
     const int y = (L - 1) * CHUNK_KEYS - (q.len - q.n);  // the first token that does
-    if (y >= q.n && L > 0) return 0;
+    if (q.wide == 0 || (y >= q.n && L > 0)) return 0;
     return y <= 0 || L == 0 ? q.wide : q.wide - min(y * a.G / WIDE_COLS, q.wide - 1);
 }
 

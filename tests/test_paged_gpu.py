@@ -294,6 +294,8 @@ def run_attention(kv, n_q, H, HK, D, page, dtype, scale=None, max_q_len=None, se
     ([600], [600], 4, 1, 64, 16, FP),
     ([900, 700], [300, 700], 32, 8, 128, 64, BF),
     ([3, 2], [3, 2], 40, 1, 64, 16, BF),                             # 40 q heads on one kv head
+    ([3, 40, 0], [5, 60, 70], 4, 2, 64, 16, BF),                     # more tokens than keys
+    ([130, 300, 258], [4, 200, 3], 8, 2, 128, 64, BF),               # few tokens on both sides of a run's end
 ])
 def test_attention(kv, n_q, H, HK, D, page, dtype):
     run_attention(kv, n_q, H, HK, D, page, dtype)
