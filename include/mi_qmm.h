@@ -326,13 +326,13 @@ int mi_argmax_noalloc(const void *x, int32_t *out, int64_t rows, int64_t V, int 
  * free_pages[0, *free_count) (capacity n_free), request after request, and
  * entered into the block table. Written: cu_q; kv_after[r] = kv_lens[r] +
  * q_lens[r]; of token t the position in its request and its slot (0 and -1 past
- * the last token: T may exceed their number, and must not be less);
- * *free_left, the free pages that remain; *refused, the number of refused
- * requests. A request that needs pages and whose pages, behind those of the
- * requests before it, exceed *free_count, or whose keys would pass its row of
- * the table, is refused: it takes none, kv_after[r] = 0 and its slots are -1.
+ * the last token: T may exceed their number); *free_left, the free pages that
+ * remain; *refused, the number of refused requests. A request that needs pages
+ * and whose pages, behind those of the requests before it, exceed *free_count,
+ * whose keys would pass its row of the table, or whose tokens pass the T rows, is
+ * refused: it takes none, kv_after[r] = 0 and its slots are -1.
  * The inputs stay as they are (the table's entries of cached keys too). 1 <= R
- * <= 4096, table_width <= 131072. */
+ * <= 4096, T <= 262144, table_width <= 131072. */
 int mi_paged_plan(int32_t *block_table, int64_t table_width, const int32_t *kv_lens,
                   const int32_t *q_lens, const int32_t *free_pages, int64_t n_free,
                   const int32_t *free_count, int64_t R, int64_t T, int64_t page_size,
@@ -362,7 +362,9 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
  * its keys kv_lens[r] (these tokens' own among them); its token i sees keys
  * j <= kv_lens[r] - n + i with n its tokens (a token that sees none gives 0). Rows of
  * out behind the last request's are left as they were. Page ids outside the pool
- * are held to it. max_q_len: the most tokens a request brings, 0 if unknown; it
+ * are held to it. A value that is not finite reaches, beside the rows that see it,
+ * the request's rows whose last key lies less than 96 keys before it (they weigh it
+ * with 0); keys behind a request's last, or in other pages, reach nothing. max_q_len: the most tokens a request brings, 0 if unknown; it
  * chooses the kernels (no request of more than 32 rows of a kv head, or some),
  * and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a workspace of
  * mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte

@@ -10,6 +10,7 @@ tensors (hip.lib() raises otherwise); there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import NamedTuple
@@ -324,6 +325,14 @@ def _i32(what: str, dev: int, *arrays) -> None:
                              f"arrays on one device, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: int):
+    """The tensors' device as the current one, for the launch."""
+    return _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
 class PagedPlan(NamedTuple):
     """One step's bookkeeping, on the GPU (``paged_plan``)."""
 
@@ -336,38 +345,50 @@ class PagedPlan(NamedTuple):
 
 
 def paged_plan(block_table, kv_lens, q_lens, free_pages, free_count, page_size: int,
-               num_tokens: int) -> PagedPlan:
+               num_tokens: int, out: PagedPlan | None = None) -> PagedPlan:
     """A step's bookkeeping in one launch: request r holds kv_lens[r] keys and
     brings q_lens[r] tokens (int32 [R]); the pages it lacks are taken from the end
     of free_pages[:free_count] (int32 [F], int32 [1]), request after request, and
     written into block_table (int32 [R, width]) in place. num_tokens: rows of the
-    step's token buffer, at least the sum of q_lens (rows behind it get position 0
-    and slot -1). A request whose pages are not there, or whose keys would pass
-    its row of the table, takes none and is counted in ``refused``."""
-    if not block_table.is_cuda:
-        hip._require_gpu(block_table)
+    step's token buffer (rows behind the sum of q_lens get position 0 and slot -1).
+    A request whose pages are not there, whose keys would pass its row of the table
+    or whose tokens those rows, takes none and is counted in ``refused``. out: an earlier
+    plan of as many requests and tokens, written again (a captured graph reads it
+    where it is); its kv_lens and free_count may not be this call's inputs."""
     shape = kv_lens.shape
     if block_table.dim() != 2 or len(shape) != 1 or q_lens.shape != shape \
             or shape[0] != block_table.shape[0] or free_pages.dim() != 1 \
             or free_count.numel() != 1:
         raise ValueError("paged_plan takes block_table [R, width], kv_lens [R], q_lens [R], "
                          "free_pages [F] and free_count [1]")
-    _i32("paged_plan", block_table.get_device(), block_table, kv_lens, q_lens, free_pages,
-         free_count)
+    dev = block_table.get_device()
+    _i32("paged_plan", dev, block_table, kv_lens, q_lens, free_pages, free_count)
     R, width = block_table.shape
     T = int(num_tokens)
     if T < 0:
         raise ValueError(f"paged_plan: num_tokens={T}")
-    # one allocation for the six outputs, which lie one after another
-    buf = block_table.new_empty(2 * (R + T) + 3)
-    at = buf.data_ptr()
-    hip._check(hip.lib().mi_paged_plan(
-        block_table.data_ptr(), width, kv_lens.data_ptr(), q_lens.data_ptr(),
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), R, T, int(page_size),
-        at, at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + T),
-        at + 4 * (2 * (R + T) + 1), at + 4 * (2 * (R + T) + 2), hip._stream(block_table)),
-        "paged_plan")
-    return PagedPlan._make(torch.split_with_sizes(buf, (R + 1, R, T, T, 1, 1)))
+    if not block_table.is_cuda:
+        hip._require_gpu(block_table)
+    if out is None:
+        # one allocation for the six outputs, which lie one after another
+        buf = block_table.new_empty(2 * (R + T) + 3)
+        at = buf.data_ptr()
+        ptrs = (at, at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + T),
+                at + 4 * (2 * (R + T) + 1), at + 4 * (2 * (R + T) + 2))
+        out = PagedPlan._make(torch.split_with_sizes(buf, (R + 1, R, T, T, 1, 1)))
+    else:
+        if [t.numel() for t in out] != [R + 1, R, T, T, 1, 1]:
+            raise ValueError(f"paged_plan: out is not a plan of {R} requests and {T} tokens")
+        _i32("paged_plan", dev, *out)
+        ptrs = [t.data_ptr() for t in out]
+        if ptrs[1] == kv_lens.data_ptr() or ptrs[4] == free_count.data_ptr():
+            raise ValueError("paged_plan: out holds this call's inputs")
+    with _on(dev):
+        hip._check(hip.lib().mi_paged_plan(
+            block_table.data_ptr(), width, kv_lens.data_ptr(), q_lens.data_ptr(),
+            free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), R, T,
+            int(page_size), *ptrs, hip._stream(block_table)), "paged_plan")
+    return out
 
 
 def rope_table(dims: int, base: float = 10000.0, scale: float = 1.0, freqs=None,
@@ -434,12 +455,13 @@ def norm_rope_paged(q, k, v, q_norm, k_norm, n_heads: int, n_kv_heads: int, eps:
         (sq, _), (sk, _), (sv, _) = q.stride(), k.stride(), v.stride()
         pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
     out = q.new_empty((T, n_heads, D))
-    hip._check(hip.lib().mi_norm_rope_paged(
-        pq, pk, pv, sq, sk, sv, None if q_norm is None else q_norm.data_ptr(),
-        None if k_norm is None else k_norm.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(traditional),
-        positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv_heads, D, n_pages, page,
-        eps, hip._dt(q), hip._stream(q)), "norm_rope_paged")
+    with _on(dev):
+        hip._check(hip.lib().mi_norm_rope_paged(
+            pq, pk, pv, sq, sk, sv, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(traditional),
+            positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv_heads, D, n_pages, page,
+            eps, hip._dt(q), hip._stream(q)), "norm_rope_paged")
     return out
 
 
@@ -457,14 +479,16 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, scale: floa
     R, = kv_lens.shape
     if block_table.dim() != 2 or block_table.shape[0] != R or cu_q.shape != (R + 1,):
         raise ValueError("paged_attention takes block_table [R, width], cu_q [R + 1], kv_lens [R]")
-    _i32("paged_attention", q.get_device(), block_table, cu_q, kv_lens)
+    dev = q.get_device()
+    _i32("paged_attention", dev, block_table, cu_q, kv_lens)
     if not q.is_cuda:
         hip._require_gpu(q)
-    if not q.is_contiguous():
-        q = q.contiguous()
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
-    hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, scale,
-                        0 if max_q_len is None else max_q_len)
+    with _on(dev):
+        hip.paged_attention(q, k_pages, v_pages, out, block_table, cu_q, kv_lens, scale,
+                            0 if max_q_len is None else max_q_len)
     return out
 
 
@@ -504,7 +528,8 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     out = TokenLogprobs(logprobs, torch.empty_like(logprobs),
                         x.new_empty((*lead, top), dtype=_I32),
                         logprobs.new_empty((*lead, top)))
-    hip.token_logprobs(x, tokens, wide, top, *out)
+    with _on(x.get_device()):
+        hip.token_logprobs(x, tokens, wide, top, *out)
     return out
 
 

@@ -203,6 +203,22 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
+// The sum of v over the wave's lanes up to and including this one: rows of 16 by
+// shifts, then row ends broadcast to the rows behind them (DPP; lanes that
+// receive nothing add 0).
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v = dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // Partial results that the last workgroup of several to finish reads. They are
 // stored with agent scope (put_part: written through, past the XCD's L2) and
 // acknowledged before the workgroup's ticket is drawn, where a release fence would

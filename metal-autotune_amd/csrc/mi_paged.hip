@@ -18,29 +18,16 @@ namespace {
 // free_pages[free_count - 1 - (end - need + w - old)].
 //
 // Nothing here is large: the call is bounded by one launch and two trips to
-// memory. So one launch does all of it: every workgroup sums the (at most 4096)
-// requests' lengths for itself, which costs less than a second launch would,
-// then serves 1024 tokens, each finding its request by bisection in LDS. The
-// table entry of a new page is written by the token at its first row: such a
-// token exists for every new page, and no other workgroup reads that entry.
-constexpr int PLAN_MAX_R = 4096;
+// memory (32 requests 2.9 us, 256 requests of 8000 tokens 6.7). So one launch does
+// all of it: every workgroup sums the (at most 4096) requests' lengths for itself,
+// which costs less than a second launch would, then serves 1024 tokens, each
+// finding its request by bisection in LDS. The table entry of a new page is written
+// by the token at its first row: such a token exists for every new page (a request
+// whose tokens pass the T rows is refused), and no other workgroup reads that entry.
+// Refused requests leave no gap in the pages: once one lacks pages or rows, so does
+// every later one that needs a page.
+constexpr int PLAN_MAX_R = 4096, PLAN_MAX_T = 1 << 18;  // (lengths held to T + 1: sums below 2^31)
 constexpr int PLAN_TOKENS = 1024;  // tokens a workgroup
-
-// The sum of v over the wave's lanes up to and including this one: rows of 16 by
-// shifts, then row ends broadcast to the rows behind them (DPP; lanes that
-// receive nothing add 0).
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xF>(v);  // row_shr:1
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-    v = dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
 
 struct PlanArgs {
     int *table;
@@ -87,7 +74,7 @@ __global__ __launch_bounds__(256) void paged_plan_kernel(PlanArgs a, int per) {
         int kv, q, old, need;
         bool fits;
         load(r, kv, q, old, need, fits);
-        const bool ok = fits && (need == 0 || bn + need <= count);
+        const bool ok = fits && (q == 0 || bq + q <= a.T) && (need == 0 || bn + need <= count);
         cu[r] = bq;
         first[r] = ok ? bn : -1;
         if (blockIdx.x == 0) {
@@ -300,10 +287,10 @@ extern "C" int mi_paged_plan(int32_t *block_table, int64_t table_width, const in
         return fail(MI_ERR_UNSUPPORTED, "page size %lld; this build covers 16, 32, 64, 128, 256",
                     (long long)page_size);
     if (R < 1 || R > PLAN_MAX_R || table_width < 1 || table_width > (1 << 17) || T < 0 ||
-        T > (1 << 30) || n_free < 0 || n_free > (1 << 30))
+        T > PLAN_MAX_T || n_free < 0 || n_free > (1 << 30))
         return fail(MI_ERR_ARG, "paged plan: R=%lld (1..%d) table width %lld (1..131072) T=%lld "
-                    "free pages %lld", (long long)R, PLAN_MAX_R, (long long)table_width,
-                    (long long)T, (long long)n_free);
+                    "(0..%d) free pages %lld", (long long)R, PLAN_MAX_R, (long long)table_width,
+                    (long long)T, PLAN_MAX_T, (long long)n_free);
     if (!block_table || !kv_lens || !q_lens || !free_count || !cu_q || !kv_after || !free_left ||
         !refused || (T && (!positions || !slots)) || (n_free && !free_pages))
         return fail(MI_ERR_ARG, "null pointer");
@@ -324,7 +311,8 @@ extern "C" int mi_norm_rope_paged(const void *q, const void *k, const void *v,
                                   int64_t Hq, int64_t Hkv, int64_t D, int64_t n_pages,
                                   int64_t page_size, float eps, int dtype, void *stream) {
     if (dtype != MI_BF16 && dtype != MI_F16)
-        return fail(MI_ERR_UNSUPPORTED, "norm_rope_paged covers bf16 and fp16 (dtype code %d)", dtype);
+        return fail(MI_ERR_UNSUPPORTED, "norm_rope_paged covers bf16 and fp16 (dtype code %d)",
+                    dtype);
     const int lp = page_log2_of(page_size);
     if (lp < 0)
         return fail(MI_ERR_UNSUPPORTED, "page size %lld; this build covers 16, 32, 64, 128, 256",

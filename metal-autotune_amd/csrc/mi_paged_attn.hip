@@ -7,6 +7,15 @@
 // s_j = scale log2(e) q . k_j,  j <= len - n + i;  0 where no key is seen.
 // Key j sits in row j % page_size of page block_table[r][j / page_size].
 //
+// What bounds it, on MI355X: decode (narrow blocks) HBM, 5.8 TB/s of K and V for 48
+// requests of 64 to 8191 keys (136 us; the rest is the chunks' starts and ends), 6.3
+// for 64 of 4096; one request of 1001 keys 8 us, a chain of trips to memory. Prompts
+// (wide blocks) the matrix cores beside the softmax VALU, at the clock that the
+// card's power leaves: 1.0 PFLOP/s over 8192 keys, where a plain matrix product of
+// 8192 reaches 1.2; MFMAs are busy 53% of the cycles, and the clock falls to 1.5-1.9
+// GHz. Dealing the next tile's score MFMAs between this one's exponentials, or eight
+// waves a stage, changed nothing there.
+//
 // The tile, the softmax and the folds are the contiguous attention's
 // (mi_attn_common.h). A kv head's query rows, token after token and in a token
 // its G q heads, are the columns of 32-wide blocks, so K and V are read once per
@@ -14,8 +23,8 @@
 //
 // Requests differ in length, and only the GPU knows the lengths. The keys of
 // every block are therefore cut into chunks of one size, chosen on the GPU from
-// the lengths of all requests so that the chunks fill the chip (chunk_of), and a
-// workgroup finds its chunk by summing over the requests. A block of one chunk
+// the lengths of all requests so that the chunks fill the chip, and a workgroup
+// finds its chunk by summing over the requests (find_item). A block of one chunk
 // writes its rows; the others' states go to a workspace, and the last workgroup of
 // a block to finish folds them, in order. The chunk size, so a row's last bits,
 // depends on the lengths of the whole batch.
@@ -51,21 +60,6 @@ struct PagedArgs {
     float scale;    // > 0, log2 units
     uint32_t flip;  // sign bits of a negative scale, for Q
 };
-
-// The sum of v over the wave's lanes up to and including this one (see
-// paged_plan_kernel's).
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xF>(v);
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);
-    v = dpp_add<0x143, 0xC>(v);
-    return v;
-}
 
 constexpr int CHUNK_KEYS = ATT_KT * PA_WAVES;  // keys are cut in multiples of this
 constexpr int MAX_CHUNKS = 128;  // of a block: one workgroup adds them
@@ -110,8 +104,9 @@ __device__ __forceinline__ int blocks_from(const PagedArgs &a, const Req &q, int
 // Item u: the wide blocks' chunks, then the narrow ones' whole chunks, then what is
 // left of them, each in the order of requests, of their blocks, of their chunks;
 // but the wide ones of at most 64 requests from those that see the most keys to
-// those that see the fewest: what starts last should be short. Every wave finds its item by itself, 64 requests a step: first the
-// runs of all blocks, which give the size of a chunk, then the chunks up to its own.
+// those that see the fewest: what starts last should be short. Every wave finds
+// its item by itself, 64 requests a step: first the runs of all blocks, which give
+// the size of a chunk, then the chunks up to its own.
 template <bool WIDE>
 __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int lane) {
     Req q = load_req<WIDE>(a, lane);
@@ -122,7 +117,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
         for (int r0 = 0;;) {
             const Req next = a.R > r0 + 64 ? load_req<WIDE>(a, r0 + 64 + lane) : q;
             longest = max(longest, q.runs);
-            const uint64_t mine = (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)mean_runs(a, q);
+            const uint64_t mine =
+                (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)mean_runs(a, q);
             const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
             total += (uint64_t)(unsigned)__builtin_amdgcn_readlane(lo, 63) +
                      ((uint64_t)(unsigned)__builtin_amdgcn_readlane(hi, 63) << 24);
@@ -131,9 +127,9 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             q = next;
         }
         total += a.target - 1;
-        runs = total >> 32 ? (int)(total / (unsigned)a.target)
-                           : (int)((unsigned)total / (unsigned)a.target);
-        runs = max(1, runs);
+        const uint64_t each = total >> 32 ? total / (unsigned)a.target
+                                          : (unsigned)total / (unsigned)a.target;
+        runs = each < 1 ? 1 : each < (1u << 30) ? (int)each : 1 << 30;
     }
     PagedItem it;
     it.r = -1;
@@ -188,7 +184,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             const int ns = max(1, (q.runs + per - 1) / per), whole = q.runs / per;
             const int blocks = wide ? q.wide : q.narrow;
             const int some = wide ? ns : kind == 1 ? whole : ns - whole, items = blocks * some;
-            const int end = before + wave_scan(items), state_end = states + wave_scan(scale * blocks * ns);
+            const int end = before + wave_scan(items);
+            const int state_end = states + wave_scan(scale * blocks * ns);
             const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
             if (past) {
                 const int l = __builtin_ctzll(past);
@@ -203,7 +200,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
                 const int each = __builtin_amdgcn_readlane(some, l), b = at / each;
                 it.split = at - b * each + (kind == 2 ? __builtin_amdgcn_readlane(whole, l) : 0);
                 it.cb = wide ? __builtin_amdgcn_readlane(blocks, l) - 1 - b : b;
-                it.first = __builtin_amdgcn_readlane(state_end - scale * blocks * ns, l) + scale * b * it.ns;
+                it.first = __builtin_amdgcn_readlane(state_end - scale * blocks * ns, l) +
+                           scale * b * it.ns;
                 return it;
             }
             before = __builtin_amdgcn_readlane(end, 63);
@@ -376,6 +374,7 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     const int t0 = it.split * it.runs * PA_WAVES + wave;
     const int ntiles = it.ns > 1 ? min(all, (it.split + 1) * it.runs * PA_WAVES) : all;
     char *kslot = lds + wave * 2 * Tl::BYTES, *vslot = kslot + Tl::BYTES;
+    const T *k = (const T *)a.k, *v = (const T *)a.v;
     AttnState<D> st;
     attn_init(st);
     uint4 qf[D / 16];
@@ -388,8 +387,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             int64_t lo, hi;
             pg.rows(0, t0 * ATT_KT, lo, hi);
             const int left = it.len - t0 * ATT_KT;
-            dma_paged_tile<T, D, false, true>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left, ks, lane);
-            dma_paged_tile<T, D, true, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left, vs, lane);
+            dma_paged_tile<T, D, false, true>(k + lo * D, k + hi * D, left, ks, lane);
+            dma_paged_tile<T, D, true, true>(v + lo * D, v + hi * D, left, vs, lane);
         }
         for (int kt = t0; kt < ntiles; kt += PA_WAVES) {  // wave-uniform
             const int nx = kt + PA_WAVES;
@@ -411,8 +410,7 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             for (int s = 0; s < D / 16; ++s) launder(kf[s]);  // the reads have returned
             __builtin_amdgcn_sched_barrier(0);
             if (more)
-                dma_paged_tile<T, D, false, true>((const T *)a.k + lo * D, (const T *)a.k + hi * D, left,
-                                            ks, lane);
+                dma_paged_tile<T, D, false, true>(k + lo * D, k + hi * D, left, ks, lane);
             f32x16 s = attn_scores<T, D>(kf, qf);
             const int k0 = kt * ATT_KT;
             if (k0 + ATT_KT > full) attn_mask(s, end - k0, h2);
@@ -428,8 +426,7 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             __builtin_amdgcn_sched_barrier(0);
             att_wait_lds();  // V's reads have returned
             if (more)
-                dma_paged_tile<T, D, true, true>((const T *)a.v + lo * D, (const T *)a.v + hi * D, left,
-                                           vs, lane);
+                dma_paged_tile<T, D, true, true>(v + lo * D, v + hi * D, left, vs, lane);
         }
     };
     run(kslot, vslot);
@@ -455,7 +452,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     if (wave < D / 32) {
         const float l = f.l + __shfl_xor(f.l, 32, 64);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *(float4 *)(cols_at + r * D + 32 * wave + 8 * j + 4 * h2) = f.o[j];
+        for (int j = 0; j < 4; ++j)
+            *(float4 *)(cols_at + r * D + 32 * wave + 8 * j + 4 * h2) = f.o[j];
         if (wave == 0 && h2 == 0) *(float2 *)(cols_at + 32 * D + 2 * r) = make_float2(l, f.m);
     }
     __syncthreads();
@@ -464,7 +462,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     for (int i = 2 * threadIdx.x; i < have * D; i += 128 * PA_WAVES)
         put_part((float2 *)(o + i), *(float2 *)(cols_at + i));
     if ((int)threadIdx.x < have)
-        put_part((float2 *)(o + 32 * D) + threadIdx.x, *(float2 *)(cols_at + 32 * D + 2 * threadIdx.x));
+        put_part((float2 *)(o + 32 * D) + threadIdx.x,
+                 *(float2 *)(cols_at + 32 * D + 2 * threadIdx.x));
     join_narrow<T, D>(a, it, hk, have, lds);
 }
 
@@ -549,9 +548,11 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         pg.rows(s, kt * ATT_KT, lo, hi);
         const int left = it.len - kt * ATT_KT;
         if (wave < 2)
-            dma_paged_tile<T, D, false, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+            dma_paged_tile<T, D, false, false>(pool + lo * D, pool + hi * D, left,
+                                               dst + wave * Tl::BYTES, lane);
         else
-            dma_paged_tile<T, D, true, false>(pool + lo * D, pool + hi * D, left, dst + wave * Tl::BYTES, lane);
+            dma_paged_tile<T, D, true, false>(pool + lo * D, pool + hi * D, left,
+                                              dst + wave * Tl::BYTES, lane);
     };
     auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more)
                     __attribute__((always_inline)) {
@@ -596,10 +597,12 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
         // the state out; the last workgroup of the block to come here folds all of
         // them, in order, each wave its own columns'
         constexpr int PAIRS = D / 32 * 8;
-        float2 *o = (float2 *)part_at<D>(a, it.first + it.split * (WIDE_COLS / 32) + wave, hk) + lane;
+        float2 *o =
+            (float2 *)part_at<D>(a, it.first + it.split * (WIDE_COLS / 32) + wave, hk) + lane;
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i)
-            put_part(o + 64 * i, make_float2(st.o[i / 8][2 * (i % 8)], st.o[i / 8][2 * (i % 8) + 1]));
+            put_part(o + 64 * i,
+                     make_float2(st.o[i / 8][2 * (i % 8)], st.o[i / 8][2 * (i % 8) + 1]));
         put_part(o + 64 * PAIRS, make_float2(st.l, st.m));
         if (!last_of(a.tickets + (int64_t)it.first * a.HK + hk, it.ns)) return;
         attn_init(st);
@@ -639,7 +642,8 @@ __device__ __forceinline__ void wide_block(const PagedArgs &a, const PagedItem &
 template <int D, bool WIDE> constexpr int paged_per_cu() { return D == 128 ? 2 : (WIDE ? 3 : 4); }
 
 // A wave an item: found once for all kv heads.
-template <bool WIDE> __global__ __launch_bounds__(256) void paged_items_kernel(PagedArgs a, int items) {
+template <bool WIDE>
+__global__ __launch_bounds__(256) void paged_items_kernel(PagedArgs a, int items) {
     const int u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (u >= items) return;
     const PagedItem it = find_item<WIDE>(a, u, threadIdx.x & 63);
@@ -649,7 +653,8 @@ template <bool WIDE> __global__ __launch_bounds__(256) void paged_items_kernel(P
 // One workgroup an item and kv head. WIDE: requests of more than 32 columns are in
 // wide blocks; without it (decode) every block is narrow.
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(64 * PA_WAVES) __attribute__((amdgpu_waves_per_eu(paged_per_cu<D, WIDE>())))
+__global__ __launch_bounds__(64 * PA_WAVES)
+__attribute__((amdgpu_waves_per_eu(paged_per_cu<D, WIDE>())))
 void paged_attn_kernel(PagedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
@@ -660,7 +665,8 @@ void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(PagedItem) / 4); ++i) f[i] = p[i];
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(PagedItem) / 4); ++i) f[i] = __builtin_amdgcn_readfirstlane(f[i]);
+        for (int i = 0; i < (int)(sizeof(PagedItem) / 4); ++i)
+            f[i] = __builtin_amdgcn_readfirstlane(f[i]);
         it = __builtin_bit_cast(PagedItem, f);
     } else {
         it = find_item<WIDE>(a, blockIdx.y, threadIdx.x & 63);
@@ -691,10 +697,11 @@ void paged_attn_kernel(PagedArgs a) {
 // at most `target` chunks and the last, shorter one of every block, and no more
 // than a row of the table has. Few blocks: as many chunks as one round of
 // workgroups takes with those last ones; many: one and a half rounds' worth, the
-// shorter ones last (64 requests of 4096 keys: 171 us, with four rounds' 183). Wide blocks, whose parts cost 66 KB written
-// and read, are then cut only where they fill less than two rounds, past 32 runs
-// (20 requests, four of 256 to 512 tokens and up to 4096 keys: 90 us; from 8 runs
-// on, 103; 8192 tokens of one prompt uncut 562 us, cut past 32 runs 694).
+// shorter ones last (64 requests of 4096 keys: 171 us, with four rounds' 183).
+// Wide blocks, whose parts cost 66 KB written and read, are then cut only where
+// they fill less than two rounds, past 32 runs (20 requests, four of 256 to 512
+// tokens and up to 4096 keys: 90 us; from 8 runs on, 103; 8192 tokens of one prompt
+// uncut 562 us, cut past 32 runs 694).
 struct PagedGrid {
     int64_t wide, narrow, items, states, target, wide_runs;
     bool cut, cut_wide, listed;
@@ -798,7 +805,8 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
                                   float scale, int dtype, void *workspace,
                                   int64_t workspace_bytes, void *stream) {
     if (dtype != MI_BF16 && dtype != MI_F16)
-        return fail(MI_ERR_UNSUPPORTED, "paged attention covers bf16 and fp16 (dtype code %d)", dtype);
+        return fail(MI_ERR_UNSUPPORTED, "paged attention covers bf16 and fp16 (dtype code %d)",
+                    dtype);
     if (D != 64 && D != 128)
         return fail(MI_ERR_UNSUPPORTED, "paged attention head dim %lld", (long long)D);
     int lp;
@@ -808,8 +816,8 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
     if (T < 0 || R < 0 || H < 1 || HK < 1 || H % HK || HK > 65535 || table_width < 1 ||
         n_pages < 1 || n_pages > (0x7fffffff >> lp) || table_width > (0x3fffffff >> lp) ||
         T > 0x3fffffff || T * (H / HK) > 0x3fffffff || R > 0x3fffffff)
-        return fail(MI_ERR_ARG, "paged attention shape T=%lld R=%lld table width %lld H=%lld HK=%lld "
-                    "pages=%lld", (long long)T, (long long)R, (long long)table_width, (long long)H,
+        return fail(MI_ERR_ARG, "paged attention shape T=%lld R=%lld table width %lld H=%lld "
+                    "HK=%lld pages=%lld", (long long)T, (long long)R, (long long)table_width, (long long)H,
                     (long long)HK, (long long)n_pages);
     if (T == 0 || R == 0) return MI_OK;
     if (!q || !k_pages || !v_pages || !out || !block_table || !cu_q || !kv_lens)
@@ -830,8 +838,9 @@ extern "C" int mi_paged_attention(const void *q, const void *k_pages, const void
     char *lists = ws ? ws + MI_PAGED_ZERO_BYTES : nullptr;
     const PagedArgs a = {q, k_pages, v_pages, out, block_table, cu_q, kv_lens,
                          ws && g.listed ? (PagedItem *)lists : nullptr, (unsigned *)ws,
-                         ws && paged_cuts(g, HK) ? (float *)(lists + paged_list_bytes(g)) : nullptr, (int)T, (int)R,
-                         (int)table_width, (int)H, (int)HK, (int)(H / HK), (int)n_pages, lp,
+                         ws && paged_cuts(g, HK) ? (float *)(lists + paged_list_bytes(g)) : nullptr,
+                         (int)T, (int)R, (int)table_width, (int)H, (int)HK, (int)(H / HK),
+                         (int)n_pages, lp,
                          (int)g.target, (int)g.wide_runs, mag, sl < 0.0f ? 0x80008000u : 0u};
     hipStream_t st = as_stream(stream);
     if (dtype == MI_BF16)

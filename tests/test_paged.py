@@ -35,6 +35,7 @@ def _plan(L, table=P, width=4, R=2, T=3, page=16, n_free=8):
     ({"page": 512}, 2, b"page size 512"), ({"R": 0}, 1, b"R=0"), ({"R": 4097}, 1, b"R=4097"),
     ({"width": 0}, 1, b"table width 0"), ({"width": 131073}, 1, b"131073"),
     ({"T": -1}, 1, b"T=-1"), ({"table": None}, 1, b"null"), ({"n_free": -1}, 1, b"free pages -1"),
+    ({"T": 262145}, 1, b"T=262145"),
 ])
 def test_plan_refusals(lib, kw, code, text):
     assert _plan(lib, **kw) == code
@@ -140,6 +141,29 @@ def test_ops_refuse_wrong_arrays():
                   kv_lens=i, scale=1.0)
         with pytest.raises(ValueError):
             ops.paged_attention(**{**kw, **bad})
+
+
+def test_launches_happen_on_the_tensors_device(monkeypatch):
+    """Where the current device is another one, it is changed for the launch."""
+    seen = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            seen.append(self.index)
+
+        def __exit__(self, *a):
+            seen.append("back")
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    with ops._on(1):
+        seen.append("launch")
+    with ops._on(0):
+        seen.append("here")
+    assert seen == [1, "launch", "back", "here"]
 
 
 def test_rope_table():

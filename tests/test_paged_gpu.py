@@ -104,6 +104,30 @@ def test_plan(R, page, kv_hi, q_hi, spare, short):
     assert all(torch.equal(a, b) for a, b in zip(p, again)) and dt.tolist() == want[0]
 
 
+def test_plan_into_an_earlier_one():
+    table, free = i32([[0, 0], [0, 0]]), i32([7, 8, 9, 10])
+    kv, count = i32([0, 0]), i32([4])
+    a = ops.paged_plan(table, kv, i32([3, 17]), free, count, 16, 20)
+    at = [t.data_ptr() for t in a]
+    b = ops.paged_plan(table, i32([3, 17]), i32([20, 0]), free, i32([1]), 16, 20, out=a)
+    assert [t.data_ptr() for t in b] == at and b.kv_lens.tolist() == [23, 17]
+    assert b.cu_q.tolist() == [0, 20, 20] and int(b.free_count) == 0 and int(b.refused) == 0
+    for bad in (dict(num_tokens=21), dict(kv_lens=b.kv_lens), dict(free_count=b.free_count)):
+        kw = dict(block_table=table, kv_lens=kv, q_lens=i32([1, 1]), free_pages=free,
+                  free_count=count, page_size=16, num_tokens=20, out=b)
+        with pytest.raises(ValueError):
+            ops.paged_plan(**{**kw, **bad})
+
+
+def test_plan_of_more_tokens_than_rows():
+    """A request whose tokens pass the rows takes no page; the next ones, neither."""
+    table, free = i32([[0, 0]] * 4), i32([7, 8, 9, 10])
+    p = ops.paged_plan(table, i32([0, 3, 20, 5]), i32([10, 20, 0, 1]), free, i32([4]), 16, 29)
+    assert p.kv_lens.tolist() == [10, 0, 20, 0] and int(p.refused) == 2
+    assert int(p.free_count) == 3 and table.tolist() == [[10, 0], [0, 0], [0, 0], [0, 0]]
+    assert p.slots.tolist() == [160 + i for i in range(10)] + [-1] * 19
+
+
 def test_plan_of_empty_requests():
     p = ops.paged_plan(i32([[5], [6]]), i32([0, 16]), i32([0, 0]), i32([]), i32([0]), 16, 0)
     assert p.cu_q.tolist() == [0, 0, 0] and p.kv_lens.tolist() == [0, 16]
@@ -346,6 +370,32 @@ def test_attention_kernel_hint_changes_no_meaning():
     """max_q_len chooses kernels: too small, too large and absent give the rows."""
     for hint in (1, 7, 500, None):
         run_attention([400, 33, 260], [130, 1, 40], 8, 2, 64, 32, BF, max_q_len=hint)
+
+
+def test_attention_beside_values_that_are_not_finite():
+    """A prompt's last values are not finite: rows whose last key lies 96 keys or
+    more before them, and other requests, do not know. Nor does decode of keys
+    behind which such values lie in the page."""
+    g = gen_of(34)
+    kv, n_q = [300, 90, 33], [300, 1, 33]
+    kp, vp, table, ks, vs = make_cache(g, kv, 16, 2, 64, BF)
+    q, cu = rnd(g, sum(n_q), 8, 64), i32([0, 300, 301, 334])
+    want, size = attention_64(q, ks, vs, n_q, 0.125)
+    for bad in (float("nan"), float("inf")):
+        vp[table[0, 299 // 16], :, 299 % 16] = bad
+        kp[table[0, 299 // 16], :, 299 % 16] = bad
+        out = ops.paged_attention(q, kp, vp, table, cu, i32(kv), 0.125)
+        keep = torch.cat([torch.arange(300 - 96), torch.arange(300, 334)])
+        check_attention(out[keep.to(DEV)], want[keep], size[keep], BF)
+
+
+def test_attention_of_a_misaligned_query():
+    g = gen_of(33)
+    kp, vp, table, ks, vs = make_cache(g, [70], 16, 2, 64, BF)
+    flat = rnd(g, 4 * 64 + 3)
+    q = flat[3:].view(1, 4, 64)
+    out = ops.paged_attention(q, kp, vp, table, i32([0, 1]), i32([70]), 0.125)
+    check_attention(out, *attention_64(q, ks, vs, [1], 0.125), BF)
 
 
 def test_attention_on_streams_and_threads():
