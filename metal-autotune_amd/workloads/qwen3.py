@@ -126,12 +126,14 @@ class PagedKVCache:
 class PagedBatch:
     """``max_requests`` requests over shared pools of ``n_pages`` pages a layer.
 
-    Lengths, block table and free list live on the GPU and are changed in place,
-    so a step can be captured in a graph. ``step(q_lens, num_tokens)`` plans the
-    next one: request r brings q_lens[r] tokens (0: it waits), whose rows lie
-    request after request in a buffer of num_tokens rows; ``plan.refused`` counts
-    the requests for which pages were missing (they keep what they have, and may
-    bring their tokens again). ``finish(r)`` gives a request's pages back."""
+    Lengths, block table, free list and plans live on the GPU and are changed in
+    place, so a step, or its layers one by one, can be captured in graphs.
+    ``step(q_lens, num_tokens)`` plans the next one: request r brings q_lens[r]
+    tokens (0: it waits), whose rows lie request after request in a buffer of
+    num_tokens rows; ``plan.refused`` counts the requests for which pages were
+    missing (they keep what they have, and may bring their tokens again). A plan
+    holds until the next one of as many rows. ``finish(r)`` gives a request's pages
+    back."""
 
     def __init__(self, cfg: "Qwen3Config", n_layers: int, max_requests: int, n_pages: int,
                  page_size: int, max_len: int, device, dtype=torch.bfloat16):
@@ -145,13 +147,15 @@ class PagedBatch:
         self.free_count = i32(1) + n_pages
         self.inv_freq = ops.rope_table(cfg.head_dim, cfg.rope_theta, device=device)
         self.plan, self.max_q_len = None, None
+        self._plans = {}  # by token rows: a graph captured over a plan reads it where it is
         shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
         self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
 
     def step(self, q_lens, num_tokens: int, max_q_len: int | None = None) -> ops.PagedPlan:
         """max_q_len: the most tokens a request brings, where the caller knows it."""
-        p = ops.paged_plan(self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
-                           self.page_size, num_tokens)
+        p = self._plans[num_tokens] = ops.paged_plan(
+            self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
+            self.page_size, num_tokens, out=self._plans.get(num_tokens))
         self.lens.copy_(torch.where(p.kv_lens > 0, p.kv_lens, self.lens))
         self.free_count.copy_(p.free_count)
         self.plan, self.max_q_len = p, max_q_len
@@ -278,11 +282,14 @@ def generate_paged(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
     """Greedy tokens of several prompts at once (1-d int64 arrays, one a request of
     an empty ``batch``): (tokens [n_tokens, R], their ``ops.TokenLogprobs`` a step).
     One prefill step for all prompts, then decode steps; nothing waits for the GPU
-    before the end."""
+    before the end, where a batch whose pages ran out raises."""
     dev = batch.lens.device
     lens = [p.numel() for p in prompts]
+    if n_tokens < 1 or not lens or min(lens) < 1:
+        raise ValueError(f"generate_paged: n_tokens={n_tokens}, prompts of {lens} tokens")
     ids = torch.cat([p.to(dev) for p in prompts])
-    batch.step(torch.tensor(lens, dtype=torch.int32, device=dev), ids.numel(), max(lens))
+    plan = batch.step(torch.tensor(lens, dtype=torch.int32, device=dev), ids.numel(), max(lens))
+    refused = plan.refused.clone()
     one = torch.ones(len(lens), dtype=torch.int32, device=dev)
     tokens, logprobs = [], []
     for i in range(n_tokens):
@@ -292,7 +299,9 @@ def generate_paged(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
         logprobs.append(ops.token_logprobs(logits, ids, top))
         ids = ids.long()
         if i + 1 < n_tokens:
-            batch.step(one, len(lens), 1)
+            refused += batch.step(one, len(lens), 1).refused
+    if int(refused):
+        raise RuntimeError("generate_paged: the batch's pages ran out, or a request's length")
     return torch.stack(tokens), logprobs
 
 

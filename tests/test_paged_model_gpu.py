@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 from autotuner_runtime import hip, ops  # noqa: E402
+from autotuner_runtime.graph import GraphWrapper  # noqa: E402
 from workloads import qwen3  # noqa: E402
 
 DEV = "cuda"
@@ -120,6 +121,43 @@ def test_decode_step_in_a_graph():
         torch.randn(1000, 1000, device=DEV) @ torch.randn(1000, 1000, device=DEV)
         static.copy_(out)
     assert batch.lens.tolist() == end
+
+
+def test_generation_past_the_pages():
+    """Two prompts of 20 and 30 tokens hold four pages of 16; a fourth
+    new token's step needs a fifth, and a row of the table holds 32 tokens here."""
+    model, ps = small(), prompts(20, 30)
+    qwen3.generate_paged(model, model.make_batch(2, 4, page_size=16, max_len=96), ps, 3)
+    for pages, max_len in ((4, 96), (3, 96), (8, 32)):
+        with pytest.raises(RuntimeError, match="ran out"):
+            qwen3.generate_paged(model, model.make_batch(2, pages, page_size=16,
+                                                         max_len=max_len), ps, 6)
+    batch = model.make_batch(2, 8, page_size=16, max_len=96)
+    for bad, n in ((ps, 0), ([], 2), ([ps[0], ps[0][:0]], 2), (ps[:1], 2)):
+        with pytest.raises(ValueError):
+            qwen3.generate_paged(model, batch, bad, n)
+
+
+def test_layers_in_graphs():
+    """Each layer wrapped for graph delivery: captured at the first step of a shape
+    and replayed at the following ones, whose plans say something else."""
+    model, ps, n = small(), prompts(30, 15, 1), 5
+    want_batch = model.make_batch(3, 12, page_size=16, max_len=96)
+    want, _ = qwen3.generate_paged(model, want_batch, ps, n)
+    layers = [GraphWrapper(layer) for layer in model.model.layers]
+    model.model.layers = torch.nn.ModuleList(layers)
+    for _ in range(2):
+        batch = model.make_batch(3, 12, page_size=16, max_len=96)
+        got, _ = qwen3.generate_paged(model, batch, ps, n)
+        assert torch.equal(got, want)
+        for a, b in zip(batch.caches, want_batch.caches):
+            for r in range(3):
+                m = int(batch.lens[r])
+                for w in range(-(-m // 16)):
+                    rows = min(16, m - 16 * w)
+                    i, j = int(batch.block_table[r, w]), int(want_batch.block_table[r, w])
+                    assert torch.equal(a.keys[i, :, :rows], b.keys[j, :, :rows])
+    assert layers[0].stats["replays"] > layers[0].stats["captures"]
 
 
 def test_pages_that_run_out_and_come_back():
