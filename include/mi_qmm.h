@@ -358,16 +358,17 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
                        int dtype, void *stream);
 
 /* Causal attention of every request's new tokens over its pages: q [T, H, D] ->
- * out [T, H, D]. Request r's tokens are rows [cu_q[r], cu_q[r + 1]) (held to T),
- * its keys kv_lens[r] (these tokens' own among them); its token i sees keys
- * j <= kv_lens[r] - n + i with n its tokens (a token that sees none gives 0). Rows of
- * out behind the last request's are left as they were. Page ids outside the pool
- * are held to it. A value that is not finite reaches, beside the rows that see it,
- * the request's rows whose last key lies less than 96 keys before it (they weigh it
- * with 0); keys behind a request's last, or in other pages, reach nothing. max_q_len: the most tokens a request brings, 0 if unknown; it
- * chooses the kernels (no request of more than 32 rows of a kv head, or some),
- * and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a workspace of
- * mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte
+ * out [T, H, D]. Request r's tokens are rows [cu_q[r], cu_q[r + 1]) (held to T;
+ * a cu_q that falls leaves them undefined), its keys kv_lens[r] (these tokens' own
+ * among them); its token i sees keys j <= kv_lens[r] - n + i with n its tokens (a
+ * token that sees none gives 0). Rows of out behind the last request's are left as
+ * they were. Page ids outside the pool are held to it. A value that is not finite
+ * reaches, beside the rows that see it, the request's rows whose last key lies less
+ * than 96 keys before it (they weigh it with 0); keys behind a request's last, or in
+ * other pages, reach nothing. max_q_len: the most tokens a request brings, 0 if
+ * unknown; it chooses the kernels (no request of more than 32 rows of a kv head, or
+ * some), and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a
+ * workspace of mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte
  * aligned) long rows' keys are split over workgroups, and a row's last workgroup
  * adds the parts: the same sums in another order, which depends on all requests'
  * lengths, deterministic for them. The workspace's first MI_PAGED_ZERO_BYTES (a

@@ -70,13 +70,17 @@ constexpr int MAX_CHUNKS = 128;  // of a block: one workgroup adds them
 constexpr int WIDE_COLS = 128;
 struct Req {
     int q0, n, len, wide, narrow, runs;
+    int falls;  // whether it ends before it starts
 };
 template <bool WIDE> __device__ __forceinline__ Req load_req(const PagedArgs &a, int r) {
     Req q;
     const bool in = r < a.R;
-    q.q0 = in ? min(max(a.cu_q[r], 0), a.T) : 0;
-    q.n = in ? min(max(a.cu_q[r + 1], q.q0), a.T) - q.q0 : 0;
-    q.len = in ? min(max(a.kv_lens[r], 0), a.W << a.page_log2) : 0;
+    const int at = min(r, a.R - 1);  // (loads in flight together, no branch)
+    const int from = a.cu_q[at], to = a.cu_q[at + 1], len = a.kv_lens[at];
+    q.falls = to < from;
+    q.q0 = min(max(from, 0), a.T);
+    q.n = in ? min(max(to, q.q0), a.T) - q.q0 : 0;
+    q.len = in ? min(max(len, 0), a.W << a.page_log2) : 0;
     const int cols = q.n * a.G;
     const bool wide = WIDE && cols > 32;
     q.wide = wide ? (cols + WIDE_COLS - 1) / WIDE_COLS : 0;
@@ -113,10 +117,11 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     int runs = 1 << 30, longest = 0;
     if (a.part) {
         // (blocks < 2^16 and runs < 2^23: summed in two halves)
-        uint64_t total = 0;
+        uint64_t total = 0, falls = 0;
         for (int r0 = 0;;) {
             const Req next = a.R > r0 + 64 ? load_req<WIDE>(a, r0 + 64 + lane) : q;
             longest = max(longest, q.runs);
+            falls |= __builtin_amdgcn_ballot_w64(q.falls != 0);
             const uint64_t mine =
                 (uint64_t)(unsigned)(q.wide + q.narrow) * (unsigned)mean_runs(a, q);
             const int lo = wave_scan((int)(mine & 0xFFFFFF)), hi = wave_scan((int)(mine >> 24));
@@ -126,6 +131,9 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             if (r0 >= a.R) break;
             q = next;
         }
+        // requests that overlap could be more blocks than there are items and tickets:
+        // none is taken
+        if (falls) u = 0x7fffffff;
         total += a.target - 1;
         const uint64_t each = total >> 32 ? total / (unsigned)a.target
                                           : (unsigned)total / (unsigned)a.target;

@@ -389,6 +389,24 @@ def test_attention_beside_values_that_are_not_finite():
         check_attention(out[keep.to(DEV)], want[keep], size[keep], BF)
 
 
+@pytest.mark.parametrize("R", [3, 200])
+def test_attention_of_offsets_that_fall(R):
+    """Of long rows nothing is written, and the workspace serves the next call as
+    before."""
+    g = gen_of(35 + R)
+    kv, n_q = [700] * R, [1] * R
+    kp, vp, table, ks, vs = make_cache(g, kv, 16, 1, 64, BF)
+    q, lens = rnd(g, R, 4, 64), i32(kv)
+    good = i32(list(range(R + 1)))
+    want = ops.paged_attention(q, kp, vp, table, good, lens, 0.125, 1)
+    check_attention(want, *attention_64(q, ks, vs, n_q, 0.125), BF)
+    falling = i32([0, R] * R)[:R + 1]
+    mark = torch.full_like(q, 7.0)
+    hip.paged_attention(q, kp, vp, mark, table, falling, lens, 0.125)
+    assert bool((mark == 7).all())
+    assert torch.equal(ops.paged_attention(q, kp, vp, table, good, lens, 0.125, 1), want)
+
+
 def test_attention_of_a_misaligned_query():
     g = gen_of(33)
     kp, vp, table, ks, vs = make_cache(g, [70], 16, 2, 64, BF)
