@@ -352,6 +352,21 @@ def test_attention_of_many_requests_of_all_lengths(R):
     run_attention(kv.tolist(), n_q.tolist(), 8, 2, 128, 16, FP, max_q_len=200)
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_attention_of_random_batches(seed):
+    """Up to 64 requests: none, one, a few or hundreds of new tokens behind none,
+    some or many keys, now and then more tokens than keys; wide blocks by length."""
+    rng = np.random.default_rng(100 + seed)
+    R = int(rng.integers(2, 65))
+    kv = rng.choice([0, 1, 127, 128, 129, 256, 300, 640], R) + rng.integers(0, 40, R)
+    n_q = np.minimum(rng.choice([0, 1, 2, 3, 8, 9, 33, 150], R), kv + (rng.random(R) < 0.1) * 5)
+    G, HK = [(4, 2), (8, 1), (1, 4), (5, 2), (2, 2), (16, 1)][seed]
+    kv[0], n_q[0] = [100, 4000][seed % 2], 60  # one in wide blocks at any of these
+    n_q[1] = max(n_q[1], 1)
+    D, page = [(64, 16), (128, 32)][seed // 3]
+    run_attention(kv.tolist(), n_q.tolist(), G * HK, HK, D, page, [BF, FP][seed % 2])
+
+
 def test_attention_without_a_workspace(monkeypatch):
     """The C entry without scratch: a workgroup a block, the same rows within
     rounding; scratch one byte short takes that path too."""
