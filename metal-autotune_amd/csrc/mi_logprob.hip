@@ -74,16 +74,21 @@ __device__ __forceinline__ float wave_add(float v) {
 
 // What a wave sums is in units of log2: t = x log2 e - C with C = rint(ref log2 e) an
 // integer, p = 2^t, S = sum p, E = sum p t: one fma a value, rounded as finely as t
-// is small, and a step from one C to another scales by a power of two. References
-// beyond 1e30 (a mask's lowest value, where x log2 e overflows; -FLT_MAX before the
-// first value) take t = (x - ref) log2 e instead.
+// is small, and a step from one C to another scales by a power of two. From 2^23 on
+// no rounding to an integer is left in fp32 and C misses ref log2 e by more than 1/2,
+// past 2e9 by more than 2^t can take (a mask of -1e10). References beyond 2^20 (such
+// masks; -FLT_MAX before the first value) take t = (x - ref) log2 e instead.
 struct Sums {
     float ref;   // shared by the wave
     float top;   // the lane's largest value
     float s, e;  // the lane's sums against ref
 };
-__device__ __forceinline__ bool far(float ref) { return !(fabsf(ref) <= 1e30f); }
+__device__ __forceinline__ bool far(float ref) { return !(fabsf(ref) <= 1048576.0f); }
 __device__ __forceinline__ float units(float ref) { return __builtin_rintf(ref * LP_LOG2E); }
+// By how much the sums' zero lies above ref log2 e.
+__device__ __forceinline__ float excess(float ref) {
+    return far(ref) ? 0.0f : __builtin_fmaf(-ref, LP_LOG2E, units(ref));
+}
 // (2^t = 0 for t below -150: the floor keeps a forbidden token's -inf out of 0 * t;
 // NaN reaches s.)
 __device__ __forceinline__ void add_value(Sums &a, float t) {
@@ -99,12 +104,13 @@ __device__ __forceinline__ void move_sums(float &s, float &e, float c) {
     s *= f;
 }
 __device__ __forceinline__ void move_ref(float &s, float &e, float from, float to) {
-    move_sums(s, e, far(from) || far(to) ? (from - to) * LP_LOG2E : units(from) - units(to));
+    move_sums(s, e, far(from) || far(to) ? (from - to) * LP_LOG2E + (excess(from) - excess(to))
+                                         : units(from) - units(to));
 }
 // ... against the row's maximum itself.
 __device__ __forceinline__ void move_to(float &s, float &e, float from, float m) {
-    move_sums(s, e, far(from) || far(m) ? (from - m) * LP_LOG2E
-                                        : __builtin_fmaf(-m, LP_LOG2E, units(from)));
+    move_sums(s, e, far(from) ? (from - m) * LP_LOG2E
+                              : __builtin_fmaf(-m, LP_LOG2E, units(from)));
 }
 
 // The order of floats as the order of ints (-0 as 0); what is no value is NONE.
