@@ -36,10 +36,11 @@
 extern "C" {
 #endif
 
-#define MI_ABI_VERSION 8  /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
+#define MI_ABI_VERSION 9  /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
                              4: mi_argmax_noalloc; 5: the qmm workspace entries;
                              6: mi_qmm_affine_qkv_norm_rope; 7: mi_sdpa_ws;
-                             8: the paged cache entries, mi_token_logprobs */
+                             8: the paged cache entries, mi_token_logprobs;
+                             9: mi_stream_capture_id */
 
 enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 };
 
@@ -57,6 +58,10 @@ int mi_abi_version(void);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char *mi_last_error(void);
+
+/* The number of the graph capture that the stream takes part in (each capture of a
+ * process has its own); MI_ERR_ARG if it is not being captured. */
+int mi_stream_capture_id(void *stream, uint64_t *id);
 
 /* mx.dequantize(w, scales, biases, group_size, bits) (affine mode):
  * out[n, k] = T(fma(s[n, k/gs], q(n, k), b[n, k/gs])), one rounding.

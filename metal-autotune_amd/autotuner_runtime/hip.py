@@ -25,7 +25,7 @@ import torch
 
 PKG = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("MI_QMM_LIB", PKG / "libmiqmm.so"))
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 MI_OK, MI_ERR_ARG, MI_ERR_UNSUPPORTED, MI_ERR_LAUNCH = 0, 1, 2, 3
@@ -39,6 +39,7 @@ _P, _I64, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 SIGNATURES: dict[str, list] = {
     "mi_abi_version": [],
     "mi_last_error": [],
+    "mi_stream_capture_id": [_P, ctypes.POINTER(ctypes.c_uint64)],
     "mi_affine_dequant": [_P, _P, _P, _P, _I64, _I64, _I, _I, _I, _P],
     "mi_affine_gather_dequant": [_P, _I64, _I, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _P],
     "mi_qmm_affine": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _I, _P],
@@ -543,8 +544,11 @@ def b_linear_f32(ins, outs, p):
 # own. Either way the buffer is kept alive as long as the process, since a graph
 # may replay at any time, also one that has to grow (the earlier calls' nodes
 # hold its address). It is made at the size asked for, and a fill, where one is
-# needed, is a node that every replay repeats.
+# needed, is a node of the graph that every replay repeats. Each graph of a scope
+# has its own, before its first use of the buffer: another graph's would not have
+# run where this one is replayed first.
 _captured: dict[tuple, torch.Tensor] = {}
+_filled: dict[tuple, int] = {}  # the capture that last zeroed the buffer
 _retired: list[torch.Tensor] = []
 _scope = threading.local()   # .token: the capture scope; .eager: the thread's workspaces
 
@@ -552,13 +556,21 @@ _scope = threading.local()   # .token: the capture scope; .eager: the thread's w
 @contextlib.contextmanager
 def graph_workspaces():
     """A scope whose graph captures share workspaces of their own (no other
-    graph or stream uses them). GraphWrapper captures each graph in one."""
+    graph or stream uses them): its graphs may be replayed in any order, but not
+    at the same time. GraphWrapper captures each graph in one."""
     prev = getattr(_scope, "token", None)
     _scope.token = object()
     try:
         yield
     finally:
         _scope.token = prev
+
+
+def _capture_id(stream: int) -> int:
+    """The number of the capture that the stream takes part in."""
+    number = ctypes.c_uint64()
+    _check(lib().mi_stream_capture_id(stream, ctypes.byref(number)), "graph capture")
+    return number.value
 
 
 def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
@@ -576,7 +588,8 @@ def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
         token = getattr(_scope, "token", None)
         key = (kind, device, stream, token)
         ws = None if token is None else _captured.get(key)
-        if ws is None or ws.numel() < nbytes:
+        fresh = ws is None or ws.numel() < nbytes
+        if fresh:
             if ws is not None:
                 _retired.append(ws)
             ws = make(max(nbytes, 4096))
@@ -584,6 +597,11 @@ def _workspace(kind: str, device, stream: int, nbytes: int, minimum: int = 4096,
                 _retired.append(ws)
             else:
                 _captured[key] = ws
+        if zero and token is not None:
+            capture = _capture_id(stream)
+            if not fresh and _filled.get(key) != capture:
+                (ws if zero is True else ws[:zero]).zero_()
+            _filled[key] = capture
         return ws
     eager = getattr(_scope, "eager", None)
     if eager is None:

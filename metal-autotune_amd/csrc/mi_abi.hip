@@ -41,4 +41,19 @@ int check_quant(int64_t N, int64_t K, int group_size, int bits, int dtype) {
 
 extern "C" int mi_abi_version(void) { return MI_ABI_VERSION; }
 
+extern "C" int mi_stream_capture_id(void *stream, uint64_t *id) {
+    if (!id) return mi::fail(MI_ERR_ARG, "null pointer");
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long number = 0;
+    const hipError_t e = hipStreamGetCaptureInfo(mi::as_stream(stream), &status, &number);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // (not the next launch's)
+        return mi::fail(MI_ERR_LAUNCH, "stream capture: %s", hipGetErrorString(e));
+    }
+    if (status != hipStreamCaptureStatusActive)
+        return mi::fail(MI_ERR_ARG, "the stream is not being captured");
+    *id = number;
+    return MI_OK;
+}
+
 extern "C" const char *mi_last_error(void) { return g_error; }
