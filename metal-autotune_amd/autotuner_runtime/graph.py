@@ -17,7 +17,9 @@ kernel's host-side dispatch.
   state holder (an object whose attributes hold tensors or plain values,
   e.g. a KV cache with its offset) by its attributes: plain values by value,
   tensors by shape/dtype and storage address (the graph writes into them in
-  place, so the same buffers must come back).
+  place, so the same buffers must come back). An object whose further state a
+  graph reads (the batch behind a paged cache: block table, plan) names that
+  state by ``graph_key``, any hashable that no other state shares.
 - First call of a signature: the holders' attributes are saved, the scope
   runs once eagerly (library loading and allocation happen outside capture),
   the attributes are restored, the call is captured with its tensor
@@ -65,7 +67,7 @@ def _attr_sig(v, carried: bool):
         return ("t", tuple(v.shape), str(v.dtype), str(v.device), v.data_ptr())
     if v is None or isinstance(v, (bool, int, float, str)):
         return ("v", v)
-    return ("o", type(v).__name__)
+    return ("o", type(v).__name__, getattr(v, "graph_key", None))
 
 
 def signature(args, carried=frozenset()) -> tuple:
@@ -78,7 +80,7 @@ def signature(args, carried=frozenset()) -> tuple:
             sig.append(("T", tuple(a.shape), str(a.dtype), str(a.device)))
         elif _is_holder(a):
             name = type(a).__name__
-            sig.append(("H", name, tuple(sorted(
+            sig.append(("H", name, getattr(a, "graph_key", None), tuple(sorted(
                 (k, _attr_sig(v, (name, k) in carried)) for k, v in vars(a).items()))))
         elif isinstance(a, (list, tuple)):
             sig.append(("L", signature(a, carried)))

@@ -147,6 +147,9 @@ class PagedBatch:
         self.free_count = i32(1) + n_pages
         self.inv_freq = ops.rope_table(cfg.head_dim, cfg.rope_theta, device=device)
         self.plan, self.max_q_len = None, None
+        # what a captured graph reads beside its tensors: this batch's, at this plan
+        self._name = object()
+        self.graph_key = (self._name, None)
         self._plans = {}  # by token rows: a graph captured over a plan reads it where it is
         shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
         self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
@@ -159,6 +162,7 @@ class PagedBatch:
         self.lens.copy_(torch.where(p.kv_lens > 0, p.kv_lens, self.lens))
         self.free_count.copy_(p.free_count)
         self.plan, self.max_q_len = p, max_q_len
+        self.graph_key = (self._name, p.cu_q.data_ptr())
         return p
 
     def finish(self, r: int) -> None:
