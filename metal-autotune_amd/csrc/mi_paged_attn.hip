@@ -44,7 +44,8 @@ struct PagedItem {
     int split, ns;   // chunk of the block's keys, chunks (a request's earlier wide
                      // blocks have fewer than its last: split >= ns is no work)
     int runs;        // CHUNK_KEYS runs a chunk
-    int first;       // the block's first state in the workspace (of 32 columns each)
+    int first;       // the block's first state in the workspace (of 32 columns each),
+                     // where it is cut
 };
 
 struct PagedArgs {
@@ -141,7 +142,7 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     }
     PagedItem it;
     it.r = -1;
-    int before = 0, states = 0, narrow_states = 0;  // items, and states of 32 columns
+    int before = 0, states = 0, narrow_states = 0;  // items, and cut blocks' states
 #pragma unroll
     for (int kind = WIDE ? 0 : 1; kind < 3; ++kind) {
         const bool wide = kind == 0;
@@ -150,8 +151,9 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             const int per = max(max(runs, a.wide_runs), (q.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
             const int ns = max(1, (q.runs + per - 1) / per);
             const int end = wave_scan(q.wide * ns);
+            const int state_items = ns > 1 ? q.wide * ns : 0, state_end = wave_scan(state_items);
             before = __builtin_amdgcn_readlane(end, 63);
-            states = scale * before;
+            states = scale * __builtin_amdgcn_readlane(state_end, 63);
             if (u >= before) continue;
             // the largest L of which more than u items see at least L runs
             int lo = 0, hi = ((a.W << a.page_log2) + CHUNK_KEYS - 1) / CHUNK_KEYS + 1, above = 0;
@@ -176,7 +178,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             const int p = u - __builtin_amdgcn_readlane(upto - at, l), b = p / it.ns;
             it.split = p - b * it.ns;
             it.cb = __builtin_amdgcn_readlane(q.wide - have, l) + b;
-            it.first = scale * (__builtin_amdgcn_readlane(end - q.wide * ns, l) + it.cb * it.ns);
+            it.first =
+                scale * (__builtin_amdgcn_readlane(state_end - state_items, l) + it.cb * it.ns);
             return it;
         }
         if (kind == 1) {
@@ -193,7 +196,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
             const int blocks = wide ? q.wide : q.narrow;
             const int some = wide ? ns : kind == 1 ? whole : ns - whole, items = blocks * some;
             const int end = before + wave_scan(items);
-            const int state_end = states + wave_scan(scale * blocks * ns);
+            const int state_items = ns > 1 ? scale * blocks * ns : 0;
+            const int state_end = states + wave_scan(state_items);
             const uint64_t past = __builtin_amdgcn_ballot_w64(end > u);
             if (past) {
                 const int l = __builtin_ctzll(past);
@@ -208,8 +212,8 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
                 const int each = __builtin_amdgcn_readlane(some, l), b = at / each;
                 it.split = at - b * each + (kind == 2 ? __builtin_amdgcn_readlane(whole, l) : 0);
                 it.cb = wide ? __builtin_amdgcn_readlane(blocks, l) - 1 - b : b;
-                it.first = __builtin_amdgcn_readlane(state_end - scale * blocks * ns, l) +
-                           scale * b * it.ns;
+                it.first =
+                    __builtin_amdgcn_readlane(state_end - state_items, l) + scale * b * it.ns;
                 return it;
             }
             before = __builtin_amdgcn_readlane(end, 63);
@@ -736,23 +740,27 @@ inline PagedGrid paged_grid(int64_t T, int64_t R, int64_t W, int64_t G, int64_t 
     g.wide_runs = few >= slots / 2 ? 1 : g.wide * HK < 2 * slots ? 32 : 1 << 23;
     g.cut = runs > 1;
     g.cut_wide = g.wide && runs > g.wide_runs;
-    int64_t wide = g.wide, narrow = g.narrow;  // chunks of each kind
+    // Chunks of each kind, and those of cut blocks, which have states: a block cut
+    // in two or more has at most twice its runs over a chunk's.
+    int64_t wide = g.wide, narrow = g.narrow, wide_states = 0, narrow_states = 0;
     if (g.cut_wide) {
         // (the chunks are counted by a request's last block, their size comes from
         // the mean: up to twice as many)
         const int64_t most = g.wide * ceil_div(runs, g.wide_runs), some = g.wide + 2 * g.target;
         wide = some < most ? some : most;
+        wide_states = wide < 4 * g.target ? wide : 4 * g.target;
     }
     if (g.cut) {
         const int64_t most = g.narrow * runs;
         narrow = g.narrow + g.target < most ? g.narrow + g.target : most;
+        narrow_states = narrow < 2 * g.target ? narrow : 2 * g.target;
     }
     g.items = wide + narrow;
     // Past 192 requests a workgroup would sum over them for longer than a launch
     // takes that lists the items once (1000 requests of 300 keys: 222 us, without
     // 423; 300 of 600: 128, 140; 129 of 1000: 96, 90).
     g.listed = R > 192;
-    g.states = wide * (WIDE_COLS / 32) + narrow;
+    g.states = wide_states * (WIDE_COLS / 32) + narrow_states;
     return g;
 }
 // The tickets take a fixed prefix of the workspace, so that calls of any sizes can
