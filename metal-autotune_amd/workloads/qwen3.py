@@ -123,6 +123,13 @@ class PagedKVCache:
         self.values = torch.zeros_like(self.keys)
 
 
+KEPT_PLANS = 64  # row counts whose plans a PagedBatch keeps, beside captured ones
+
+
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class PagedBatch:
     """``max_requests`` requests over shared pools of ``n_pages`` pages a layer.
 
@@ -132,8 +139,9 @@ class PagedBatch:
     tokens (0: it waits), whose rows lie request after request in a buffer of
     num_tokens rows; ``plan.refused`` counts the requests for which pages were
     missing (they keep what they have, and may bring their tokens again). A plan
-    holds until the next one of as many rows. ``finish(r)`` gives a request's pages
-    back."""
+    holds until the next one of as many rows, which is written in its place where it
+    is one of the last ``KEPT_PLANS`` row counts' or a graph capture made it or read
+    it as ``plan`` (the layers do). ``finish(r)`` gives a request's pages back."""
 
     def __init__(self, cfg: "Qwen3Config", n_layers: int, max_requests: int, n_pages: int,
                  page_size: int, max_len: int, device, dtype=torch.bfloat16):
@@ -146,23 +154,37 @@ class PagedBatch:
         self.free_pages = torch.arange(n_pages, dtype=torch.int32, device=device)
         self.free_count = i32(1) + n_pages
         self.inv_freq = ops.rope_table(cfg.head_dim, cfg.rope_theta, device=device)
-        self.plan, self.max_q_len = None, None
+        self.max_q_len = None
         # what a captured graph reads beside its tensors: this batch's, at this plan
         self._name = object()
         self.graph_key = (self._name, None)
-        self._plans = {}  # by token rows: a graph captured over a plan reads it where it is
+        # by token rows; the captured ones are where a graph reads or writes them
+        self._plan, self._plans, self._captured = None, {}, {}
         shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
         self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
 
     def step(self, q_lens, num_tokens: int, max_q_len: int | None = None) -> ops.PagedPlan:
         """max_q_len: the most tokens a request brings, where the caller knows it."""
-        p = self._plans[num_tokens] = ops.paged_plan(
+        p = ops.paged_plan(
             self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
-            self.page_size, num_tokens, out=self._plans.get(num_tokens))
+            self.page_size, num_tokens,
+            out=self._captured.get(num_tokens) or self._plans.get(num_tokens))
+        self._plans.pop(num_tokens, None)
+        self._plans[num_tokens] = p  # the last
+        if len(self._plans) > KEPT_PLANS:
+            del self._plans[next(iter(self._plans))]
         self.lens.copy_(torch.where(p.kv_lens > 0, p.kv_lens, self.lens))
         self.free_count.copy_(p.free_count)
-        self.plan, self.max_q_len = p, max_q_len
+        self._plan, self.max_q_len = p, max_q_len
         self.graph_key = (self._name, p.cu_q.data_ptr())
+        return self.plan
+
+    @property
+    def plan(self) -> ops.PagedPlan | None:
+        """The last step's plan."""
+        p = self._plan
+        if p is not None and _capturing(p.slots):
+            self._captured[p.slots.shape[0]] = p
         return p
 
     def finish(self, r: int) -> None:
@@ -185,12 +207,13 @@ class Attention(nn.Module):
         """The planned step's attention from its q, k and v [1, T, heads * D]:
         [1, T, H * D]."""
         c, b = self.cfg, cache.batch
+        plan = b.plan
         qr = ops.norm_rope_paged(q[0], k[0], v[0], self.q_norm.weight, self.k_norm.weight,
                                  c.num_attention_heads, c.num_key_value_heads, c.rms_norm_eps,
-                                 b.inv_freq, b.plan.positions, b.plan.slots, cache.keys,
+                                 b.inv_freq, plan.positions, plan.slots, cache.keys,
                                  cache.values)
-        o = ops.paged_attention(qr, cache.keys, cache.values, b.block_table, b.plan.cu_q,
-                                b.plan.kv_lens, self.scale, b.max_q_len)
+        o = ops.paged_attention(qr, cache.keys, cache.values, b.block_table, plan.cu_q,
+                                plan.kv_lens, self.scale, b.max_q_len)
         return o.view(1, o.shape[0], -1)
 
     def forward(self, x, cache: KVCache | PagedKVCache):
