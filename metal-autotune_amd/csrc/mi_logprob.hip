@@ -91,10 +91,10 @@ __device__ __forceinline__ float excess(float ref) {
 }
 // (2^t = 0 for t below -150: the floor keeps a forbidden token's -inf out of 0 * t;
 // NaN reaches s.)
-__device__ __forceinline__ void add_value(Sums &a, float t) {
+__device__ __forceinline__ void add_value(float &s, float &e, float t) {
     const float p = __builtin_amdgcn_exp2f(t);
-    a.s += p;
-    a.e = __builtin_fmaf(p, fmaxf(t, -300.0f), a.e);
+    s += p;
+    e = __builtin_fmaf(p, fmaxf(t, -300.0f), e);
 }
 // Sums against a reference c units higher.
 __device__ __forceinline__ void move_sums(float &s, float &e, float c) {
@@ -228,18 +228,24 @@ __device__ __forceinline__ void add_chunk(Sums &a, const Piece<T> (&pc)[Row<T>::
         move_ref(a.s, a.e, a.ref, to);
         a.ref = to;
     }
+    // a chunk's values by themselves first: two short chains of roundings, not one
+    // through the row's values
+    float s = 0.0f, e = 0.0f;
     if (far(a.ref)) {  // (uniform)
 #pragma unroll
         for (int i = 0; i < PER; ++i)
 #pragma unroll
-            for (int e = 0; e < N; ++e) add_value(a, (pc[i].f[e] - a.ref) * LP_LOG2E);
+            for (int j = 0; j < N; ++j) add_value(s, e, (pc[i].f[j] - a.ref) * LP_LOG2E);
     } else {
         const float c2 = units(a.ref);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
 #pragma unroll
-            for (int e = 0; e < N; ++e) add_value(a, __builtin_fmaf(pc[i].f[e], LP_LOG2E, -c2));
+            for (int j = 0; j < N; ++j)
+                add_value(s, e, __builtin_fmaf(pc[i].f[j], LP_LOG2E, -c2));
     }
+    a.s += s;
+    a.e += e;
 }
 
 // The chunks c0, c0 + STEP, ... below c1 of a row, by one wave. The row's ends come
