@@ -60,15 +60,25 @@ __device__ __forceinline__ void attn_mask(f32x16 &s, int vis, int h2) {
         s[i] = 8 * (i / 4) + 4 * h2 + (i % 4) < vis ? s[i] : -INFINITY;
 }
 
+// What rounding to T took from two values, in T.
+template <typename T> __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t pk) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    const T2 v = __builtin_bit_cast(T2, pk);
+    return pk2<T>(a - (float)v[0], b - (float)v[1]);
+}
+
 // Scores to probabilities of one key tile: s[i] = S^T (key 8*(i/4) + 4*h2 +
 // i%4 of the tile, the lane's query row; -inf where the row does not see the
 // key), pk gets 2^(s scale - m) in pairs of T, in register order. The row sum
 // adds the fp32 values, in four chains (rounded to T first, the denominator
-// would carry T's error of a probability, up to 2^-8 in bf16). scale > 0 (a
-// negative scale was moved into Q's sign).
-template <typename T, int D>
+// would carry T's error of a probability, up to 2^-9 in bf16). The pairs are
+// operands of the second product's MFMAs, hence in T: of a result's norm that rounding
+// costs about what the result's own does (300 rows over 1000 keys 2.2e-3 in bf16, where
+// 1.7e-3 is the least that bf16 can hold). REST: rest gets what it took, for a
+// product of its own. scale > 0 (a negative scale was moved into Q's sign).
+template <typename T, int D, bool REST = false>
 __device__ __forceinline__ void attn_softmax(AttnState<D> &st, const f32x16 &s, uint32_t (&pk)[8],
-                                             float scale) {
+                                             float scale, uint32_t *rest = nullptr) {
 #pragma clang fp contract(off)
     float mt = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -98,6 +108,7 @@ __device__ __forceinline__ void attn_softmax(AttnState<D> &st, const f32x16 &s, 
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, nm));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], scale, nm));
         pk[i] = pk2<T>(p0, p1);
+        if constexpr (REST) rest[i] = rest2<T>(p0, p1, pk[i]);
         float &a = sum[2 * (i & 1)], &b = sum[2 * (i & 1) + 1];
         a = i < 2 ? p0 : a + p0;
         b = i < 2 ? p1 : b + p1;

@@ -16,6 +16,13 @@
 // GHz. Dealing the next tile's score MFMAs between this one's exponentials, or eight
 // waves a stage, changed nothing there.
 //
+// Probabilities enter the second product as T. Narrow blocks, whose MFMAs wait for HBM,
+// take the product of what that rounding left too: what is off is then the result's own
+// rounding (one row over 4096 keys: 2.0e-3 -> 1.67e-3 of the norm in bf16, 2.6e-4 ->
+// 2.1e-4 in fp16; 48 requests 136.8 -> 137.5 us). Wide blocks do not (2.2e-3 and
+// 2.8e-4): they are bound by these products (8192 tokens 526 -> 694 us with it, four
+// prompts of 2048 161 -> 203).
+//
 // The tile, the softmax and the folds are the contiguous attention's
 // (mi_attn_common.h). A kv head's query rows, token after token and in a token
 // its G q heads, are the columns of 32-wide blocks, so K and V are read once per
@@ -28,6 +35,8 @@
 // writes its rows; the others' states go to a workspace, and the last workgroup of
 // a block to finish folds them, in order. The chunk size, so a row's last bits,
 // depends on the lengths of the whole batch.
+#include <type_traits>
+
 #include "mi_attn_common.h"
 
 namespace mi {
@@ -359,6 +368,17 @@ template <int STEP> struct TilePages {
     }
 };
 
+// Whether a wave's sums have a NaN (or infinities of both signs).
+template <int D> __device__ __forceinline__ bool not_a_number(const AttnState<D> &st) {
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i & 3] += st.o[t][i];
+    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    return __builtin_amdgcn_ballot_w64(all != all) != 0;
+}
+
 // A narrow block: wave w takes the key tiles w, w + 4, ... of the chunk into LDS of
 // its own (a K and a V slot, refilled as soon as their reads are in registers: no
 // barrier), and the four states are folded at the end. Bound by HBM: K and V are
@@ -391,7 +411,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
     attn_init(st);
     uint4 qf[D / 16];
     uint32_t flip = a.flip;
-    auto run = [&](char *__restrict__ ks, char *__restrict__ vs) __attribute__((always_inline)) {
+    auto run = [&](char *__restrict__ ks, char *__restrict__ vs, auto with_rest)
+                   __attribute__((always_inline)) {
         read_q<D>((const T *)a.q + qrow * D, h2, qf);
         TilePages<PA_WAVES> pg(a, it.r, hk);
         if (t0 < ntiles) {
@@ -426,8 +447,8 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             f32x16 s = attn_scores<T, D>(kf, qf);
             const int k0 = kt * ATT_KT;
             if (k0 + ATT_KT > full) attn_mask(s, end - k0, h2);
-            uint32_t p[8];
-            attn_softmax<T, D>(st, s, p, a.scale);
+            uint32_t p[8], rest[8];
+            attn_softmax<T, D, with_rest.value>(st, s, p, a.scale, rest);
             if (more)
                 att_wait_vmcnt<Tl::NI>();
             else
@@ -435,13 +456,21 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
             VFrag<T, D> vf;
             read_v<T, D>(vs, vf, lane);
             attn_pv<T, D>(st, p, vf);
+            if constexpr (with_rest.value) attn_pv<T, D>(st, rest, vf);
             __builtin_amdgcn_sched_barrier(0);
             att_wait_lds();  // V's reads have returned
             if (more)
                 dma_paged_tile<T, D, true, true>(v + lo * D, v + hi * D, left, vs, lane);
         }
     };
-    run(kslot, vslot);
+    run(kslot, vslot, std::true_type{});
+    // an infinite value times a rest of 0, or below it, leaves NaN: once more, without
+    // the rests
+    if (not_a_number(st)) {
+        flip = a.flip;
+        attn_init(st);
+        run(kslot, vslot, std::false_type{});
+    }
 
     // fold (0 + 1) + (2 + 3): wave t folds O^T tile t
     __syncthreads();
