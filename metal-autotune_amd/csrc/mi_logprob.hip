@@ -17,10 +17,11 @@
 // them, reads the k best chunks again and keeps what reaches the k-th maximum
 // (as good as k values in all, but for ties) in a list, a lane an entry.
 //
-// Bound by HBM at many rows (the row's one read, 9.5 VALU instructions a value of
-// the 13 that fit beside it: 1024 rows of 151936 bf16, 311 MB, 55.8 us, 5.6 TB/s); by the launch and its trips to memory, one after
+// Bound by HBM at many rows (the row's one read, 8.7 VALU instructions a value of
+// the 13 that fit beside it: 1024 rows of 151936 bf16, 311 MB, 57.4 us back to back,
+// 5.4 TB/s; fp32, 622 MB, 97 us, 6.4); by the launch and its trips to memory, one after
 // another, at few, where a row is split over workgroups (one row of as many, with its
-// 5 likeliest: 9.3 us).
+// 5 likeliest: 10.0 us).
 #include <math.h>
 
 #include "mi_common.h"

@@ -9,11 +9,11 @@
 //
 // What bounds it, on MI355X: decode (narrow blocks) HBM, 5.8 TB/s of K and V for 48
 // requests of 64 to 8191 keys (136 us; the rest is the chunks' starts and ends), 6.3
-// for 64 of 4096; one request of 1001 keys 8 us, a chain of trips to memory. Prompts
-// (wide blocks) the matrix cores beside the softmax VALU, at the clock that the
-// card's power leaves: 1.0 PFLOP/s over 8192 keys, where a plain matrix product of
-// 8192 reaches 1.2; MFMAs are busy 53% of the cycles, and the clock falls to 1.5-1.9
-// GHz. Dealing the next tile's score MFMAs between this one's exponentials, or eight
+// for 64 of 4096 (170 us); one request of 1001 keys 9.5 us (8.4 at least), a chain of
+// trips to memory. Prompts (wide blocks) the matrix cores beside the softmax VALU, at
+// the clock that the card's power leaves: 1.0 PFLOP/s over 8192 keys (526 to 552 us from
+// card to card), where a plain matrix product of 8192 reaches 1.2; MFMAs are busy 52% of
+// the cycles, and the clock falls to 1.5-1.9 GHz. Dealing the next tile's score MFMAs between this one's exponentials, or eight
 // waves a stage, changed nothing there.
 //
 // Probabilities enter the second product as T. Narrow blocks, whose MFMAs wait for HBM,
@@ -741,8 +741,10 @@ void paged_attn_kernel(PagedArgs a) {
 // shorter ones last (64 requests of 4096 keys: 171 us, with four rounds' 183).
 // Wide blocks, whose parts cost 66 KB written and read, are then cut only where
 // they fill less than two rounds, past 32 runs (20 requests, four of 256 to 512
-// tokens and up to 4096 keys: 90 us; from 8 runs on, 103; 8192 tokens of one prompt
-// uncut 562 us, cut past 32 runs 694).
+// tokens and up to 4096 keys: 89 us; from 8 runs on, 97). Past two rounds the longest
+// block's chain is mostly hidden (8192 tokens of one prompt 542 us; cut past 32 runs as
+// well, 554), but not where one request's keys outgrow the others' by far: 512 tokens
+// behind 32256 keys beside eight prompts of 1024 take 777 us, and cut 397.
 struct PagedGrid {
     int64_t wide, narrow, items, states, target, wide_runs;
     bool cut, cut_wide, listed;
