@@ -370,7 +370,8 @@ int mi_norm_rope_paged(const void *q, const void *k, const void *v, int64_t q_ro
  * they were. Page ids outside the pool are held to it. A value that is not finite
  * reaches, beside the rows that see it, the request's rows whose last key lies less
  * than 96 keys before it (they weigh it with 0); keys behind a request's last, or in
- * other pages, reach nothing. max_q_len: the most tokens a request brings, 0 if
+ * other pages, reach nothing. (Other rows and heads over the same values may differ in
+ * what rounding their probabilities leaves.) max_q_len: the most tokens a request brings, 0 if
  * unknown; it chooses the kernels (no request of more than 32 rows of a kv head, or
  * some), and all lengths are right with any. bf16 and fp16, D in {64, 128}. With a
  * workspace of mi_paged_attention_workspace_bytes(...) bytes (0: nothing to split; 16-byte

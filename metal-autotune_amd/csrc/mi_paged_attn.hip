@@ -13,8 +13,8 @@
 // trips to memory. Prompts (wide blocks) the matrix cores beside the softmax VALU, at
 // the clock that the card's power leaves: 1.0 PFLOP/s over 8192 keys (526 to 552 us from
 // card to card), where a plain matrix product of 8192 reaches 1.2; MFMAs are busy 52% of
-// the cycles, and the clock falls to 1.5-1.9 GHz. Dealing the next tile's score MFMAs between this one's exponentials, or eight
-// waves a stage, changed nothing there.
+// the cycles, and the clock falls to 1.5-1.9 GHz. Dealing the next tile's score MFMAs
+// between this one's exponentials, or eight waves a stage, changed nothing there.
 //
 // Probabilities enter the second product as T. Narrow blocks, whose MFMAs wait for HBM,
 // take the product of what that rounding left too: what is off is then the result's own
