@@ -36,11 +36,12 @@
 extern "C" {
 #endif
 
-#define MI_ABI_VERSION 9  /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
+#define MI_ABI_VERSION 10 /* 2: mi_argmax takes a workspace; 3: mi_gelu_mlp_f32;
                              4: mi_argmax_noalloc; 5: the qmm workspace entries;
                              6: mi_qmm_affine_qkv_norm_rope; 7: mi_sdpa_ws;
                              8: the paged cache entries, mi_token_logprobs;
-                             9: mi_stream_capture_id */
+                             9: mi_stream_capture_id;
+                             10: mi_beam_select */
 
 enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 };
 
@@ -410,6 +411,30 @@ int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_s
                       const void *tokens, int tokens_are_64, int top, float *logprobs,
                       float *entropy, int32_t *top_ids, float *top_logprobs, int dtype,
                       void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Beam search's choice (no counterpart in the reference, which samples greedily): of
+ * each of R prompts the K best continuations of its B beams. Row r B + b of logits T
+ * [R B, V] (row stride row_stride elements) is beam b of prompt r; scores [R, B] are the
+ * beams' (a sum of log probabilities, say). Candidate (b, v) has (x[b, v] - lse_b) +
+ * score_b, lse_b the row's log sum exp; a beam that has finished (finished [R, B], bytes,
+ * not 0; NULL: none) has one, (b, eos), at its own score, and its logits are not read. A
+ * beam whose score is -inf or NaN has none, nor has a row with a NaN or +inf; logits of
+ * -inf are no candidates. The best first: within a beam by logits, the lowest token first
+ * among equal ones; across beams by the candidates in 64 bits (lse_b to about 1e-7), the
+ * lowest beam first among equals. Written, [R, K] each: out_scores (rounded to fp32 once);
+ * parents, the row r B + b of each; tokens; out_finished, 1 where the parent had finished
+ * or the token is eos (-1: none is). Where there are fewer than K candidates the rest is
+ * -inf, r B, 0, 0. 0 <= R <= 4096, 1 <= B <= 64, 1 <= K <= min(64, B V), V <= 2^20.
+ * workspace: device memory of mi_beam_select_workspace_bytes(...) bytes, 16-byte aligned,
+ * whose first MI_BEAM_ZERO_BYTES (a fixed prefix) are zero before its first use; every
+ * call leaves them zero. Calls sharing one must not overlap. */
+#define MI_BEAM_ZERO_BYTES 18432
+int64_t mi_beam_select_workspace_bytes(int64_t R, int64_t B, int64_t V, int64_t K);
+int mi_beam_select(const void *logits, int64_t row_stride, const float *scores,
+                   const uint8_t *finished, int64_t eos, int64_t R, int64_t B, int64_t V,
+                   int64_t K, float *out_scores, int32_t *parents, int32_t *tokens,
+                   uint8_t *out_finished, int dtype, void *workspace, int64_t workspace_bytes,
+                   void *stream);
 
 #ifdef __cplusplus
 }

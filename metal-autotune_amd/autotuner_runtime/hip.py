@@ -25,12 +25,13 @@ import torch
 
 PKG = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("MI_QMM_LIB", PKG / "libmiqmm.so"))
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 MI_OK, MI_ERR_ARG, MI_ERR_UNSUPPORTED, MI_ERR_LAUNCH = 0, 1, 2, 3
 MI_ACT_NONE, MI_ACT_SWIGLU, MI_ACT_GELU = 0, 1, 2
 PAGED_ZERO_BYTES, LOGPROBS_ZERO_BYTES = 262144, 4096  # MI_PAGED_ / MI_LOGPROBS_ZERO_BYTES
+BEAM_ZERO_BYTES = 18432  # MI_BEAM_ZERO_BYTES
 
 _DT = {torch.float32: MI_F32, torch.float16: MI_F16, torch.bfloat16: MI_BF16}
 
@@ -85,13 +86,17 @@ SIGNATURES: dict[str, list] = {
     "mi_paged_attention_workspace_bytes": [_I64] * 8,
     "mi_token_logprobs_workspace_bytes": [_I64, _I64, _I, _I],
     "mi_token_logprobs": [_P, _I64, _I64, _I64, _P, _I, _I, _P, _P, _P, _P, _I, _P, _I64, _P],
+    "mi_beam_select_workspace_bytes": [_I64] * 4,
+    "mi_beam_select": [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64,
+                       _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
             "mi_gelu_mlp_f32_workspace_bytes": ctypes.c_int64,
             "mi_qmm_workspace_bytes": ctypes.c_int64,
             "mi_sdpa_workspace_bytes": ctypes.c_int64,
             "mi_paged_attention_workspace_bytes": ctypes.c_int64,
-            "mi_token_logprobs_workspace_bytes": ctypes.c_int64}
+            "mi_token_logprobs_workspace_bytes": ctypes.c_int64,
+            "mi_beam_select_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -482,6 +487,27 @@ def token_logprobs(x, tokens, wide: bool, top: int, logprobs, entropy, ids, top_
                                    dt, ws, nbytes, stream), "token_logprobs")
 
 
+@functools.lru_cache(maxsize=1024)
+def _beam_workspace_bytes(R, B, V, K) -> int:
+    """mi_beam_select_workspace_bytes, a function of these numbers alone."""
+    return int(lib().mi_beam_select_workspace_bytes(R, B, V, K))
+
+
+def beam_select(x, scores, finished, eos: int, K: int, out_scores, parents, tokens,
+                out_finished) -> None:
+    """mi_beam_select over checked tensors."""
+    R, B = scores.shape
+    V = x.shape[1]
+    dt, stream = _dt(x), _stream(x)
+    nbytes = _beam_workspace_bytes(R, B, V, K)
+    ws = _workspace("beam", x.device, stream, nbytes, 1 << 20,
+                    zero=BEAM_ZERO_BYTES).data_ptr() if nbytes else None
+    _check(lib().mi_beam_select(x.data_ptr(), x.stride(0), scores.data_ptr(), _ptr(finished), eos,
+                                R, B, V, K, out_scores.data_ptr(), parents.data_ptr(),
+                                tokens.data_ptr(), out_finished.data_ptr(), dt, ws, nbytes,
+                                stream), "beam_select")
+
+
 def b_swiglu(ins, outs, p):
     g, u = ins
     (y,) = outs
@@ -526,8 +552,8 @@ def b_linear_f32(ins, outs, p):
 
 # Workspaces: scratch of the entries that make several launches or sum across
 # workgroups (the K-part sums of the _ws qmm entries, the split decode's partial
-# states, the tickets and partial results of mi_gelu_mlp_f32, mi_paged_attention
-# and mi_token_logprobs). Only the tickets need a zero fill when made (every call
+# states, the tickets and partial results of mi_gelu_mlp_f32, mi_paged_attention,
+# mi_token_logprobs and mi_beam_select). Only the tickets need a zero fill when made (every call
 # leaves them zero).
 #
 # Eager calls share one workspace per (thread, kind, device, stream): one

@@ -533,5 +533,55 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     return out
 
 
+# -- several continuations of a prompt (no counterpart in the reference) ----------
+
+class BeamStep(NamedTuple):
+    """``beam_select``'s choice, [R, width] each, the best first."""
+
+    scores: torch.Tensor    # fp32; -inf where there were fewer candidates
+    parents: torch.Tensor   # int32: the row of the logits that each continues
+    tokens: torch.Tensor    # int32: the token that it continues with
+    finished: torch.Tensor  # bool
+
+
+def beam_select(logits, scores, width: int | None = None, finished=None,
+                eos: int | None = None) -> BeamStep:
+    """Beam search's choice: of R prompts of B beams each the ``width`` (default B, 1 to
+    64) best continuations over beams and vocabulary. logits [R * B, V], beam after beam
+    of prompt after prompt; scores fp32 [R, B], to which the candidates' log probabilities
+    are added (-inf: a beam that offers nothing, as all but one are at the first step).
+    finished [R, B] (bool): beams that have ended offer themselves alone, with the token
+    ``eos`` at their own score. The best first; among equal ones the lowest beam, then the
+    lowest token. Candidates of different beams are compared in 64 bits. Where there are
+    fewer than ``width``, the rest has score -inf, the prompt's first beam and token 0."""
+    if not logits.is_cuda:
+        hip._require_gpu(logits)
+    dev = logits.get_device()
+    if scores.dim() != 2 or scores.dtype is not _F32 or scores.get_device() != dev \
+            or not scores.is_contiguous():
+        raise ValueError(f"beam_select: scores must be a contiguous float32 [prompts, beams] on "
+                         f"{logits.device}, got {scores.dtype} {tuple(scores.shape)}")
+    R, B = scores.shape
+    if logits.dim() != 2 or logits.shape[0] != R * B:
+        raise ValueError(f"beam_select: logits must be [{R * B}, V], got {tuple(logits.shape)}")
+    if finished is not None:
+        if finished.shape != scores.shape or finished.dtype is not torch.bool \
+                or finished.get_device() != dev or not finished.is_contiguous():
+            raise ValueError(f"beam_select: finished must be a contiguous bool {(R, B)} on "
+                             f"{logits.device}")
+        if eos is None:
+            raise ValueError("beam_select: finished beams need the token eos")
+    K = B if width is None else int(width)
+    if K < 1:
+        raise ValueError(f"beam_select: width={K}")
+    x = logits if logits.stride(1) == 1 and logits.stride(0) >= 0 else logits.contiguous()
+    ids = torch.empty((2, R, K), dtype=_I32, device=x.device)
+    out = BeamStep(scores.new_empty((R, K)), ids[0], ids[1],
+                   torch.empty((R, K), dtype=torch.bool, device=x.device))
+    with _on(dev):
+        hip.beam_select(x, scores, finished, -1 if eos is None else eos, K, *out)
+    return out
+
+
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)

@@ -23,8 +23,8 @@
 // 2.8e-4): they are bound by these products (8192 tokens 526 -> 694 us with it, four
 // prompts of 2048 161 -> 203).
 //
-// The tile, the softmax and the folds are the contiguous attention's
-// (mi_attn_common.h). A kv head's query rows, token after token and in a token
+// The tile, the softmax and the folds are the contiguous attention's (mi_attn_common.h,
+// mi_paged_common.h). A kv head's query rows, token after token and in a token
 // its G q heads, are the columns of 32-wide blocks, so K and V are read once per
 // block and kv head and a block sees nearly one causal range.
 //
@@ -37,12 +37,10 @@
 // depends on the lengths of the whole batch.
 #include <type_traits>
 
-#include "mi_attn_common.h"
+#include "mi_paged_common.h"
 
 namespace mi {
 namespace {
-
-constexpr int PA_WAVES = ATT_STREAMS;
 
 // The work of one workgroup beside its kv head.
 struct PagedItem {
@@ -71,13 +69,9 @@ struct PagedArgs {
     uint32_t flip;  // sign bits of a negative scale, for Q
 };
 
-constexpr int CHUNK_KEYS = ATT_KT * PA_WAVES;  // keys are cut in multiples of this
-constexpr int MAX_CHUNKS = 128;  // of a block: one workgroup adds them
-
 // One request a lane: its first token, tokens, keys, column blocks (wide: of
 // WIDE_COLS columns) and CHUNK_KEYS runs of keys. (Offsets and lengths are held
 // to the rows and the table that there are.)
-constexpr int WIDE_COLS = 128;
 struct Req {
     int q0, n, len, wide, narrow, runs;
     int falls;  // whether it ends before it starts
@@ -235,36 +229,6 @@ __device__ __forceinline__ PagedItem find_item(const PagedArgs &a, int u, int la
     return it;
 }
 
-#if defined(__HIP_DEVICE_COMPILE__)
-// The DMA of one key tile of K or V: rows [0, left) of it (at most 32) lie at
-// lo (rows 0..15) and hi (rows 16..31, its own 16 rows); the rest arrive as zeros.
-// NT: non-temporal, for what is read once (decode: 48 requests of 64 to 8191 keys
-// 152 -> 136 us; wide blocks, which share keys through the L2, 97 -> 105 with it).
-template <typename T, int D, bool ISV, bool NT>
-__device__ __forceinline__ void dma_paged_tile(const T *lo, const T *hi, int left, char *dst,
-                                               int lane) {
-    typedef Tile<D> Tl;
-    const int n0 = left < 0 ? 0 : (left < 16 ? left : 16);
-    const int n1 = left < 16 ? 0 : (left < 32 ? left - 16 : 16);
-    const __amdgpu_buffer_rsrc_t r0 = att_rsrc(lo, (uint32_t)(n0 * D * 2));
-    const __amdgpu_buffer_rsrc_t r1 = att_rsrc(hi, (uint32_t)(n1 * D * 2));
-#pragma unroll
-    for (int i = 0; i < Tl::NI; ++i) {
-        const int row = i * Tl::RPI + lane / Tl::CPR, pos = lane % Tl::CPR;
-        const int c = pos ^ (ISV ? swz_v<D>(row) : swz_k<D>(row));
-        const bool second = i * Tl::RPI >= 16;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(second ? r1 : r0, (lds_ptr)(dst + i * 1024), 16,
-                                                 ((row & 15) * D + 8 * c) * 2, 0, 0, NT ? 2 : 0);
-    }
-}
-#endif
-
-template <int D> struct PagedLds {
-    static constexpr int SLOTS = PA_WAVES * 2 * Tile<D>::BYTES;  // = two wide stages
-    static constexpr int FOLD = PA_WAVES * Part<D>::BYTES;
-    static constexpr int BYTES = SLOTS > FOLD ? SLOTS : FOLD;
-};
-
 // A chunk's state in the workspace, of 32 columns, in whole lines of a wave's
 // stores (written past the caches, pieces of a line cost a line each): a narrow
 // block's is columns of D sums, then of (l, m); a wide one's is the registers' pairs
@@ -343,42 +307,6 @@ __device__ __forceinline__ void join_narrow(const PagedArgs &a, const PagedItem 
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// The pages of a wave's next 64 tiles kt, kt + STEP, ..., one a lane (a tile of
-// 16-row pages has two), and a tile's first and second 16 rows of the kv head in
-// the pools.
-template <int STEP> struct TilePages {
-    const int *row;
-    int64_t hk;
-    int W, pages, lp, HK;
-    int id0, id1;
-    __device__ __forceinline__ TilePages(const PagedArgs &a, int r, int hk_)
-        : row(a.table + (int64_t)r * a.W), hk(hk_), W(a.W), pages(a.pages), lp(a.page_log2),
-          HK(a.HK), id0(0), id1(0) {}
-    __device__ __forceinline__ void load(int kt, int lane) {
-        const int key = (kt + STEP * lane) * ATT_KT;
-        id0 = min(max(row[min(key >> lp, W - 1)], 0), pages - 1);
-        id1 = min(max(row[min((key + 16) >> lp, W - 1)], 0), pages - 1);
-    }
-    // the tile `at` steps (mod 64) behind the loaded one, of first key `key`
-    __device__ __forceinline__ void rows(int at, int key, int64_t &lo, int64_t &hi) const {
-        const int64_t mask = ((int64_t)1 << lp) - 1;
-        lo = (((int64_t)__builtin_amdgcn_readlane(id0, at & 63) * HK + hk) << lp) + (key & mask);
-        hi = (((int64_t)__builtin_amdgcn_readlane(id1, at & 63) * HK + hk) << lp) +
-             ((key + 16) & mask);
-    }
-};
-
-// Whether a wave's sums have a NaN (or infinities of both signs).
-template <int D> __device__ __forceinline__ bool not_a_number(const AttnState<D> &st) {
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i & 3] += st.o[t][i];
-    const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    return __builtin_amdgcn_ballot_w64(all != all) != 0;
-}
-
 // A narrow block: wave w takes the key tiles w, w + 4, ... of the chunk into LDS of
 // its own (a K and a V slot, refilled as soon as their reads are in registers: no
 // barrier), and the four states are folded at the end. Bound by HBM: K and V are
@@ -506,45 +434,6 @@ __device__ __forceinline__ void narrow_block(const PagedArgs &a, const PagedItem
         put_part((float2 *)(o + 32 * D) + threadIdx.x,
                  *(float2 *)(cols_at + 32 * D + 2 * threadIdx.x));
     join_narrow<T, D>(a, it, hk, have, lds);
-}
-
-// attn_softmax over two key tiles.
-template <typename T, int D>
-__device__ __forceinline__ void softmax_pair(AttnState<D> &st, const f32x16 (&s)[2],
-                                             uint32_t (&pk)[2][8], float scale) {
-#pragma clang fp contract(off)
-    float mt[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        mt[j] = fmaxf(s[j][0], s[j][1]);
-#pragma unroll
-        for (int i = 2; i < 16; i += 2) mt[j] = fmaxf(fmaxf(mt[j], s[j][i]), s[j][i + 1]);
-    }
-    const float m = max_halves(fmaxf(mt[0], mt[1])) * scale;
-    const bool grow = m > st.m + 8.0f;
-    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-        const float m_new = grow ? m : st.m;
-        const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - m_new);
-        st.l *= corr;
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[t][i] *= corr;
-        st.m = m_new;
-    }
-    const float nm = st.m == -INFINITY ? 0.0f : -st.m;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][2 * i], scale, nm));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][2 * i + 1], scale, nm));
-            pk[j][i] = pk2<T>(p0, p1);
-            sum[2 * (i & 1)] += p0;
-            sum[2 * (i & 1) + 1] += p1;
-        }
-    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // A wide block: wave w has the columns 32 w .. 32 w + 31 of the block's 128, and
@@ -821,12 +710,6 @@ int launch_paged_w(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
 template <typename T, int D>
 int launch_paged(const PagedArgs &a, const PagedGrid &g, hipStream_t st) {
     return g.wide ? launch_paged_w<T, D, true>(a, g, st) : launch_paged_w<T, D, false>(a, g, st);
-}
-
-bool page_log2_of(int64_t page, int &lp) {
-    for (lp = 4; lp <= 8; ++lp)
-        if (page == (1 << lp)) return true;
-    return false;
 }
 
 }  // namespace
