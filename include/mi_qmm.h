@@ -41,7 +41,8 @@ extern "C" {
                              6: mi_qmm_affine_qkv_norm_rope; 7: mi_sdpa_ws;
                              8: the paged cache entries, mi_token_logprobs;
                              9: mi_stream_capture_id;
-                             10: mi_beam_select */
+                             10: mi_beam_select, mi_paged_fork,
+                                 mi_paged_compact */
 
 enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 };
 
@@ -435,6 +436,44 @@ int mi_beam_select(const void *logits, int64_t row_stride, const float *scores,
                    int64_t K, float *out_scores, int32_t *parents, int32_t *tokens,
                    uint8_t *out_finished, int dtype, void *workspace, int64_t workspace_bytes,
                    void *stream);
+
+/* Pages of the cache above forked, copied, given back and compacted, in all layers at
+ * once: pools is a device array of n_pools base addresses (16-byte aligned), each of a
+ * pool of n_pages pages of Hkv heads of page_size rows of row_bytes (a multiple of 16).
+ * A page is in use if a live entry of the table names it (the first
+ * ceil(kv_lens[r] / page_size) of row r; ids outside the pool count for nothing). R <=
+ * 4096, table_width <= 131072, n_pages <= 2^20, n_free >= n_pages.
+ *
+ * mi_paged_fork: request r goes on from the keys of request sources[r] (itself, too);
+ * sources[r] < 0 ends it (kv_lens[r] = 0). Full pages are then shared. A part-filled last
+ * page stays with one request of those that go on from its owner (the owner itself, else
+ * the lowest); every other takes a page from the end of free_pages[0, *free_count), in
+ * the order of requests, and a copy of its rows. Pages that are not in use afterwards are
+ * put behind the free ones before that, in the order of their ids. Table, lengths, free
+ * list and pools are changed in place; entries of a row behind its live ones stay. If
+ * pages are missing, or a source is R or more, nothing changes and *refused is their
+ * number (else 0). A part-filled page must have one owner before the call, as it has after.
+ *
+ * mi_paged_compact: the pages in use move to the lowest ids, those past their number *live
+ * into the free ids below it, both in order, and the table follows; every other page is
+ * free afterwards: *free_count = n_pages - *live, the lowest at the end of free_pages.
+ *
+ * workspace: mi_paged_fork_workspace_bytes / mi_paged_compact_workspace_bytes, 16-byte
+ * aligned, whose first MI_PAGES_ZERO_BYTES (a fixed prefix) are zero before its first use;
+ * every call leaves them zero. Calls sharing one must not overlap. */
+#define MI_PAGES_ZERO_BYTES 262208
+int64_t mi_paged_fork_workspace_bytes(int64_t R, int64_t table_width);
+int mi_paged_fork(int32_t *block_table, int64_t table_width, int32_t *kv_lens,
+                  const int32_t *sources, int64_t R, int32_t *free_pages, int64_t n_free,
+                  int32_t *free_count, int32_t *refused, void *const *pools, int64_t n_pools,
+                  int64_t n_pages, int64_t Hkv, int64_t page_size, int64_t row_bytes,
+                  void *workspace, int64_t workspace_bytes, void *stream);
+int64_t mi_paged_compact_workspace_bytes(int64_t n_pages);
+int mi_paged_compact(int32_t *block_table, int64_t table_width, const int32_t *kv_lens, int64_t R,
+                     int32_t *free_pages, int64_t n_free, int32_t *free_count, int32_t *live,
+                     void *const *pools, int64_t n_pools, int64_t n_pages, int64_t Hkv,
+                     int64_t page_size, int64_t row_bytes, void *workspace,
+                     int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

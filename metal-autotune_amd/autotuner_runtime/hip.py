@@ -31,7 +31,7 @@ MI_F32, MI_F16, MI_BF16 = 0, 1, 2
 MI_OK, MI_ERR_ARG, MI_ERR_UNSUPPORTED, MI_ERR_LAUNCH = 0, 1, 2, 3
 MI_ACT_NONE, MI_ACT_SWIGLU, MI_ACT_GELU = 0, 1, 2
 PAGED_ZERO_BYTES, LOGPROBS_ZERO_BYTES = 262144, 4096  # MI_PAGED_ / MI_LOGPROBS_ZERO_BYTES
-BEAM_ZERO_BYTES = 18432  # MI_BEAM_ZERO_BYTES
+BEAM_ZERO_BYTES, PAGES_ZERO_BYTES = 18432, 262208  # MI_BEAM_ / MI_PAGES_ZERO_BYTES
 
 _DT = {torch.float32: MI_F32, torch.float16: MI_F16, torch.bfloat16: MI_BF16}
 
@@ -89,6 +89,12 @@ SIGNATURES: dict[str, list] = {
     "mi_beam_select_workspace_bytes": [_I64] * 4,
     "mi_beam_select": [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64,
                        _P],
+    "mi_paged_fork_workspace_bytes": [_I64, _I64],
+    "mi_paged_fork": [_P, _I64, _P, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P,
+                      _I64, _P],
+    "mi_paged_compact_workspace_bytes": [_I64],
+    "mi_paged_compact": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P,
+                         _I64, _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
             "mi_gelu_mlp_f32_workspace_bytes": ctypes.c_int64,
@@ -96,7 +102,9 @@ RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctype
             "mi_sdpa_workspace_bytes": ctypes.c_int64,
             "mi_paged_attention_workspace_bytes": ctypes.c_int64,
             "mi_token_logprobs_workspace_bytes": ctypes.c_int64,
-            "mi_beam_select_workspace_bytes": ctypes.c_int64}
+            "mi_beam_select_workspace_bytes": ctypes.c_int64,
+            "mi_paged_fork_workspace_bytes": ctypes.c_int64,
+            "mi_paged_compact_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -508,6 +516,33 @@ def beam_select(x, scores, finished, eos: int, K: int, out_scores, parents, toke
                                 stream), "beam_select")
 
 
+def paged_fork(table, kv_lens, sources, free_pages, free_count, refused, pools) -> None:
+    """mi_paged_fork over checked arrays; pools: an ops.PagePools."""
+    R, W = table.shape
+    n_pages, HK, page, row = pools.shape
+    stream = _stream(table)
+    nbytes = int(lib().mi_paged_fork_workspace_bytes(R, W))
+    ws = _workspace("pages", table.device, stream, nbytes, 1 << 20, zero=PAGES_ZERO_BYTES)
+    _check(lib().mi_paged_fork(table.data_ptr(), W, kv_lens.data_ptr(), sources.data_ptr(), R,
+                               free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+                               refused.data_ptr(), pools.pointers.data_ptr(), len(pools.pools),
+                               n_pages, HK, page, row, ws.data_ptr(), ws.numel(), stream),
+           "paged_fork")
+
+
+def paged_compact(table, kv_lens, free_pages, free_count, live, pools) -> None:
+    """mi_paged_compact over checked arrays; pools: an ops.PagePools."""
+    R, W = table.shape
+    n_pages, HK, page, row = pools.shape
+    stream = _stream(table)
+    nbytes = int(lib().mi_paged_compact_workspace_bytes(n_pages))
+    ws = _workspace("pages", table.device, stream, nbytes, 1 << 20, zero=PAGES_ZERO_BYTES)
+    _check(lib().mi_paged_compact(table.data_ptr(), W, kv_lens.data_ptr(), R, free_pages.data_ptr(),
+                                  free_pages.shape[0], free_count.data_ptr(), live.data_ptr(),
+                                  pools.pointers.data_ptr(), len(pools.pools), n_pages, HK, page,
+                                  row, ws.data_ptr(), ws.numel(), stream), "paged_compact")
+
+
 def b_swiglu(ins, outs, p):
     g, u = ins
     (y,) = outs
@@ -553,7 +588,8 @@ def b_linear_f32(ins, outs, p):
 # Workspaces: scratch of the entries that make several launches or sum across
 # workgroups (the K-part sums of the _ws qmm entries, the split decode's partial
 # states, the tickets and partial results of mi_gelu_mlp_f32, mi_paged_attention,
-# mi_token_logprobs and mi_beam_select). Only the tickets need a zero fill when made (every call
+# mi_token_logprobs, mi_beam_select and the paged fork and compaction, whose bitmaps
+# count as such). Only the tickets need a zero fill when made (every call
 # leaves them zero).
 #
 # Eager calls share one workspace per (thread, kind, device, stream): one

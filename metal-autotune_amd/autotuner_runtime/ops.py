@@ -583,5 +583,79 @@ def beam_select(logits, scores, width: int | None = None, finished=None,
     return out
 
 
+class PagePools(NamedTuple):
+    """The pools of all layers as ``paged_fork`` and ``paged_compact`` take them
+    (``page_pools``)."""
+
+    pointers: torch.Tensor  # int64, on the device: where each begins
+    pools: tuple            # the pools, kept alive
+    shape: tuple            # (pages, heads, page size, bytes of a row)
+
+
+def page_pools(pools) -> PagePools:
+    """Pools [pages, heads, page size, head dim] of one shape and type on one device
+    (every layer's k_pages and v_pages), made once and kept: whatever pages a fork or a
+    compaction moves, it moves in all of them."""
+    pools = tuple(pools)
+    if not pools:
+        raise ValueError("page_pools: no pools")
+    first = pools[0]
+    if not first.is_cuda:
+        hip._require_gpu(first)
+    for p in pools:
+        if p.dim() != 4 or p.shape != first.shape or p.dtype is not first.dtype \
+                or p.get_device() != first.get_device() or not p.is_contiguous() \
+                or p.data_ptr() & 15:
+            raise ValueError(f"page_pools: the pools must be contiguous, 16-byte aligned "
+                             f"{first.dtype} {tuple(first.shape)} on {first.device}, got {p.dtype} "
+                             f"{tuple(p.shape)} on {p.device}")
+    n, heads, page, D = first.shape
+    pointers = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(first.device)
+    return PagePools(pointers, pools, (n, heads, page, D * first.element_size()))
+
+
+def _check_pages(what: str, pools: PagePools, block_table, kv_lens, free_pages, free_count,
+                 *more) -> int:
+    dev = pools.pointers.get_device()
+    if block_table.dim() != 2 or kv_lens.shape != block_table.shape[:1] or free_pages.dim() != 1 \
+            or free_count.numel() != 1 or any(t.shape != kv_lens.shape for t in more):
+        raise ValueError(f"{what} takes block_table [R, width], an entry of [R] a request, "
+                         "free_pages [F] and free_count [1]")
+    _i32(what, dev, block_table, kv_lens, free_pages, free_count, *more)
+    if not block_table.shape[0]:
+        raise ValueError(f"{what}: no requests")
+    return dev
+
+
+def paged_fork(block_table, kv_lens, sources, free_pages, free_count,
+               pools: PagePools) -> torch.Tensor:
+    """Requests that go on from others' keys: request r continues request sources[r]
+    (int32 [R]; itself, too), or ends where that is negative. Full pages are shared from
+    then on, a part-filled last one stays with one of those that go on from it and is
+    copied for the others, in every layer's pools; pages that nobody holds any more go
+    back to the free list first (in the order of their ids), and the copies' pages come
+    from its end. block_table, kv_lens, free_pages (of as many entries as there are pages)
+    and free_count are changed in place. Returns int32 [1]: 0, or how many pages were
+    missing (sources past the last request count as such); then nothing has changed.
+    Shared pages are full: the next step's tokens never fall into them."""
+    dev = _check_pages("paged_fork", pools, block_table, kv_lens, free_pages, free_count, sources)
+    refused = kv_lens.new_empty(1)
+    with _on(dev):
+        hip.paged_fork(block_table, kv_lens, sources, free_pages, free_count, refused, pools)
+    return refused
+
+
+def paged_compact(block_table, kv_lens, free_pages, free_count, pools: PagePools) -> torch.Tensor:
+    """The pages that requests hold moved to the lowest ids, in every layer's pools, so
+    that the rest of the pools can go: block_table, free_pages (of as many entries as
+    there are pages) and free_count are changed in place; every page that no request
+    holds is free afterwards. Returns int32 [1]: how many are held."""
+    dev = _check_pages("paged_compact", pools, block_table, kv_lens, free_pages, free_count)
+    live = kv_lens.new_empty(1)
+    with _on(dev):
+        hip.paged_compact(block_table, kv_lens, free_pages, free_count, live, pools)
+    return live
+
+
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
