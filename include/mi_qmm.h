@@ -42,7 +42,7 @@ extern "C" {
                              8: the paged cache entries, mi_token_logprobs;
                              9: mi_stream_capture_id;
                              10: mi_beam_select, mi_paged_fork,
-                                 mi_paged_compact */
+                                 mi_paged_compact, mi_paged_shared_* */
 
 enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 };
 
@@ -474,6 +474,39 @@ int mi_paged_compact(int32_t *block_table, int64_t table_width, const int32_t *k
                      void *const *pools, int64_t n_pools, int64_t n_pages, int64_t Hkv,
                      int64_t page_size, int64_t row_bytes, void *workspace,
                      int64_t workspace_bytes, void *stream);
+
+/* Causal attention of requests that share prefixes, whose keys and values are read once a
+ * group. The plan is made once a step, for the attention of every layer: group g is the
+ * requests [cu_groups[g], cu_groups[g + 1]) (int32 [n_groups + 1]; requests outside all
+ * groups are by themselves). keys[g] (int32 [n_groups], written) is the number of leading
+ * keys, of whole pages and cached before the step, that all of its requests with tokens and
+ * keys hold in the same pages; 0 where there is no such request. schedule: device memory
+ * of mi_paged_shared_plan_ints(...) int32 (16-byte aligned), opaque, for
+ * mi_paged_shared_attention over the same table, lengths and sizes. cu_q, kv_lens as
+ * there; offsets (of either kind) that fall make a plan without work. 1 <= R <= 4096,
+ * n_groups <= R, T <= 2^18.
+ *
+ * mi_paged_shared_attention: mi_paged_attention's result for the step that the plan was
+ * made for, within rounding: the same sums in another order, which depends on all requests'
+ * lengths and groups, deterministic for them. A schedule of other sizes leaves out as it
+ * was. workspace: mi_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no
+ * initialization needed. Calls sharing one must not overlap. */
+int64_t mi_paged_shared_plan_ints(int64_t T, int64_t R, int64_t n_groups, int64_t table_width,
+                                  int64_t H, int64_t HK, int64_t D, int64_t page_size);
+int mi_paged_shared_plan(const int32_t *block_table, int64_t table_width, const int32_t *cu_q,
+                         const int32_t *kv_lens, int64_t R, const int32_t *cu_groups,
+                         int64_t n_groups, int64_t T, int64_t H, int64_t HK, int64_t D,
+                         int64_t page_size, int32_t *keys, int32_t *schedule,
+                         int64_t schedule_ints, void *stream);
+int64_t mi_paged_shared_attention_workspace_bytes(int64_t T, int64_t R, int64_t n_groups,
+                                                  int64_t table_width, int64_t H, int64_t HK,
+                                                  int64_t D, int64_t page_size);
+int mi_paged_shared_attention(const void *q, const void *k_pages, const void *v_pages, void *out,
+                              const int32_t *block_table, const int32_t *schedule, int64_t T,
+                              int64_t R, int64_t n_groups, int64_t table_width, int64_t H,
+                              int64_t HK, int64_t D, int64_t n_pages, int64_t page_size,
+                              float scale, int dtype, void *workspace, int64_t workspace_bytes,
+                              void *stream);
 
 #ifdef __cplusplus
 }

@@ -95,6 +95,12 @@ SIGNATURES: dict[str, list] = {
     "mi_paged_compact_workspace_bytes": [_I64],
     "mi_paged_compact": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P,
                          _I64, _P],
+    "mi_paged_shared_plan_ints": [_I64] * 8,
+    "mi_paged_shared_plan": [_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
+                             _I64, _P],
+    "mi_paged_shared_attention_workspace_bytes": [_I64] * 8,
+    "mi_paged_shared_attention": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                  _I64, _I64, _F, _I, _P, _I64, _P],
 }
 RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctypes.c_int64,
             "mi_gelu_mlp_f32_workspace_bytes": ctypes.c_int64,
@@ -104,7 +110,9 @@ RESTYPES = {"mi_last_error": ctypes.c_char_p, "mi_argmax_workspace_bytes": ctype
             "mi_token_logprobs_workspace_bytes": ctypes.c_int64,
             "mi_beam_select_workspace_bytes": ctypes.c_int64,
             "mi_paged_fork_workspace_bytes": ctypes.c_int64,
-            "mi_paged_compact_workspace_bytes": ctypes.c_int64}
+            "mi_paged_compact_workspace_bytes": ctypes.c_int64,
+            "mi_paged_shared_plan_ints": ctypes.c_int64,
+            "mi_paged_shared_attention_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None
@@ -541,6 +549,44 @@ def paged_compact(table, kv_lens, free_pages, free_count, live, pools) -> None:
                                   free_pages.shape[0], free_count.data_ptr(), live.data_ptr(),
                                   pools.pointers.data_ptr(), len(pools.pools), n_pages, HK, page,
                                   row, ws.data_ptr(), ws.numel(), stream), "paged_compact")
+
+
+@functools.lru_cache(maxsize=1024)
+def shared_plan_ints(T, R, groups, W, H, HK, D, page) -> int:
+    """mi_paged_shared_plan_ints, a function of these numbers alone (ValueError where
+    they are refused)."""
+    n = int(lib().mi_paged_shared_plan_ints(T, R, groups, W, H, HK, D, page))
+    if n == 0:
+        raise ValueError(f"paged_shared_plan: {lib().mi_last_error().decode(errors='replace')}")
+    return n
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_workspace_bytes(T, R, groups, W, H, HK, D, page) -> int:
+    """mi_paged_shared_attention_workspace_bytes, a function of these numbers alone."""
+    return int(lib().mi_paged_shared_attention_workspace_bytes(T, R, groups, W, H, HK, D, page))
+
+
+def paged_shared_plan(table, cu_q, kv_lens, cu_groups, plan) -> None:
+    """mi_paged_shared_plan over checked arrays into an ops.SharedPlan."""
+    T, R, groups, W, H, HK, D, page = plan.shape
+    _check(lib().mi_paged_shared_plan(table.data_ptr(), W, cu_q.data_ptr(), kv_lens.data_ptr(), R,
+                                      cu_groups.data_ptr(), groups, T, H, HK, D, page,
+                                      plan.keys.data_ptr(), plan.schedule.data_ptr(),
+                                      plan.schedule.shape[0], _stream(table)), "paged_shared_plan")
+
+
+def paged_shared_attention(q, k_pages, v_pages, out, table, plan, scale: float) -> None:
+    """mi_paged_shared_attention over checked tensors, with the parts' workspace."""
+    T, R, groups, W, H, HK, D, page = plan.shape
+    stream = _stream(q)
+    nbytes = _shared_workspace_bytes(*plan.shape)
+    ws = _workspace("shared", q.device, stream, nbytes, 4 << 20).data_ptr() if nbytes else None
+    _check(lib().mi_paged_shared_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                           out.data_ptr(), table.data_ptr(),
+                                           plan.schedule.data_ptr(), T, R, groups, W, H, HK, D,
+                                           k_pages.shape[0], page, scale, _dt(q), ws, nbytes,
+                                           stream), "paged_shared_attention")
 
 
 def b_swiglu(ins, outs, p):

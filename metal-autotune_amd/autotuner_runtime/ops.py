@@ -657,5 +657,71 @@ def paged_compact(block_table, kv_lens, free_pages, free_count, pools: PagePools
     return live
 
 
+class SharedPlan(NamedTuple):
+    """A step's plan of attention behind shared prefixes (``paged_shared_plan``)."""
+
+    keys: torch.Tensor      # int32 [groups]: the leading keys that all of a group hold alike
+    schedule: torch.Tensor  # the work, for ``paged_shared_attention``
+    shape: tuple            # (T, R, groups, width, H, HK, D, page size): what it is for
+
+
+def paged_shared_plan(block_table, cu_q, kv_lens, cu_groups, page_size: int, num_tokens: int,
+                      n_heads: int, n_kv_heads: int, head_dim: int,
+                      out: SharedPlan | None = None) -> SharedPlan:
+    """What groups of requests share, and a step's attention laid out for it, once for all
+    layers: group g is the requests [cu_groups[g], cu_groups[g + 1]) (int32 [groups + 1];
+    requests outside all groups are by themselves), whose common leading keys are found
+    from block_table's rows: whole pages, cached before the step, that all of the group's
+    requests hold. block_table, cu_q, kv_lens: a step's, as ``paged_attention`` takes them
+    (``paged_plan`` makes them), of num_tokens rows. out: an earlier plan of these sizes,
+    written again (a captured graph reads it where it is)."""
+    R, = kv_lens.shape
+    if block_table.dim() != 2 or block_table.shape[0] != R or cu_q.shape != (R + 1,) \
+            or cu_groups.dim() != 1 or cu_groups.shape[0] < 2:
+        raise ValueError("paged_shared_plan takes block_table [R, width], cu_q [R + 1], kv_lens [R] "
+                         "and cu_groups [groups + 1]")
+    dev = block_table.get_device()
+    _i32("paged_shared_plan", dev, block_table, cu_q, kv_lens, cu_groups)
+    if not block_table.is_cuda:
+        hip._require_gpu(block_table)
+    shape = (int(num_tokens), R, cu_groups.shape[0] - 1, block_table.shape[1], int(n_heads),
+             int(n_kv_heads), int(head_dim), int(page_size))
+    if out is None:
+        n = hip.shared_plan_ints(*shape)
+        buf = block_table.new_empty(n + shape[2])
+        out = SharedPlan(buf[n:], buf[:n], shape)
+    elif out.shape != shape or out.schedule.get_device() != dev:
+        raise ValueError(f"paged_shared_plan: out is a plan for {out.shape}, not {shape}")
+    with _on(dev):
+        hip.paged_shared_plan(block_table, cu_q, kv_lens, cu_groups, out)
+    return out
+
+
+def paged_shared_attention(q, k_pages, v_pages, block_table, plan: SharedPlan,
+                           scale: float) -> torch.Tensor:
+    """``paged_attention`` of the step that ``plan`` was made for, with the keys that a
+    group's requests share read once for all of them: q [T, H, D] -> [T, H, D]. The same
+    results within rounding. block_table: the plan's. Rows behind the last request's are
+    not written."""
+    T, R, _, width, H, HK, D, page = plan.shape
+    if q.shape != (T, H, D):
+        raise ValueError(f"paged_shared_attention: the plan is for q {(T, H, D)}, got "
+                         f"{tuple(q.shape)}")
+    _, hk, rows, _ = _paged_pools("paged_shared_attention", q, k_pages, v_pages, D)
+    if hk != HK or rows != page or block_table.shape != (R, width):
+        raise ValueError(f"paged_shared_attention: the plan is for pages of {HK} heads of {page} rows "
+                         f"and a table {(R, width)}")
+    dev = q.get_device()
+    _i32("paged_shared_attention", dev, block_table, plan.schedule)
+    if not q.is_cuda:
+        hip._require_gpu(q)
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_like(q)
+    with _on(dev):
+        hip.paged_shared_attention(q, k_pages, v_pages, out, block_table, plan, scale)
+    return out
+
+
 def default_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)

@@ -43,7 +43,7 @@ FLAGS = [
 # loop's VALU), which also cost occupancy. Same instructions otherwise, same
 # results.
 SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-                for name in ("mi_attn.hip", "mi_paged_attn.hip")}
+                for name in ("mi_attn.hip", "mi_paged_attn.hip", "mi_shared_attn.hip")}
 
 
 def _run(cmd: list[str]) -> None:
