@@ -31,10 +31,11 @@ instead of normalizing its input again (one launch fewer per layer, same
 bits).
 
 Several requests of different lengths run together over a paged cache
-(``PagedBatch``, ``Qwen3Model.forward_paged``, ``generate_paged``; no counterpart
-in the reference): the layers and their region wrapper are the same, the tokens
-of all requests being the rows of one [1, T, hidden] input; only the attention
-prologue and the attention are the paged ones (``Attention.paged``).
+(``PagedBatch``, ``Qwen3Model.forward_paged``, ``generate_paged``, and
+``generate_beams`` for beam search; no counterpart in the reference): the layers and
+their region wrapper are the same, the tokens of all requests being the rows of one
+[1, T, hidden] input; only the attention prologue and the attention are the paged ones
+(``Attention.paged``).
 
 Only the last position's logits are computed in prefill (the caller takes
 logits[:, -1] before sampling; everything before it is dead work,
@@ -45,6 +46,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch import nn
@@ -141,10 +143,16 @@ class PagedBatch:
     missing (they keep what they have, and may bring their tokens again). A plan
     holds until the next one of as many rows, which is written in its place where it
     is one of the last ``KEPT_PLANS`` row counts' or a graph capture made it or read
-    it as ``plan`` (the layers do). ``finish(r)`` gives a request's pages back."""
+    it as ``plan`` (the layers do). ``finish(r)`` gives a request's pages back.
+
+    ``beams`` > 1: every so many requests, from the first, are a group whose prompts are
+    alike (the beams of one, or its samples): ``fork(sources)`` lets requests go on from
+    others' keys, and a step's attention reads the keys that a group shares once (``shared``,
+    its plan). ``compact()`` moves the pages in use to the lowest ids. Every request's
+    part-filled page is its own, so nothing but the cache's entries need know."""
 
     def __init__(self, cfg: "Qwen3Config", n_layers: int, max_requests: int, n_pages: int,
-                 page_size: int, max_len: int, device, dtype=torch.bfloat16):
+                 page_size: int, max_len: int, device, dtype=torch.bfloat16, beams: int = 1):
         def i32(*shape):
             return torch.zeros(shape, dtype=torch.int32, device=device)
 
@@ -155,44 +163,80 @@ class PagedBatch:
         self.free_count = i32(1) + n_pages
         self.inv_freq = ops.rope_table(cfg.head_dim, cfg.rope_theta, device=device)
         self.max_q_len = None
+        self.beams = beams
+        self.cu_groups = None
+        if beams > 1:
+            self.cu_groups = torch.tensor([*range(0, max_requests, beams), max_requests],
+                                          dtype=torch.int32, device=device)
+        self.heads = (cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim)
         # what a captured graph reads beside its tensors: this batch's, at this plan
         self._name = object()
         self.graph_key = (self._name, None)
-        # by token rows; the captured ones are where a graph reads or writes them
-        self._plan, self._plans, self._captured = None, {}, {}
+        # (plan, what groups share or None), by token rows; the captured ones are where a
+        # graph reads or writes them
+        self._plan, self._plans, self._captured = (None, None), {}, {}
         shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
         self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
+        self._pools = None
+        if self.lens.is_cuda:
+            self.pools()
 
     def step(self, q_lens, num_tokens: int, max_q_len: int | None = None) -> ops.PagedPlan:
         """max_q_len: the most tokens a request brings, where the caller knows it."""
+        old, shared = self._captured.get(num_tokens) or self._plans.get(num_tokens) or (None, None)
         p = ops.paged_plan(
             self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
-            self.page_size, num_tokens,
-            out=self._captured.get(num_tokens) or self._plans.get(num_tokens))
+            self.page_size, num_tokens, out=old)
+        if self.cu_groups is not None:
+            shared = ops.paged_shared_plan(self.block_table, p.cu_q, p.kv_lens, self.cu_groups,
+                                           self.page_size, num_tokens, *self.heads, out=shared)
         self._plans.pop(num_tokens, None)
-        self._plans[num_tokens] = p  # the last
+        self._plans[num_tokens] = p, shared  # the last
         if len(self._plans) > KEPT_PLANS:
             del self._plans[next(iter(self._plans))]
         self.lens.copy_(torch.where(p.kv_lens > 0, p.kv_lens, self.lens))
         self.free_count.copy_(p.free_count)
-        self._plan, self.max_q_len = p, max_q_len
+        self._plan, self.max_q_len = (p, shared), max_q_len
         self.graph_key = (self._name, p.cu_q.data_ptr())
         return self.plan
 
     @property
     def plan(self) -> ops.PagedPlan | None:
         """The last step's plan."""
-        p = self._plan
+        p = self._plan[0]
         if p is not None and _capturing(p.slots):
-            self._captured[p.slots.shape[0]] = p
+            self._captured[p.slots.shape[0]] = self._plan
         return p
 
+    @property
+    def shared(self) -> ops.SharedPlan | None:
+        """What groups share in the last step, where there are any."""
+        return self._plan[1] if self.plan is not None else None
+
+    def pools(self) -> ops.PagePools:
+        """The caches' pools, for the operators over all layers' pages."""
+        now = [t for c in self.caches for t in (c.keys, c.values)]
+        if self._pools is None or any(a is not b for a, b in zip(now, self._pools.pools)):
+            self._pools = ops.page_pools(now)
+        return self._pools
+
+    def fork(self, sources) -> torch.Tensor:
+        """Request r goes on from the keys of request sources[r] (int32, on the GPU; one of
+        its own step is as good), or ends where that is negative. Returns int32 [1], the
+        pages that were missing: then nothing has changed."""
+        return ops.paged_fork(self.block_table, self.lens, sources, self.free_pages,
+                              self.free_count, self.pools())
+
+    def compact(self) -> torch.Tensor:
+        """The pages in use moved to the lowest ids; returns int32 [1], their number."""
+        return ops.paged_compact(self.block_table, self.lens, self.free_pages, self.free_count,
+                                 self.pools())
+
     def finish(self, r: int) -> None:
-        n = -(-int(self.lens[r]) // self.page_size)
-        at = int(self.free_count)
-        self.free_pages[at:at + n] = self.block_table[r, :n]
-        self.free_count += n
-        self.lens[r] = 0
+        """The request's pages go back, but for those that others hold too."""
+        sources = torch.arange(self.lens.shape[0], dtype=torch.int32, device=self.lens.device)
+        sources[r] = -1
+        self.fork(sources)
 
 
 class Attention(nn.Module):
@@ -212,8 +256,12 @@ class Attention(nn.Module):
                                  c.num_attention_heads, c.num_key_value_heads, c.rms_norm_eps,
                                  b.inv_freq, plan.positions, plan.slots, cache.keys,
                                  cache.values)
-        o = ops.paged_attention(qr, cache.keys, cache.values, b.block_table, plan.cu_q,
-                                plan.kv_lens, self.scale, b.max_q_len)
+        if b.shared is not None:
+            o = ops.paged_shared_attention(qr, cache.keys, cache.values, b.block_table, b.shared,
+                                           self.scale)
+        else:
+            o = ops.paged_attention(qr, cache.keys, cache.values, b.block_table, plan.cu_q,
+                                    plan.kv_lens, self.scale, b.max_q_len)
         return o.view(1, o.shape[0], -1)
 
     def forward(self, x, cache: KVCache | PagedKVCache):
@@ -289,9 +337,9 @@ class Qwen3Model(nn.Module):
         return self.model.embed_tokens.as_linear(self.model.norm(h))
 
     def make_batch(self, max_requests: int, n_pages: int, page_size: int = 64,
-                   max_len: int = 8192) -> PagedBatch:
+                   max_len: int = 8192, beams: int = 1) -> PagedBatch:
         return PagedBatch(self.cfg, len(self.model.layers), max_requests, n_pages, page_size,
-                          max_len, self.model.norm.weight.device)
+                          max_len, self.model.norm.weight.device, beams=beams)
 
     def forward_paged(self, ids, batch: PagedBatch):
         """The planned step (``batch.step``): ids [T], every request's tokens one
@@ -330,6 +378,58 @@ def generate_paged(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
     if int(refused):
         raise RuntimeError("generate_paged: the batch's pages ran out, or a request's length")
     return torch.stack(tokens), logprobs
+
+
+class Beams(NamedTuple):
+    """``generate_beams``' continuations, the best of each prompt first."""
+
+    sequences: torch.Tensor  # int32 [prompts, beams, n_tokens]; behind an eos, eos
+    scores: torch.Tensor     # fp32 [prompts, beams]: their summed log probabilities
+    finished: torch.Tensor   # bool [prompts, beams]: whether each has come to the eos
+
+
+def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
+                   eos: int | None = None) -> Beams:
+    """Beam search over several prompts at once (1-d int64 arrays), ``batch.beams`` beams
+    each (an empty batch of as many requests as there are beams in all). Prompt i is
+    prefilled once, as request i * beams; its beams share its pages from then on, and part
+    from each other's as they differ. A beam that has come to ``eos`` stays as it is. Nothing
+    waits for the GPU before the end, where a batch whose pages ran out raises. The batch's
+    requests are left as the last choice found them."""
+    dev, B = batch.lens.device, batch.beams
+    lens = [p.numel() for p in prompts]
+    R = len(lens)
+    if n_tokens < 1 or not lens or min(lens) < 1 or batch.lens.shape[0] != R * B:
+        raise ValueError(f"generate_beams: n_tokens={n_tokens}, prompts of {lens} tokens, "
+                         f"{batch.lens.shape[0]} requests of {B} beams")
+    ids = torch.cat([p.to(dev) for p in prompts])
+    q_lens = torch.tensor([n if b == 0 else 0 for n in lens for b in range(B)],
+                          dtype=torch.int32, device=dev)
+    refused = batch.step(q_lens, ids.numel(), max(lens)).refused.clone()
+    one = torch.ones_like(q_lens)
+    # at first one beam of each prompt has a score, and the others come from it
+    scores = torch.full((R, B), -math.inf, device=dev)
+    scores[:, 0] = 0.0
+    done = torch.zeros((R, B), dtype=torch.bool, device=dev)
+    steps = []
+    for i in range(n_tokens):
+        logits = model.forward_paged(ids, batch)
+        s = ops.beam_select(logits, scores, finished=None if eos is None else done, eos=eos)
+        steps.append(s)
+        scores, done = s.scores, s.finished
+        if i + 1 < n_tokens:
+            refused += batch.fork(s.parents.view(-1))
+            refused += batch.step(one, R * B, 1).refused
+            ids = s.tokens.view(-1).long()
+    # every beam's tokens, from its last one back
+    at = torch.arange(R * B, device=dev)
+    tokens = []
+    for s in reversed(steps):
+        tokens.append(s.tokens.view(-1)[at])
+        at = s.parents.view(-1)[at].long()
+    if int(refused):
+        raise RuntimeError("generate_beams: the batch's pages ran out, or a request's length")
+    return Beams(torch.stack(tokens[::-1], -1).view(R, B, n_tokens), scores, done)
 
 
 # ---------------------------------------------------------------------------
