@@ -32,6 +32,7 @@ constexpr int SP_THREADS = 1024;
 constexpr int SP_MIN_KEYS = 128, SP_MAX_COLS = 64;
 
 // A part of the work, for one kv head.
+enum { NARROW, WIDE, PREFIX_WIDE };  // a block of 32 columns, or of 128
 struct SharedItem {
     int r;       // the request whose pages hold the keys
     int t0;      // the first token of the columns' rows
@@ -39,7 +40,7 @@ struct SharedItem {
     int c0;      // the block's first
     int k0, k1;  // its keys
     int state;   // its first column's state, -1: the block writes its rows itself
-    int wide;    // a block of 128 columns, else of 32
+    int kind;
 };
 // What a token's rows are joined from.
 struct SharedToken {
@@ -66,7 +67,7 @@ struct PlanArgs {
     SharedItem *items;
     SharedToken *tokens;
     int R, W, T, G, NG, page_log2;
-    int max_items, target, wide_runs, key;
+    int max_items, slots, key;
     int64_t states;
 };
 
@@ -158,6 +159,10 @@ struct Segment {
     int blocks, runs;
     bool alone;  // nothing else is joined with it
 };
+// Runs a part that are wanted, of narrow and of wide blocks (parts_wanted).
+struct Each {
+    int narrow, wide;
+};
 __device__ __forceinline__ Segment segment_of(const PlanArgs &a, int s) {
     Segment g;
     if (s < a.NG) {
@@ -175,10 +180,23 @@ __device__ __forceinline__ Segment segment_of(const PlanArgs &a, int s) {
     g.runs = (g.to - g.from + CHUNK_KEYS - 1) / CHUNK_KEYS;
     return g;
 }
-// Parts of each of its blocks, and runs a part, where `each` runs are wanted.
-__device__ __forceinline__ int parts_of(const PlanArgs &a, const Segment &g, int each, int &per) {
-    per = max(max(each, g.cols > 32 ? a.wide_runs : 1), (g.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
+// Parts of each of its blocks, and runs a part.
+__device__ __forceinline__ int parts_of(const Segment &g, const Each &each, int &per) {
+    per = max(g.cols > 32 ? each.wide : each.narrow, (g.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
     return max(1, (g.runs + per - 1) / per);
+}
+// One round of workgroups for all blocks' runs; where it would be a long one, narrow blocks,
+// whose parts' states are small, are cut for one and a half: what waits for HBM at a part's
+// start and end is then hidden by others. (us, one round / one and a half: 96 requests of
+// up to 4000 keys behind 3968 147 / 140, 32 pairs behind 1984 62 / 57; but 8 requests
+// behind 8192, a short round, 16.2 / 22, and 96 wide requests behind 16256 120 / 133.)
+__device__ __forceinline__ Each parts_wanted(unsigned long long runs, int slots) {
+    const unsigned long long one = (runs + slots - 1) / slots;
+    const unsigned long long more = (2 * runs + 3 * slots - 1) / (3 * slots);
+    Each e;
+    e.wide = one < 1 ? 1 : one < (1u << 30) ? (int)one : 1 << 30;
+    e.narrow = one < 8 ? e.wide : more < (1u << 30) ? (int)more : 1 << 30;
+    return e;
 }
 __device__ __forceinline__ int width_of(const Segment &g) { return min(g.cols, WIDE_COLS); }
 
@@ -207,13 +225,12 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
     }
     if (runs) atomicAdd(&total, runs);
     __syncthreads();
-    const unsigned long long want = (total + a.target - 1) / a.target;
-    const int each = want < 1 ? 1 : want < (1u << 30) ? (int)want : 1 << 30;
+    const Each each = parts_wanted(total, a.slots);
     int items = 0, states = 0;
     for (int s = s0; s < s1; ++s) {
         const Segment g = segment_of(a, s);
         int per;
-        const int ns = parts_of(a, g, each, per);
+        const int ns = parts_of(g, each, per);
         items += g.blocks * ns;
         if (!g.alone || ns > 1) states += g.blocks * ns * width_of(g);
     }
@@ -225,7 +242,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
     for (int s = s0; s < s1; ++s) {
         const Segment g = segment_of(a, s);
         int per;
-        const int ns = parts_of(a, g, each, per);
+        const int ns = parts_of(g, each, per);
         ia += g.blocks * ns;
         if (!g.alone || ns > 1) sa += g.blocks * ns * width_of(g);
         item_end[s] = ia;
@@ -250,7 +267,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
         }
         const Segment g = segment_of(a, hi);
         int per;
-        const int ns = parts_of(a, g, each, per), width = width_of(g);
+        const int ns = parts_of(g, each, per), width = width_of(g);
         const int i = u - (hi ? item_end[hi - 1] : 0), part = i % ns;
         // (wide blocks from the last, which sees the most keys)
         const int block = g.blocks - 1 - i / ns;
@@ -259,7 +276,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
         it.t0 = g.t0;
         it.cols = g.cols;
         it.c0 = block * width;
-        it.wide = g.cols > 32;
+        it.kind = g.cols <= 32 ? NARROW : hi < a.NG ? PREFIX_WIDE : WIDE;
         // keys that the block's last token sees
         int to = g.to;
         if (hi >= a.NG) {
@@ -288,7 +305,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
             o.seen = min(max(p.len - p.n + t - p.q0 + 1, 0), p.len);
             int per;
             const Segment g = segment_of(a, a.NG + lo);
-            const int ns = parts_of(a, g, each, per), s = a.NG + lo;
+            const int ns = parts_of(g, each, per), s = a.NG + lo;
             if (g.cols && (!g.alone || ns > 1)) {
                 o.own = s ? state_end[s - 1] : 0;
                 o.own_parts = ns | width_of(g) << 16;
@@ -298,7 +315,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
                 const int of = a.group_of[lo];
                 const Segment f = segment_of(a, of);
                 o.prefix = of ? state_end[of - 1] : 0;
-                o.prefix_parts = parts_of(a, f, each, per) | width_of(f) << 16;
+                o.prefix_parts = parts_of(f, each, per) | width_of(f) << 16;
                 o.prefix_col = (t - f.t0) * a.G;
             }
         }
@@ -442,8 +459,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
 
 // A block of 128 columns: wave w has the columns 32 w .. 32 w + 31, and all four share
 // each stage of two key tiles, staged by DMA into one of two buffers while the other is
-// read.
-template <typename T, int D>
+// read. REST: with the product of what rounding the probabilities left.
+template <typename T, int D, bool REST>
 __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedItem &it, int hk,
                                             char *lds) {
     typedef Tile<D> Tl;
@@ -478,8 +495,8 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             dma_paged_tile<T, D, true, false>(pool + lo * D, pool + hi * D, it.k1 - key,
                                               dst + wave * Tl::BYTES, lane);
     };
-    auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more)
-                    __attribute__((always_inline)) {
+    auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more,
+                    auto with_rest) __attribute__((always_inline)) {
         // every wave's DMAs of stage s have landed, and every wave is done with
         // the buffer the next ones go to
         att_wait_vmcnt<0>();
@@ -503,20 +520,30 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             attn_mask(sc[0], end - k0, h2);
             attn_mask(sc[1], end - k0 - ATT_KT, h2);
         }
-        uint32_t p[2][8];
-        softmax_pair<T, D>(st, sc, p, a.scale);
+        uint32_t p[2][8], rest[2][8];
+        softmax_pair<T, D, with_rest.value>(st, sc, p, a.scale, rest);
         attn_pv<T, D>(st, p[0], vf);
+        if constexpr (with_rest.value) attn_pv<T, D>(st, rest[0], vf);
         read_v<T, D>(cb + 3 * Tl::BYTES, vf, lane);
         attn_pv<T, D>(st, p[1], vf);
+        if constexpr (with_rest.value) attn_pv<T, D>(st, rest[1], vf);
     };
     const int stages = (ntiles + 1) / 2;
     char *b0 = lds, *b1 = lds + STAGE;
-    attn_init(st);
-    read_q<D>((const T *)a.q + qrow * D, h2, qf);
-    if (stages) issue(0, b0);
-    for (int s = 0; s < stages; s += 2) {  // workgroup-uniform
-        step(b0, b1, s, s + 1 < stages);
-        if (s + 1 < stages) step(b1, b0, s + 1, s + 2 < stages);
+    auto run = [&](auto with_rest) __attribute__((always_inline)) {
+        attn_init(st);
+        read_q<D>((const T *)a.q + qrow * D, h2, qf);
+        if (stages) issue(0, b0);
+        for (int s = 0; s < stages; s += 2) {  // workgroup-uniform
+            step(b0, b1, s, s + 1 < stages, with_rest);
+            if (s + 1 < stages) step(b1, b0, s + 1, s + 2 < stages, with_rest);
+        }
+    };
+    run(std::integral_constant<bool, REST>{});
+    // (as in the narrow block; here all four waves, which share the stages)
+    if (REST && __syncthreads_or(not_a_number(st))) {
+        flip = a.flip;
+        run(std::false_type{});
     }
     if (it.state < 0) {
         const float inv = row_inv(st.l);
@@ -563,56 +590,79 @@ void shared_attn_kernel(SharedArgs a) {
     for (int i = 0; i < (int)(sizeof(SharedItem) / 4); ++i)
         f[i] = __builtin_amdgcn_readfirstlane(f[i]);
     const SharedItem it = __builtin_bit_cast(SharedItem, f);
-    if (it.wide)
-        shared_wide<T, D>(a, it, blockIdx.x, lds);
+    if (it.kind == PREFIX_WIDE)
+        shared_wide<T, D, true>(a, it, blockIdx.x, lds);
+    else if (it.kind == WIDE)
+        shared_wide<T, D, false>(a, it, blockIdx.x, lds);
     else
         shared_narrow<T, D>(a, it, blockIdx.x, lds);
 #endif
 }
 
-// A row's parts joined, in order: D / 4 lanes a row, of four values each.
-template <typename T, int D>
+// A row's parts joined: D / 4 lanes a row, of four values each. GROUPS such lanes take
+// every so manyth part, in order, and are added in order.
+template <typename T, int D, int GROUPS>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 #pragma clang fp contract(off)
-    constexpr int LANES = D / 4;
-    const int lane = threadIdx.x % LANES;
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    if (row >= (int64_t)a.T * a.H || a.head[1] != a.key) return;
-    const int t = (int)(row / a.H), h = (int)(row - (int64_t)t * a.H), hk = h / a.G;
-    const SharedToken k = a.tokens[t];
-    if (k.prefix < 0 && k.own < 0) return;
+    constexpr int LANES = D / 4, ROWS = 256 / (LANES * GROUPS);
+    __shared__ float4 sums[GROUPS > 1 ? GROUPS * ROWS * LANES : 1];
+    __shared__ float2 lms[GROUPS > 1 ? GROUPS * ROWS : 1];
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    const int at_row = sub % ROWS, group = sub / ROWS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + at_row;
+    const bool there = row < (int64_t)a.T * a.H && a.head[1] == a.key;
+    const int t = there ? (int)(row / a.H) : 0, h = there ? (int)(row - (int64_t)t * a.H) : 0;
+    const int hk = h / a.G, g = h - hk * a.G;
+    SharedToken k = {0, -1, 0, 0, -1, 0, 0, 0};
+    if (there) k = a.tokens[t];
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f, m = -INFINITY;
-    auto join = [&](int first, int parts, int col) {
-        const int n = parts & 0xffff, width = parts >> 16, b = col / width;
-        const int64_t at = hk * a.states + first + (int64_t)b * n * width + (col - b * width);
-        constexpr int IN_FLIGHT = 8;
-        for (int s0 = 0; s0 < n; s0 += IN_FLIGHT) {
-            float4 v[IN_FLIGHT];
-            float2 w[IN_FLIGHT];
-#pragma unroll
-            for (int i = 0; i < IN_FLIGHT; ++i) {
-                const int64_t c = at + (int64_t)min(s0 + i, n - 1) * width;
-                v[i] = *(const float4 *)(a.o + c * D + 4 * lane);
-                w[i] = a.lm[c];
-            }
-#pragma unroll
-            for (int i = 0; i < IN_FLIGHT; ++i) {
-                // (a part that saw no key of the row: whatever its sums)
-                if (s0 + i >= n || w[i].y == -INFINITY) continue;
-                const MergeCoef c = merge_coef(m, w[i].y);
-                o.x = merge_one(o.x, v[i].x, c);
-                o.y = merge_one(o.y, v[i].y, c);
-                o.z = merge_one(o.z, v[i].z, c);
-                o.w = merge_one(o.w, v[i].w, c);
-                l = merge_one(l, w[i].x, c);
-                m = c.m_new;
-            }
-        }
+    auto add = [&](const float4 &v, const float2 &w) {
+        if (w.y == -INFINITY) return;  // (a part that saw no key of the row: whatever its sums)
+        const MergeCoef c = merge_coef(m, w.y);
+        o.x = merge_one(o.x, v.x, c);
+        o.y = merge_one(o.y, v.y, c);
+        o.z = merge_one(o.z, v.z, c);
+        o.w = merge_one(o.w, v.w, c);
+        l = merge_one(l, w.x, c);
+        m = c.m_new;
     };
-    const int g = h - hk * a.G;
-    if (k.prefix >= 0) join(k.prefix, k.prefix_parts, k.prefix_col + g);
-    if (k.own >= 0) join(k.own, k.own_parts, k.own_col + g);
+    // the prefix's parts, then the row's own, as one list
+    auto place = [&](int first, int parts, int col, int &n, int &width) -> int64_t {
+        n = first < 0 ? 0 : parts & 0xffff;
+        width = first < 0 ? 1 : parts >> 16;
+        const int b = col / width;
+        return hk * a.states + first + (int64_t)b * n * width + (col - b * width);
+    };
+    int np, wp, no, wo;
+    const int64_t pa = place(k.prefix, k.prefix_parts, k.prefix_col + g, np, wp);
+    const int64_t oa = place(k.own, k.own_parts, k.own_col + g, no, wo) - (int64_t)np * wo;
+    const int n = np + no;
+    constexpr int IN_FLIGHT = 8;
+    for (int s0 = group; s0 < n; s0 += GROUPS * IN_FLIGHT) {
+        float4 v[IN_FLIGHT];
+        float2 w[IN_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; ++i) {
+            const int s = min(s0 + GROUPS * i, n - 1);
+            const int64_t c = s < np ? pa + (int64_t)s * wp : oa + (int64_t)s * wo;
+            v[i] = *(const float4 *)(a.o + c * D + 4 * lane);
+            w[i] = a.lm[c];
+        }
+#pragma unroll
+        for (int i = 0; i < IN_FLIGHT; ++i)
+            if (s0 + GROUPS * i < n) add(v[i], w[i]);
+    }
+    if constexpr (GROUPS > 1) {
+        sums[threadIdx.x] = o;
+        if (lane == 0) lms[sub] = make_float2(l, m);
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i)
+            add(sums[threadIdx.x + i * ROWS * LANES], lms[sub + i * ROWS]);
+    }
+    if (k.prefix < 0 && k.own < 0) return;  // (nothing to join)
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     st8((T *)a.out + row * D + 4 * lane, pack4<T>(e));
@@ -628,7 +678,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 // blocks are filled up to 128, so at most two, and one of the request's own keys; of a
 // block cut in n parts n - 1 more, and n <= 2 (n - 1) where nothing else is joined with it.
 struct SharedGrid {
-    int64_t items, states, target, wide_runs, ints;
+    int64_t items, states, slots, ints;
     int64_t at_groups, at_group_of, at_items, at_tokens;  // in the schedule, ints
     int key;
 };
@@ -636,14 +686,14 @@ inline SharedGrid shared_grid(int64_t T, int64_t R, int64_t NG, int64_t W, int64
                               int64_t D, int64_t page) {
     SharedGrid g;
     const int64_t G = H / HK, cols = T * G;
-    const int64_t slots = 256 * (D == 128 ? shared_per_cu<128>() : shared_per_cu<64>());
     const int64_t some = (R < T ? R : T) + (NG < T ? NG : T);
-    g.target = 3 * slots / 2 / HK;
-    if (g.target < 1) g.target = 1;
-    g.wide_runs = 1;
+    // workgroups that the chip holds, for each kv head
+    g.slots = 256 * (D == 128 ? shared_per_cu<128>() : shared_per_cu<64>()) / HK;
+    if (g.slots < 1) g.slots = 1;
+    const int64_t target = 3 * g.slots / 2 + 1;
     const int64_t blocks = 2 * (cols / WIDE_COLS) + some;
     const int64_t runs = ceil_div(W * page, CHUNK_KEYS);
-    const int64_t extra = g.target < blocks * runs ? g.target : blocks * runs;
+    const int64_t extra = target < blocks * runs ? target : blocks * runs;
     g.items = blocks + extra;
     const int64_t joined = cols < R * SP_MAX_COLS ? cols : R * SP_MAX_COLS;
     g.states = 3 * joined + 2 * extra * (cols < WIDE_COLS ? cols : WIDE_COLS);
@@ -680,8 +730,13 @@ int check_shared(const char *what, int64_t T, int64_t R, int64_t NG, int64_t W, 
 template <typename T, int D>
 int launch_shared(const SharedArgs &a, const SharedGrid &g, hipStream_t st) {
     shared_attn_kernel<T, D><<<dim3((unsigned)a.HK, (unsigned)g.items), 64 * PA_WAVES, 0, st>>>(a);
-    shared_join_kernel<T, D>
-        <<<(unsigned)ceil_div((int64_t)a.T * a.H * (D / 4), 256), 256, 0, st>>>(a);
+    // few rows: eight groups of lanes a row, whose parts are then read together (8 requests
+    // behind 8192 keys 28 -> 22 us in all; 128 of them 52 with, 46 without)
+    const int64_t rows = (int64_t)a.T * a.H, lanes = rows * (D / 4);
+    if (rows <= 1024)
+        shared_join_kernel<T, D, 8><<<(unsigned)ceil_div(8 * lanes, 256), 256, 0, st>>>(a);
+    else
+        shared_join_kernel<T, D, 1><<<(unsigned)ceil_div(lanes, 256), 256, 0, st>>>(a);
     return launch_status("shared attention");
 }
 
@@ -717,8 +772,8 @@ extern "C" int mi_paged_shared_plan(const int32_t *block_table, int64_t table_wi
                         (SharedGroup *)(schedule + g.at_groups), schedule + g.at_group_of,
                         (SharedItem *)(schedule + g.at_items),
                         (SharedToken *)(schedule + g.at_tokens), (int)R, (int)table_width, (int)T,
-                        (int)(H / HK), (int)n_groups, lp, (int)g.items, (int)g.target,
-                        (int)g.wide_runs, g.key, g.states};
+                        (int)(H / HK), (int)n_groups, lp, (int)g.items, (int)g.slots,
+                        g.key, g.states};
     hipStream_t st = as_stream(stream);
     shared_keys_kernel<<<(unsigned)n_groups, SP_THREADS, 0, st>>>(a);
     int64_t grid = ceil_div(T + g.items, 2 * SP_THREADS);
