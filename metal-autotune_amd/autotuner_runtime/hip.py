@@ -524,12 +524,24 @@ def beam_select(x, scores, finished, eos: int, K: int, out_scores, parents, toke
                                 stream), "beam_select")
 
 
+@functools.lru_cache(maxsize=1024)
+def _fork_workspace_bytes(R, W) -> int:
+    """mi_paged_fork_workspace_bytes, a function of these numbers alone."""
+    return int(lib().mi_paged_fork_workspace_bytes(R, W))
+
+
+@functools.lru_cache(maxsize=1024)
+def _compact_workspace_bytes(n_pages) -> int:
+    """mi_paged_compact_workspace_bytes, a function of the number alone."""
+    return int(lib().mi_paged_compact_workspace_bytes(n_pages))
+
+
 def paged_fork(table, kv_lens, sources, free_pages, free_count, refused, pools) -> None:
     """mi_paged_fork over checked arrays; pools: an ops.PagePools."""
     R, W = table.shape
     n_pages, HK, page, row = pools.shape
     stream = _stream(table)
-    nbytes = int(lib().mi_paged_fork_workspace_bytes(R, W))
+    nbytes = _fork_workspace_bytes(R, W)
     ws = _workspace("pages", table.device, stream, nbytes, 1 << 20, zero=PAGES_ZERO_BYTES)
     _check(lib().mi_paged_fork(table.data_ptr(), W, kv_lens.data_ptr(), sources.data_ptr(), R,
                                free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
@@ -543,7 +555,7 @@ def paged_compact(table, kv_lens, free_pages, free_count, live, pools) -> None:
     R, W = table.shape
     n_pages, HK, page, row = pools.shape
     stream = _stream(table)
-    nbytes = int(lib().mi_paged_compact_workspace_bytes(n_pages))
+    nbytes = _compact_workspace_bytes(n_pages)
     ws = _workspace("pages", table.device, stream, nbytes, 1 << 20, zero=PAGES_ZERO_BYTES)
     _check(lib().mi_paged_compact(table.data_ptr(), W, kv_lens.data_ptr(), R, free_pages.data_ptr(),
                                   free_pages.shape[0], free_count.data_ptr(), live.data_ptr(),

@@ -575,9 +575,9 @@ def beam_select(logits, scores, width: int | None = None, finished=None,
     if K < 1:
         raise ValueError(f"beam_select: width={K}")
     x = logits if logits.stride(1) == 1 and logits.stride(0) >= 0 else logits.contiguous()
-    ids = torch.empty((2, R, K), dtype=_I32, device=x.device)
-    out = BeamStep(scores.new_empty((R, K)), ids[0], ids[1],
-                   torch.empty((R, K), dtype=torch.bool, device=x.device))
+    parents = x.new_empty((R, K), dtype=_I32)
+    out = BeamStep(scores.new_empty((R, K)), parents, torch.empty_like(parents),
+                   x.new_empty((R, K), dtype=torch.bool))
     with _on(dev):
         hip.beam_select(x, scores, finished, -1 if eos is None else eos, K, *out)
     return out

@@ -17,22 +17,30 @@
 // is that of the sum's largest terms, about 1e-7. Rows are cut the same wherever they lie,
 // so that rows of equal logits have equal lse, and equal candidates stay equal.
 //
-// Bound by HBM at many rows (the row's one read), by launch and trips to memory, one
-// after another, at few: pass, the row's ticket, ranks, second reading, the prompt's
-// ticket, the lists.
+// Bound at many rows by HBM beside the VALU (exponentials; 2000 rows of 151936 bf16, 608 MB,
+// 126 us, 4.8 TB/s), at few by launch and trips to memory, one after another: pass, the
+// row's ticket, ranks, second reading, the prompt's ticket, the lists (four rows 13.2 us,
+// 240 rows, 73 MB, 24).
 #include "mi_rows.h"
 
 namespace mi {
 namespace {
 
 constexpr int BS_MAX_R = 4096, BS_MAX_B = 64, BS_MAX_K = LP_MAX_TOP;
-constexpr int64_t BS_SPLIT_ROWS = 512;  // rows from which on none is split
+constexpr int64_t BS_SPLIT_ROWS = 160;  // rows from which on none is split
 static_assert((BS_SPLIT_ROWS + BS_MAX_R) * 4 <= MI_BEAM_ZERO_BYTES, "a ticket a row and a prompt");
 
 // A part of a row's sum: the reference, the largest value, sum 2^(x log2 e - zero).
 struct Part3 {
     float ref, top, s;
 };
+
+// By how much, in units, sums against `from` have to be scaled for `to`: an integer where
+// both are near, so that nothing is lost.
+__device__ __forceinline__ float moved(float from, float to) {
+    return far(from) || far(to) ? (from - to) * LP_LOG2E + (excess(from) - excess(to))
+                                : units(from) - units(to);
+}
 
 // One chunk added to a wave's sum; the key of its maximum at maxima[c].
 template <typename T>
@@ -48,9 +56,7 @@ __device__ __forceinline__ void add_beam_chunk(Part3 &a, const Piece<T> (&pc)[Ro
     if (lane == 0) maxima[c] = key_of(cm);
     a.top = fmaxf(a.top, cm);
     if (cm > a.ref + 2.0f) {  // (uniform)
-        a.s *= __builtin_amdgcn_exp2f(far(a.ref) || far(cm)
-                                          ? (a.ref - cm) * LP_LOG2E + (excess(a.ref) - excess(cm))
-                                          : units(a.ref) - units(cm));
+        a.s *= __builtin_amdgcn_exp2f(moved(a.ref, cm));
         a.ref = cm;
     }
     float s = 0.0f;
@@ -79,13 +85,13 @@ __device__ __forceinline__ Part3 beam_pass(const Row<T, true> &row, int c0, int 
     Part3 a = {-3.4028235e38f, -INFINITY, 0.0f};
     const int w1 = min(c1, row.V / LP_CHUNK);
     uint4 raw[PER];
-    if (c0 < w1) row.template load<false>(c0, lane, raw);
+    if (c0 < w1) row.template load<true>(c0, lane, raw);
     for (int c = c0; c < w1; c += STEP) {
         Piece<T> pc[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) launder(raw[i]);
         row.open(raw, pc);
-        if (c + STEP < w1) row.template load<false>(c + STEP, lane, raw);
+        if (c + STEP < w1) row.template load<true>(c + STEP, lane, raw);
         add_beam_chunk<T>(a, pc, c, maxima, lane);
     }
     const int end = row.V / LP_CHUNK;  // the chunk that the row fills in part
@@ -98,15 +104,31 @@ __device__ __forceinline__ Part3 beam_pass(const Row<T, true> &row, int c0, int 
     return a;
 }
 
-// log of a part's sum e^x, in 64 bits. Where the zero is an integer number of units,
-// t was x times log2 e's fp32 value; what that lacks is put back at the part's largest
-// value (the others weigh less the farther they lie from it).
-__device__ __forceinline__ double part_log(const Part3 &p) {
+// Parts joined, one a lane (n of them; the others' are of no matter), in every lane.
+struct Joined {
+    float ref, top;
+    double s;
+};
+__device__ __forceinline__ Joined join_parts(Part3 p, int n, int lane) {
+    if (lane >= n) p = {-3.4028235e38f, -INFINITY, 0.0f};
+    Joined j;
+    j.ref = wave_max(p.ref);
+    j.top = wave_max(p.top);
+    j.s = (double)(p.s * __builtin_amdgcn_exp2f(moved(p.ref, j.ref)));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) j.s += __shfl_xor(j.s, o, 64);
+    return j;
+}
+// log sum e^x of what was joined, in 64 bits; NaN where there was a NaN or +inf, or no
+// value above -inf. Where the zero is an integer number of units, t was x times log2 e's
+// fp32 value; what that lacks is put back at the largest value (the others weigh less the
+// farther they lie from it).
+__device__ __forceinline__ double joined_log(const Joined &j) {
     constexpr double LN2 = 0.69314718055994530942, LACKS = 1.44269504088896340736 - (double)LP_LOG2E;
-    if (p.s == 0.0f) return -INFINITY;
-    const double ls = log((double)p.s);
-    return far(p.ref) ? (double)p.ref + ls
-                      : LN2 * ((double)units(p.ref) + (double)p.top * LACKS) + ls;
+    if (!(j.s > 0.0)) return NAN;
+    const double ls = log(j.s);
+    return far(j.ref) ? (double)j.ref + ls
+                      : LN2 * ((double)units(j.ref) + (double)j.top * LACKS) + ls;
 }
 
 struct BeamArgs {
@@ -210,10 +232,8 @@ template <int WAVES> inline size_t beam_lds(int64_t B, int64_t K) {
     const size_t join = (size_t)(B * K * 12 + B * 4);
     return join > sizeof(BeamLds<WAVES>) ? join : sizeof(BeamLds<WAVES>);
 }
-template <typename T, bool SPLIT>
-__global__ __launch_bounds__(64 * (SPLIT ? LP_SPLIT_WAVES : LP_WAVES))
-void beam_kernel(BeamArgs a) {
-    constexpr int WAVES = SPLIT ? LP_SPLIT_WAVES : LP_WAVES;
+template <typename T, bool SPLIT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void beam_kernel(BeamArgs a) {
     __shared__ Part3 part[WAVES];
     // the row's, then the prompt's (beam_lds)
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -229,17 +249,23 @@ void beam_kernel(BeamArgs a) {
         const Part3 p = beam_pass<T, WAVES>(row, c0 + wave, c1, maxima, lane);
         if (lane == 0) part[wave] = p;
         __syncthreads();
+        Part3 mine;
         if constexpr (SPLIT) {
             int *all = a.maxima + r * a.nc;
             for (int c = c0 + threadIdx.x; c < c1; c += 64 * WAVES)
                 __hip_atomic_store(all + c, maxima[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            float4 *sums = a.part + (r * segments + blockIdx.x) * WAVES;
-            if (threadIdx.x < WAVES) {
-                const Part3 q = part[threadIdx.x];
-                put_part((float2 *)(sums + threadIdx.x), make_float2(q.ref, q.top));
-                put_part((float2 *)(sums + threadIdx.x) + 1, make_float2(q.s, 0.0f));
+            if (wave == 0) {
+                const Joined j = join_parts(part[lane % WAVES], WAVES, lane);
+                float4 *sums = a.part + r * segments + blockIdx.x;
+                if (lane == 0) {
+                    put_part((float2 *)sums, make_float2(j.ref, j.top));
+                    put_part((float2 *)sums + 1, make_float2((float)j.s, 0.0f));
+                }
             }
             if (!last_of(a.row_tickets + r, segments)) return;
+            const float2 *sums = (const float2 *)(a.part + r * segments + min(lane, segments - 1));
+            const float2 u = get_part(sums);
+            mine = {u.x, u.y, get_part(sums + 1).x};
             for (int c = threadIdx.x; c < nc; c += 64 * WAVES)
                 maxima[c] = __hip_atomic_load(all + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -249,27 +275,9 @@ void beam_kernel(BeamArgs a) {
         __syncthreads();
         rank_chunks<WAVES>(maxima, nc, a.K, t);
         if (wave == 0) {
-            // the parts joined, in one order: log sum e^(lse_i - top) + top
-            const int n = segments * WAVES;
-            const float4 *sums = a.part + r * segments * WAVES;
-            auto get = [&](int i) -> Part3 {
-                if constexpr (!SPLIT) return part[i];
-                const float2 u = get_part((const float2 *)(sums + i));
-                return {u.x, u.y, get_part((const float2 *)(sums + i) + 1).x};
-            };
-            double best = -INFINITY;
-            bool wrong = false;
-            for (int i = lane; i < n; i += 64) {
-                const double l = part_log(get(i));
-                wrong |= !(l < INFINITY);  // (NaN, +inf)
-                best = fmax(best, l);
-            }
-            for (int o = 1; o < 64; o <<= 1) best = fmax(best, __shfl_xor(best, o, 64));
-            double sum = 0.0;
-            for (int i = lane; i < n; i += 64) sum += exp(part_log(get(i)) - best);
-            for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-            double lse = best + log(sum);
-            if (__builtin_amdgcn_ballot_w64(wrong)) lse = NAN;
+            Part3 p = part[lane % WAVES];
+            if constexpr (SPLIT) p = mine;
+            const double lse = joined_log(join_parts(p, SPLIT ? segments : WAVES, lane));
             if (lane == 0)
                 __hip_atomic_store((uint64_t *)(a.lse + r), __builtin_bit_cast(uint64_t, lse),
                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -290,43 +298,50 @@ void beam_kernel(BeamArgs a) {
     join_beams<WAVES>(prompt, a, lds);
 }
 
-// Segments of a row, as the log probabilities': none from 512 rows on; below, about 512
-// workgroups in all, of at least a chunk a wave.
+// Segments of a row, and a workgroup's waves. Few rows are split, about 512 workgroups of
+// eight waves in all, of at least a chunk a wave and at most 64 a row (a lane a segment joins
+// them): 64 rows of 151936 17.3 us, in one workgroup of 16 waves each 19.3. From 160 rows
+// on none is, which spares the row's ticket (240 rows 27.7 -> 24; 480 47 -> 35), of 16
+// waves as long as there is hardly more than one a CU (240 rows 24, of eight 25.4; 480 44,
+// of eight 36).
 struct BeamSplit {
-    int64_t nc, segments, per;
+    int64_t nc, segments, per, waves;
 };
 inline BeamSplit beam_split(int64_t rows, int64_t V) {
     BeamSplit s;
     s.nc = ceil_div(V, LP_CHUNK);
-    const int64_t most = ceil_div(s.nc, LP_SPLIT_WAVES);
-    const int64_t want = rows < BS_SPLIT_ROWS ? ceil_div(512, rows) : 1;
-    s.per = ceil_div(s.nc, want < most ? want : most);
+    int64_t want = rows < BS_SPLIT_ROWS ? ceil_div(512, rows) : 1;
+    if (want > ceil_div(s.nc, 8)) want = ceil_div(s.nc, 8);
+    if (want > 64) want = 64;
+    s.per = ceil_div(s.nc, want);
     s.segments = ceil_div(s.nc, s.per);
+    s.waves = s.segments == 1 && rows <= 320 ? 16 : 8;
     return s;
 }
 inline int64_t beam_bytes(const BeamSplit &s, int64_t rows, int64_t K) {
     const int64_t split =
-        rows < BS_SPLIT_ROWS ? rows * (s.segments * LP_SPLIT_WAVES * 16 + ceil_div(s.nc, 2) * 8) : 0;
+        s.segments > 1 ? rows * (s.segments * 16 + ceil_div(s.nc, 2) * 8) : 0;
     return MI_BEAM_ZERO_BYTES + split + rows * (8 + 8 * K);
 }
 
 template <typename T>
 int launch_beam(BeamArgs a, int64_t rows, const BeamSplit &s, char *ws, hipStream_t st) {
-    const bool split = rows < BS_SPLIT_ROWS;
+    const bool split = s.segments > 1;
     a.row_tickets = (unsigned *)ws;
     a.prompt_tickets = a.row_tickets + BS_SPLIT_ROWS;
     a.nc = (int)(ceil_div(s.nc, 2) * 2);
     a.per = (int)s.per;
     a.part = (float4 *)(ws + MI_BEAM_ZERO_BYTES);
-    a.maxima = (int *)(a.part + (split ? rows * s.segments * LP_SPLIT_WAVES : 0));
+    a.maxima = (int *)(a.part + (split ? rows * s.segments : 0));
     a.lse = (double *)(a.maxima + (split ? rows * a.nc : 0));
     a.best = (float2 *)(a.lse + rows);
     if (split)
-        beam_kernel<T, true><<<dim3((unsigned)s.segments, (unsigned)rows), 64 * LP_SPLIT_WAVES,
-                               beam_lds<LP_SPLIT_WAVES>(a.B, a.K), st>>>(a);
+        beam_kernel<T, true, 8><<<dim3((unsigned)s.segments, (unsigned)rows), 64 * 8,
+                               beam_lds<8>(a.B, a.K), st>>>(a);
+    else if (s.waves == 16)
+        beam_kernel<T, false, 16><<<(unsigned)rows, 64 * 16, beam_lds<16>(a.B, a.K), st>>>(a);
     else
-        beam_kernel<T, false>
-            <<<(unsigned)rows, 64 * LP_WAVES, beam_lds<LP_WAVES>(a.B, a.K), st>>>(a);
+        beam_kernel<T, false, 8><<<(unsigned)rows, 64 * 8, beam_lds<8>(a.B, a.K), st>>>(a);
     return launch_status("beam select");
 }
 

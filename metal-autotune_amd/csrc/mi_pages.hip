@@ -87,90 +87,111 @@ __device__ __forceinline__ int wg_before(int v, int *total) {
     return at;
 }
 
+// A bitmap's words of this thread, [w0, w1) of `words`, each read once where there are at
+// most KEPT of them (65536 pages).
+template <typename F> struct Words {
+    static constexpr int KEPT = 4;
+    F get;
+    int w0, w1;
+    unsigned kept[KEPT];
+    __device__ __forceinline__ Words(int words, F get_) : get(get_) {
+        const int per = (words + PG_THREADS - 1) / PG_THREADS;
+        w0 = min((int)threadIdx.x * per, words), w1 = min(w0 + per, words);
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) kept[i] = w0 + i < w1 ? get(w0 + i) : 0;
+    }
+    template <typename G> __device__ __forceinline__ void each(G f) {
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i)
+            if (w0 + i < w1) f(w0 + i, kept[i]);
+        for (int w = w0 + KEPT; w < w1; ++w) f(w, get(w));
+    }
+};
+template <typename F> __device__ __forceinline__ Words<F> words_of(int pages, F get) {
+    return Words<F>((pages + 31) >> 5, get);
+}
+
 __device__ __forceinline__ void fork_books(const PagesArgs &a) {
-    __shared__ int keeper[PG_MAX_R];
-    const int words = (a.pages + 31) >> 5, per = (words + PG_THREADS - 1) / PG_THREADS;
-    const int w0 = min((int)threadIdx.x * per, words), w1 = min(w0 + per, words);
+    __shared__ int keeper[PG_MAX_R], source[PG_MAX_R], length[PG_MAX_R];  // length: the source's
     const int each = (a.R + PG_THREADS - 1) / PG_THREADS;
     const int r0 = min((int)threadIdx.x * each, a.R), r1 = min(r0 + each, a.R);
     const int mask = (1 << a.page_log2) - 1;
-    auto gone = [&](int w) { return get_agent(a.before + w) & ~get_agent(a.after + w); };
-    int mine = 0, wrong = 0;
-    for (int w = w0; w < w1; ++w) mine += __popc(gone(w));
-    for (int r = r0; r < r1; ++r) keeper[r] = 0x7fffffff;
-    __syncthreads();
+    const int count = min(max(*a.free_count, 0), a.n_free);
+    int wrong = 0;
     for (int r = r0; r < r1; ++r) {
         const int s = a.sources[r];
         wrong += s >= a.R;
-        if ((unsigned)s < (unsigned)a.R) atomicMin(&keeper[s], s == r ? -1 : r);
+        source[r] = (unsigned)s < (unsigned)a.R ? s : -1;
+        keeper[r] = 0x7fffffff;
     }
+    auto gone = words_of(a.pages, [&](int w) { return get_agent(a.before + w) & ~get_agent(a.after + w); });
+    int mine = 0;
+    gone.each([&](int, unsigned g) { mine += __popc(g); });
+    for (int r = r0; r < r1; ++r) length[r] = source[r] < 0 ? 0 : a.lens[source[r]];
     __syncthreads();
-    auto copies = [&](int r, int s) {
-        return (unsigned)s < (unsigned)a.R && (held(a, a.lens[s]) & mask) &&
-               keeper[s] != (s == r ? -1 : r);
+    for (int r = r0; r < r1; ++r)
+        if (source[r] >= 0) atomicMin(&keeper[source[r]], source[r] == r ? -1 : r);
+    __syncthreads();
+    auto copies = [&](int r) {
+        const int s = source[r];
+        return s >= 0 && (held(a, length[r]) & mask) && keeper[s] != (s == r ? -1 : r);
     };
     int need = 0;
-    for (int r = r0; r < r1; ++r) need += copies(r, a.sources[r]);
+    for (int r = r0; r < r1; ++r) need += copies(r);
     int freed, needed, wrongs;
     const int at = wg_before(mine, &freed);
     const int taken = wg_before(need, &needed);
     wg_before(wrong, &wrongs);
-    const int count = min(max(*a.free_count, 0), a.n_free);
     const int have = min(count + freed, a.n_free);
     const int lacking = max(needed - have, 0) + wrongs;
     const bool ok = lacking == 0;
     // pages back to the list; the bitmaps zero again
-    for (int w = w0, i = count + at; w < w1; ++w) {
-        unsigned g = gone(w);
+    int i = count + at;
+    gone.each([&](int w, unsigned g) {
         put_agent(a.before + w, 0u);
         put_agent(a.after + w, 0u);
         for (; ok && g; g &= g - 1, ++i)
             if (i < a.n_free) put_agent(a.free_pages + i, 32 * w + __builtin_ctz(g));
-    }
+    });
     settled();
     for (int r = r0, j = taken; ok && r < r1; ++r) {
-        const int s = a.sources[r];
-        const bool there = (unsigned)s < (unsigned)a.R;
-        const int len = there ? a.lens[s] : 0;
         int page = -1;
-        if (copies(r, s)) {
+        if (copies(r)) {
             page = get_agent(a.free_pages + (have - 1 - j));
-            const int n = held(a, len);
+            const int n = held(a, length[r]);
             int *m = a.moves + 4 * j++;
-            m[0] = a.table[(int64_t)s * a.W + (n >> a.page_log2)];
+            m[0] = a.table[(int64_t)source[r] * a.W + (n >> a.page_log2)];
             m[1] = page;
             m[2] = n & mask;
         }
-        a.new_len[r] = len;
+        a.new_len[r] = length[r];
         a.new_last[r] = page;
     }
     if (threadIdx.x == 0) {
         a.head[0] = ok ? needed : -1;
         *a.result = lacking;
+        if (ok) *a.free_count = have - needed;  // (every thread has read it: barriers since)
     }
-    __syncthreads();  // (every thread has read the count)
-    if (threadIdx.x == 0 && ok) *a.free_count = have - needed;
 }
 
 __device__ __forceinline__ void compact_books(const PagesArgs &a) {
-    const int words = (a.pages + 31) >> 5, per = (words + PG_THREADS - 1) / PG_THREADS;
-    const int w0 = min((int)threadIdx.x * per, words), w1 = min(w0 + per, words);
+    auto used = words_of(a.pages, [&](int w) { return get_agent(a.before + w); });
     int mine = 0, live, n, holes = 0, movers = 0;
-    for (int w = w0; w < w1; ++w) mine += __popc(get_agent(a.before + w));
+    used.each([&](int, unsigned u) { mine += __popc(u); });
     wg_before(mine, &live);
     // the bits of word w that lie below page `live`
     auto below = [&](int w) {
         const int d = live - 32 * w;
         return d >= 32 ? ~0u : d <= 0 ? 0u : (1u << d) - 1;
     };
-    for (int w = w0; w < w1; ++w) {
-        const unsigned u = get_agent(a.before + w), b = below(w);
+    used.each([&](int w, unsigned u) {
+        const unsigned b = below(w);
         holes += __popc(~u & b);
         movers += __popc(u & ~b);
-    }
+    });
     int h = wg_before(holes, &n), m = wg_before(movers, &n);
-    for (int w = w0; w < w1; ++w) {
-        const unsigned u = get_agent(a.before + w), b = below(w);
+    used.each([&](int w, unsigned u) {
+        const unsigned b = below(w);
         put_agent(a.before + w, 0u);
         for (unsigned g = ~u & b; g; g &= g - 1)
             put_agent(a.moves + 4 * h++ + 1, 32 * w + __builtin_ctz(g));
@@ -178,7 +199,7 @@ __device__ __forceinline__ void compact_books(const PagesArgs &a) {
             put_agent(a.moves + 4 * m, 32 * w + __builtin_ctz(g));
             a.moves[4 * m + 2] = 1 << a.page_log2;
         }
-    }
+    });
     settled();
     for (int i = threadIdx.x; i < n; i += PG_THREADS)
         a.to[get_agent(a.moves + 4 * i)] = get_agent(a.moves + 4 * i + 1);

@@ -114,6 +114,11 @@ __device__ __forceinline__ uint4 ld16_any(const void *p) {
     const Bytes16 b = *(const Bytes16 *)p;
     return make_uint4(b.v[0], b.v[1], b.v[2], b.v[3]);
 }
+__device__ __forceinline__ uint4 ld16_any_nt(const void *p) {
+    typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(2)));
+    const U4 v = __builtin_nontemporal_load((const U4 *)p);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
 
 // A row as 16-byte pieces from the one that holds its first value; value i of
 // piece p is row element p N + i - skew. What lies outside the row reads as -inf.
@@ -143,7 +148,7 @@ template <typename T, bool ANY = false> struct Row {
         for (int i = 0; i < PER; ++i) {
             const char *at =
                 base + ((int64_t)chunk * LP_CHUNK + (64 * i + lane) * N) * (int)sizeof(T);
-            raw[i] = ANY ? ld16_any(at) : NT ? ld16_nt(at) : ld16(at);
+            raw[i] = ANY ? (NT ? ld16_any_nt(at) : ld16_any(at)) : NT ? ld16_nt(at) : ld16(at);
         }
     }
     __device__ __forceinline__ void open(const uint4 (&raw)[PER], Piece<T> (&pc)[PER]) const {
