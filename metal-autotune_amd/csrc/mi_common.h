@@ -55,6 +55,10 @@ __device__ __forceinline__ uint4 ld16_nt(const void *p) {
 __device__ __forceinline__ uint2 ld8(const void *p) { return *(const uint2 *)p; }
 __device__ __forceinline__ void st16(void *p, uint4 v) { *(uint4 *)p = v; }
 __device__ __forceinline__ void st8(void *p, uint2 v) { *(uint2 *)p = v; }
+__device__ __forceinline__ void st16_nt(void *p, uint4 v) {
+    typedef unsigned U4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store((U4){v.x, v.y, v.z, v.w}, (U4 *)p);
+}
 
 // Unpack the 8 values of a 16-byte group of T into floats.
 template <typename T> __device__ __forceinline__ void unpack8(uint4 raw, float (&f)[8]) {

@@ -117,16 +117,17 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
             if (s.n == 0 || s.len == 0) continue;
             const int *row = a.table + (int64_t)r * a.W;
             const int stop = *(volatile int *)&limit;
-            for (int w0 = 0; w0 < stop; w0 += 256) {
-                int x[4], y[4];
+            constexpr int AHEAD = 8;
+            for (int w0 = 0; w0 < stop; w0 += 64 * AHEAD) {
+                int x[AHEAD], y[AHEAD];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < AHEAD; ++i) {
                     const int w = min(w0 + 64 * i + lane, stop - 1);
                     x[i] = with[w], y[i] = row[w];
                 }
                 bool differ = false;
 #pragma unroll
-                for (int i = 3; i >= 0; --i) {
+                for (int i = AHEAD - 1; i >= 0; --i) {
                     const uint64_t b = __builtin_amdgcn_ballot_w64(x[i] != y[i]);
                     if (b) {
                         differ = true;
@@ -203,7 +204,7 @@ __device__ __forceinline__ int width_of(const Segment &g) { return min(g.cols, W
 // The list. Every workgroup sums over all segments by itself, then makes its share of the
 // items and tokens, each finding its segment by bisection.
 __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
-    __shared__ int item_end[2 * SP_MAX_R], state_end[2 * SP_MAX_R];
+    __shared__ int item_end[2 * SP_MAX_R], state_end[2 * SP_MAX_R], cu[SP_MAX_R + 1];
     __shared__ int waves[2][SP_THREADS / 64];
     __shared__ unsigned long long total;
     __shared__ int wrong;
@@ -214,13 +215,20 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
     __syncthreads();
     // offsets that fall: nothing is taken (their rows could be those of others)
     bool falls = false;
-    for (int r = threadIdx.x; r < a.R; r += SP_THREADS) falls |= a.cu_q[r + 1] < a.cu_q[r];
+    for (int r = threadIdx.x; r <= a.R; r += SP_THREADS) {
+        cu[r] = a.cu_q[r];
+        falls |= r < a.R && a.cu_q[r + 1] < cu[r];
+    }
     for (int g = threadIdx.x; g < a.NG; g += SP_THREADS)
         falls |= a.cu_groups[g + 1] < a.cu_groups[g];
     if (falls) wrong = 1;
+    // (the thread's first segment, as a rule its only one, is kept)
+    Segment kept = {};
+    if (s0 < s1) kept = segment_of(a, s0);
+    auto segment = [&](int s) { return s == s0 ? kept : segment_of(a, s); };
     unsigned long long runs = 0;
     for (int s = s0; s < s1; ++s) {
-        const Segment g = segment_of(a, s);
+        const Segment g = segment(s);
         runs += (unsigned long long)g.blocks * g.runs;
     }
     if (runs) atomicAdd(&total, runs);
@@ -228,7 +236,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
     const Each each = parts_wanted(total, a.slots);
     int items = 0, states = 0;
     for (int s = s0; s < s1; ++s) {
-        const Segment g = segment_of(a, s);
+        const Segment g = segment(s);
         int per;
         const int ns = parts_of(g, each, per);
         items += g.blocks * ns;
@@ -240,7 +248,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
     int ia = iu - items, sa = su - states;
     for (int w = 0; w < wave; ++w) ia += waves[0][w], sa += waves[1][w];
     for (int s = s0; s < s1; ++s) {
-        const Segment g = segment_of(a, s);
+        const Segment g = segment(s);
         int per;
         const int ns = parts_of(g, each, per);
         ia += g.blocks * ns;
@@ -255,8 +263,10 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
         a.head[0] = ok ? all : 0;
         a.head[1] = a.key;
     }
-    const int step = gridDim.x * SP_THREADS, at = blockIdx.x * SP_THREADS + threadIdx.x;
-    for (int u = at; ok && u < all; u += step) {
+    // every other workgroup makes items, every other one tokens
+    const int step = gridDim.x / 2 * SP_THREADS;
+    const int at = blockIdx.x / 2 * SP_THREADS + threadIdx.x;
+    for (int u = at; ok && blockIdx.x % 2 == 0 && u < all; u += step) {
         int lo = -1, hi = segments - 1;  // item_end[lo] <= u < item_end[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -290,12 +300,12 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
                        ? -1 : (hi ? state_end[hi - 1] : 0) + (block * ns + part) * width;
         a.items[u] = it;
     }
-    for (int t = at; t < a.T; t += step) {
+    for (int t = at; blockIdx.x % 2 && t < a.T; t += step) {
         SharedToken o = {0, -1, 0, 0, -1, 0, 0, 0};
-        int lo = 0, hi = a.R;  // cu_q[lo] <= t < cu_q[hi]
+        int lo = 0, hi = a.R;  // cu[lo] <= t < cu[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (a.cu_q[mid] <= t)
+            if (cu[mid] <= t)
                 lo = mid;
             else
                 hi = mid;
@@ -776,10 +786,9 @@ extern "C" int mi_paged_shared_plan(const int32_t *block_table, int64_t table_wi
                         g.key, g.states};
     hipStream_t st = as_stream(stream);
     shared_keys_kernel<<<(unsigned)n_groups, SP_THREADS, 0, st>>>(a);
-    int64_t grid = ceil_div(T + g.items, 2 * SP_THREADS);
-    if (grid < 1) grid = 1;
-    if (grid > 64) grid = 64;
-    shared_plan_kernel<<<(unsigned)grid, SP_THREADS, 0, st>>>(a);
+    int64_t grid = ceil_div(T > g.items ? T : g.items, SP_THREADS);
+    grid = grid < 1 ? 1 : grid > 32 ? 32 : grid;
+    shared_plan_kernel<<<(unsigned)(2 * grid), SP_THREADS, 0, st>>>(a);
     return launch_status("shared plan");
 }
 
