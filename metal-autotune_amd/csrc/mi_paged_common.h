@@ -18,12 +18,19 @@ constexpr int WIDE_COLS = 128;
 // lo (rows 0..15) and hi (rows 16..31, its own 16 rows); the rest arrive as zeros.
 // NT: non-temporal, for what is read once (decode: 48 requests of 64 to 8191 keys
 // 152 -> 136 us; wide blocks, which share keys through the L2, 97 -> 105 with it).
-template <typename T, int D, bool ISV, bool NT>
+// SCALAR: `left` clamped in scalar registers; else it is vector work, and each of the first
+// rows' loads a loop over lanes (96 requests behind 16256 keys 125 -> 120 us; but decode
+// with heads of 64, which four waves a SIMD leave 128 registers, would spill).
+template <typename T, int D, bool ISV, bool NT, bool SCALAR = false>
 __device__ __forceinline__ void dma_paged_tile(const T *lo, const T *hi, int left, char *dst,
                                                int lane) {
     typedef Tile<D> Tl;
-    const int n0 = left < 0 ? 0 : (left < 16 ? left : 16);
-    const int n1 = left < 16 ? 0 : (left < 32 ? left - 16 : 16);
+    int n0 = left < 0 ? 0 : (left < 16 ? left : 16);
+    int n1 = left < 16 ? 0 : (left < 32 ? left - 16 : 16);
+    if constexpr (SCALAR) {
+        n0 = __builtin_amdgcn_readfirstlane(n0);
+        n1 = __builtin_amdgcn_readfirstlane(n1);
+    }
     const __amdgpu_buffer_rsrc_t r0 = att_rsrc(lo, (uint32_t)(n0 * D * 2));
     const __amdgpu_buffer_rsrc_t r1 = att_rsrc(hi, (uint32_t)(n1 * D * 2));
 #pragma unroll

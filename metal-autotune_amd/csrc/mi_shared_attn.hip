@@ -32,7 +32,7 @@ constexpr int SP_THREADS = 1024;
 constexpr int SP_MIN_KEYS = 128, SP_MAX_COLS = 64;
 
 // A part of the work, for one kv head.
-enum { NARROW, WIDE, PREFIX_WIDE };  // a block of 32 columns, or of 128
+enum { NARROW, WIDE_REST, WIDE };  // a block of 32 columns, or of 128
 struct SharedItem {
     int r;       // the request whose pages hold the keys
     int t0;      // the first token of the columns' rows
@@ -89,6 +89,7 @@ __device__ __forceinline__ Span span_of(const PlanArgs &a, int r) {
 // tokens or keys do not count.
 __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
     __shared__ int lead, limit, most, others;
+    __shared__ bool part[SP_MAX_R];  // whether the request counts
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int first = min(max(a.cu_groups[g], 0), a.R);
     const int end = min(max(a.cu_groups[g + 1], first), a.R);
@@ -97,7 +98,8 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
     for (int r = first + (int)threadIdx.x; r < end; r += SP_THREADS) {
         const Span s = span_of(a, r);
         a.group_of[r] = g;
-        if (s.n == 0 || s.len == 0) continue;
+        part[r] = s.n > 0 && s.len > 0;
+        if (!part[r]) continue;
         atomicMin(&lead, r);
         atomicMin(&limit, max(s.len - s.n, 0) >> a.page_log2);
         atomicMax(&most, s.n);
@@ -112,30 +114,37 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
     const int l = lead;
     if (l < end) {
         const int *with = a.table + (int64_t)l * a.W;
-        for (int r = l + 1 + wave; r < end; r += SP_THREADS / 64) {
-            const Span s = span_of(a, r);
-            if (s.n == 0 || s.len == 0) continue;
-            const int *row = a.table + (int64_t)r * a.W;
-            const int stop = *(volatile int *)&limit;
-            constexpr int AHEAD = 8;
-            for (int w0 = 0; w0 < stop; w0 += 64 * AHEAD) {
-                int x[AHEAD], y[AHEAD];
+        // a wave compares four requests' rows with the lead's, 256 entries a step
+        constexpr int ROWS = 4, AHEAD = 4, WAVES = SP_THREADS / 64;
+        for (int r0 = l + 1 + wave; r0 < end; r0 += ROWS * WAVES) {
+            const int *row[ROWS];
+#pragma unroll
+            for (int j = 0; j < ROWS; ++j) {
+                const int r = r0 + j * WAVES;
+                row[j] = r < end && part[r] ? a.table + (int64_t)r * a.W : with;
+            }
+            for (int w0 = 0; w0 < *(volatile int *)&limit; w0 += 64 * AHEAD) {
+                int x[AHEAD], y[ROWS][AHEAD];
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i) {
-                    const int w = min(w0 + 64 * i + lane, stop - 1);
-                    x[i] = with[w], y[i] = row[w];
+                    const int w = min(w0 + 64 * i + lane, a.W - 1);
+                    x[i] = with[w];
+#pragma unroll
+                    for (int j = 0; j < ROWS; ++j) y[j][i] = row[j][w];
                 }
-                bool differ = false;
+                int first_other = a.W;  // (entries past the limit may differ: it stands)
 #pragma unroll
                 for (int i = AHEAD - 1; i >= 0; --i) {
-                    const uint64_t b = __builtin_amdgcn_ballot_w64(x[i] != y[i]);
-                    if (b) {
-                        differ = true;
-                        if (lane == 0)
-                            atomicMin(&limit, min(w0 + 64 * i + (int)__builtin_ctzll(b), stop));
-                    }
+                    bool other = false;
+#pragma unroll
+                    for (int j = 0; j < ROWS; ++j) other |= x[i] != y[j][i];
+                    const uint64_t b = __builtin_amdgcn_ballot_w64(other);
+                    if (b) first_other = w0 + 64 * i + (int)__builtin_ctzll(b);
                 }
-                if (differ) break;
+                if (first_other < a.W) {
+                    if (lane == 0) atomicMin(&limit, first_other);
+                    break;
+                }
             }
         }
     }
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(SP_THREADS) void shared_plan_kernel(PlanArgs a) {
         it.t0 = g.t0;
         it.cols = g.cols;
         it.c0 = block * width;
-        it.kind = g.cols <= 32 ? NARROW : hi < a.NG ? PREFIX_WIDE : WIDE;
+        it.kind = g.cols <= 32 ? NARROW : hi < a.NG && g.blocks == 1 ? WIDE_REST : WIDE;
         // keys that the block's last token sees
         int to = g.to;
         if (hi >= a.NG) {
@@ -394,8 +403,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
             int64_t lo, hi;
             const int key = it.k0 + t0 * ATT_KT;
             pg.rows(0, key, lo, hi);
-            dma_paged_tile<T, D, false, true>(k + lo * D, k + hi * D, it.k1 - key, ks, lane);
-            dma_paged_tile<T, D, true, true>(v + lo * D, v + hi * D, it.k1 - key, vs, lane);
+            dma_paged_tile<T, D, false, true, true>(k + lo * D, k + hi * D, it.k1 - key, ks, lane);
+            dma_paged_tile<T, D, true, true, true>(v + lo * D, v + hi * D, it.k1 - key, vs, lane);
         }
         for (int kt = t0; kt < ntiles; kt += PA_WAVES) {  // wave-uniform
             const int nx = kt + PA_WAVES, key = it.k0 + nx * ATT_KT;
@@ -415,7 +424,7 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
 #pragma unroll
             for (int s = 0; s < D / 16; ++s) launder(kf[s]);  // the reads have returned
             __builtin_amdgcn_sched_barrier(0);
-            if (more) dma_paged_tile<T, D, false, true>(k + lo * D, k + hi * D, it.k1 - key, ks, lane);
+            if (more) dma_paged_tile<T, D, false, true, true>(k + lo * D, k + hi * D, it.k1 - key, ks, lane);
             f32x16 s = attn_scores<T, D>(kf, qf);
             const int k0 = it.k0 + kt * ATT_KT;
             if (k0 + ATT_KT > full) attn_mask(s, end - k0, h2);
@@ -431,7 +440,7 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
             if constexpr (with_rest.value) attn_pv<T, D>(st, rest, vf);
             __builtin_amdgcn_sched_barrier(0);
             att_wait_lds();  // V's reads have returned
-            if (more) dma_paged_tile<T, D, true, true>(v + lo * D, v + hi * D, it.k1 - key, vs, lane);
+            if (more) dma_paged_tile<T, D, true, true, true>(v + lo * D, v + hi * D, it.k1 - key, vs, lane);
         }
     };
     run(kslot, vslot, std::true_type{});
@@ -499,10 +508,10 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
         int64_t lo, hi;
         pg.rows(s, key, lo, hi);
         if (wave < 2)
-            dma_paged_tile<T, D, false, false>(pool + lo * D, pool + hi * D, it.k1 - key,
+            dma_paged_tile<T, D, false, false, true>(pool + lo * D, pool + hi * D, it.k1 - key,
                                                dst + wave * Tl::BYTES, lane);
         else
-            dma_paged_tile<T, D, true, false>(pool + lo * D, pool + hi * D, it.k1 - key,
+            dma_paged_tile<T, D, true, false, true>(pool + lo * D, pool + hi * D, it.k1 - key,
                                               dst + wave * Tl::BYTES, lane);
     };
     auto step = [&](const char *__restrict__ cb, char *__restrict__ nb, int s, bool more,
@@ -591,16 +600,17 @@ __attribute__((amdgpu_waves_per_eu(shared_per_cu<D>())))
 void shared_attn_kernel(SharedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[PagedLds<D>::BYTES];
-    if (a.head[1] != a.key || (int)blockIdx.y >= a.head[0]) return;  // (workgroup-uniform)
     const int *p = (const int *)(a.items + blockIdx.y);
     int f[sizeof(SharedItem) / 4];
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(SharedItem) / 4); ++i) f[i] = p[i];
+    const int items = a.head[0], key = a.head[1];  // (asked for together)
+    if (key != a.key || (int)blockIdx.y >= items) return;  // (workgroup-uniform)
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(SharedItem) / 4); ++i)
         f[i] = __builtin_amdgcn_readfirstlane(f[i]);
     const SharedItem it = __builtin_bit_cast(SharedItem, f);
-    if (it.kind == PREFIX_WIDE)
+    if (it.kind == WIDE_REST)
         shared_wide<T, D, true>(a, it, blockIdx.x, lds);
     else if (it.kind == WIDE)
         shared_wide<T, D, false>(a, it, blockIdx.x, lds);
@@ -620,11 +630,12 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const int at_row = sub % ROWS, group = sub / ROWS;
     const int64_t row = (int64_t)blockIdx.x * ROWS + at_row;
-    const bool there = row < (int64_t)a.T * a.H && a.head[1] == a.key;
-    const int t = there ? (int)(row / a.H) : 0, h = there ? (int)(row - (int64_t)t * a.H) : 0;
+    const int64_t at_most = min(row, (int64_t)a.T * a.H - 1);
+    const int t = (int)(at_most / a.H), h = (int)(at_most - (int64_t)t * a.H);
     const int hk = h / a.G, g = h - hk * a.G;
-    SharedToken k = {0, -1, 0, 0, -1, 0, 0, 0};
-    if (there) k = a.tokens[t];
+    SharedToken k = a.tokens[t];
+    const int key = a.head[1];  // (asked for together)
+    if (row != at_most || key != a.key) k.prefix = k.own = -1;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f, m = -INFINITY;
     auto add = [&](const float4 &v, const float2 &w) {
