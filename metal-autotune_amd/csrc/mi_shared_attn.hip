@@ -15,6 +15,21 @@
 // shares, from the table's rows, and a list of the parts. The attention is a workgroup a
 // part and kv head, then a kernel that joins a row's parts. A block whose keys are not cut
 // and that has no prefix writes its rows itself.
+//
+// What bounds it, on MI355X (32 q / 8 kv heads): four beams behind 960 keys 9.4 us, two
+// launches and a chain of trips to memory; 64 requests in five groups, heads of 64, 94 MB,
+// 28 us, HBM at 4.1 TB/s while the parts are read (23 us, of which about 6 are their starts
+// and ends); 96 requests of up to four tokens behind 16256 keys, 359 MB and 61 GFLOP, 119
+// us: the matrix cores over the prefix (65 us by themselves at 1 PFLOP/s), then HBM over
+// the requests' own keys (52 us), which overlap little, since two workgroups a CU is all
+// that its registers and LDS hold (either kind dealt among the other gained nothing). The
+// paged attention, which reads the prefix once a request, takes 12.2, 54 and 583 us.
+//
+// Probabilities enter the second product as T. Where a group's rows are one block, reading
+// K and V bounds it, and the product of what that rounding left is taken too, as for single
+// tokens in the paged attention: what is off is then the result's own rounding (bf16 1.7e-3
+// of the norm, fp16 2.1e-4). Larger groups are bound by these products, as prompts are, and
+// keep one rounding (2.3e-3, 2.7e-4; with the rests 96 requests take 146 us instead of 125).
 #include <type_traits>
 
 #include "mi_paged_common.h"
@@ -28,7 +43,10 @@ namespace {
 constexpr int SP_MAX_R = 4096;
 constexpr int SP_THREADS = 1024;
 // Keys that a group has to share, and the columns (rows of a kv head) that each of its
-// requests may have, for it to be worth a part of its own.
+// requests may have, for it to be worth parts of its own. (us with / without: 16 groups of
+// four sharing 64 keys 20.4 / 18.6, 128 21.0 / 22.3, 512 23.2 / 29.7, 1024 29.0 / 40.8; 16
+// requests behind 2048, in fours, of 64 columns each 27.7 / 32.7, of 128 42.4 / 43.1; eight
+// behind 4096 of 64 27.9 / 29.9, of 128 38.2 / 36.9, of 512 101 / 94.)
 constexpr int SP_MIN_KEYS = 128, SP_MAX_COLS = 64;
 
 // A part of the work, for one kv head.
@@ -190,10 +208,13 @@ __device__ __forceinline__ Segment segment_of(const PlanArgs &a, int s) {
     g.runs = (g.to - g.from + CHUNK_KEYS - 1) / CHUNK_KEYS;
     return g;
 }
-// Parts of each of its blocks, and runs a part.
+// Parts of each of its blocks, and runs a part: parts of one length, and none for a quarter
+// of one (16 prompts of 128 tokens behind 2048 keys, a round of whole blocks, 146 -> 90 us).
 __device__ __forceinline__ int parts_of(const Segment &g, const Each &each, int &per) {
-    per = max(g.cols > 32 ? each.wide : each.narrow, (g.runs + MAX_CHUNKS - 1) / MAX_CHUNKS);
-    return max(1, (g.runs + per - 1) / per);
+    const int want = g.cols > 32 ? each.wide : each.narrow;
+    const int ns = min(max(1, (g.runs - want / 4 + want - 1) / want), MAX_CHUNKS);
+    per = max(1, (g.runs + ns - 1) / ns);
+    return ns;
 }
 // One round of workgroups for all blocks' runs; where it would be a long one, narrow blocks,
 // whose parts' states are small, are cut for one and a half: what waits for HBM at a part's
@@ -737,7 +758,7 @@ int check_shared(const char *what, int64_t T, int64_t R, int64_t NG, int64_t W, 
                     (long long)page);
     if (T < 0 || T > (1 << 18) || R < 1 || R > SP_MAX_R || NG < 1 || NG > R || W < 1 ||
         W > (0x3fffffff >> lp) || H < 1 || HK < 1 || H % HK || HK > 65535 ||
-        T * (H / HK) > 0x3fffff)
+        T * (H / HK) > 0x3fffff || H > 0x3fffffff / (T + 1))
         return fail(MI_ERR_ARG, "%s T=%lld (to 2^18) R=%lld (1 to %d) groups=%lld (1 to R) table "
                     "width %lld H=%lld HK=%lld", what, (long long)T, (long long)R, SP_MAX_R,
                     (long long)NG, (long long)W, (long long)H, (long long)HK);
