@@ -117,10 +117,10 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
         const Span s = span_of(a, r);
         a.group_of[r] = g;
         part[r] = s.n > 0 && s.len > 0;
+        atomicMax(&most, s.n);  // (of all: their rows are columns of the prefix's blocks)
         if (!part[r]) continue;
         atomicMin(&lead, r);
         atomicMin(&limit, max(s.len - s.n, 0) >> a.page_log2);
-        atomicMax(&most, s.n);
         atomicAdd(&others, 1);
     }
     // requests outside the groups are in none
@@ -717,8 +717,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
 // in one of its request's, of 128 (or the last, shorter one of each). Parts: one and a
 // half rounds of workgroups, beside one a block. States, of a block's columns one a part:
 // where a prefix is shared (requests of at most SP_MAX_COLS columns) one of the prefix, whose
-// blocks are filled up to 128, so at most two, and one of the request's own keys; of a
-// block cut in n parts n - 1 more, and n <= 2 (n - 1) where nothing else is joined with it.
+// blocks are filled up to 128, so at most two, and one of the request's own keys; of other
+// blocks that are cut, filled up as well, at most two a column; and all parts beyond those.
 struct SharedGrid {
     int64_t items, states, slots, ints;
     int64_t at_groups, at_group_of, at_items, at_tokens;  // in the schedule, ints
@@ -738,7 +738,8 @@ inline SharedGrid shared_grid(int64_t T, int64_t R, int64_t NG, int64_t W, int64
     const int64_t extra = target < blocks * runs ? target : blocks * runs;
     g.items = blocks + extra;
     const int64_t joined = cols < R * SP_MAX_COLS ? cols : R * SP_MAX_COLS;
-    g.states = 3 * joined + 2 * extra * (cols < WIDE_COLS ? cols : WIDE_COLS);
+    const int64_t more = extra * (cols < WIDE_COLS ? cols : WIDE_COLS);
+    g.states = 3 * joined + more + (2 * cols < more ? 2 * cols : more);
     g.at_groups = 16;
     g.at_group_of = g.at_groups + NG * (int64_t)(sizeof(SharedGroup) / 4);
     g.at_items = ceil_div(g.at_group_of + R, 8) * 8;

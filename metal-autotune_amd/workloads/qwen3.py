@@ -187,9 +187,9 @@ class PagedBatch:
         p = ops.paged_plan(
             self.block_table, self.lens, q_lens, self.free_pages, self.free_count,
             self.page_size, num_tokens, out=old)
-        if self.cu_groups is not None:
-            shared = ops.paged_shared_plan(self.block_table, p.cu_q, p.kv_lens, self.cu_groups,
-                                           self.page_size, num_tokens, *self.heads, out=shared)
+        shared = None if self.cu_groups is None else ops.paged_shared_plan(
+            self.block_table, p.cu_q, p.kv_lens, self.cu_groups, self.page_size, num_tokens,
+            *self.heads, out=shared)
         self._plans.pop(num_tokens, None)
         self._plans[num_tokens] = p, shared  # the last
         if len(self._plans) > KEPT_PLANS:

@@ -207,6 +207,20 @@ def test_a_refused_request_in_a_group():
     assert float((got[rest].float() - out[rest].float()).abs().max()) < 0.02
 
 
+def test_a_refused_prompt_in_a_group():
+    """One whose step was refused has a thousand tokens among single ones."""
+    g = gen_of(73)
+    kv, n_q = [300, 0, 260, 280, 250], [1, 1000, 1, 1, 2]
+    kp, vp, table, ks, vs = make_cache(g, [(12, kv)], 16, 2, 64, BF)
+    T = sum(n_q)
+    q, cu, lens = rnd(g, T, 8, 64), i32([0] + np.cumsum(n_q).tolist()), i32(kv)
+    plan = ops.paged_shared_plan(table, cu, lens, i32([0, 5]), 16, T, 8, 2, 64)
+    assert plan.keys.tolist() == [192] and int(plan.schedule[0]) > 0
+    out = ops.paged_shared_attention(q, kp, vp, table, plan, 0.125)
+    check_attention(out, *attention_64(q, ks, vs, n_q, 0.125), BF)
+    assert not out[1:1001].any()
+
+
 def test_offsets_that_fall():
     """Nothing is written where they do, and the next plan is as before."""
     out, plan, (q, kp, vp, table, cu, lens, scale) = run([(12, [300, 250, 260])], [1, 2, 1], 8, 2, 64, 16,
