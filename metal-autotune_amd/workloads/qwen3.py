@@ -148,7 +148,8 @@ class PagedBatch:
     ``beams`` > 1: every so many requests, from the first, are a group whose prompts are
     alike (the beams of one, or its samples): ``fork(sources)`` lets requests go on from
     others' keys, and a step's attention reads the keys that a group shares once (``shared``,
-    its plan). ``compact()`` moves the pages in use to the lowest ids. Every request's
+    its plan). ``compact()`` moves the pages in use to the lowest ids. Both belong between a
+    step's forward pass and the next step, whose plan says where its tokens go. Every request's
     part-filled page is its own, so nothing but the cache's entries need know."""
 
     def __init__(self, cfg: "Qwen3Config", n_layers: int, max_requests: int, n_pages: int,
@@ -221,8 +222,8 @@ class PagedBatch:
         return self._pools
 
     def fork(self, sources) -> torch.Tensor:
-        """Request r goes on from the keys of request sources[r] (int32, on the GPU; one of
-        its own step is as good), or ends where that is negative. Returns int32 [1], the
+        """Request r goes on from the keys of request sources[r] (int32, on the GPU:
+        ``beam_select``'s parents, say), or ends where that is negative. Returns int32 [1], the
         pages that were missing: then nothing has changed."""
         return ops.paged_fork(self.block_table, self.lens, sources, self.free_pages,
                               self.free_count, self.pools())
