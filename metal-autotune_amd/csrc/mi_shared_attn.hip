@@ -665,7 +665,9 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f, m = -INFINITY;
     auto add = [&](const float4 &v, const float2 &w) {
-        if (w.y == -INFINITY) return;  // (a part that saw no key of the row: whatever its sums)
+        // (a part that saw no key of the row, whatever its sums; of one whose scores are all
+        // NaN l is NaN, and so are they)
+        if (w.y == -INFINITY && w.x == 0.0f) return;
         const MergeCoef c = merge_coef(m, w.y);
         o.x = merge_one(o.x, v.x, c);
         o.y = merge_one(o.y, v.y, c);
