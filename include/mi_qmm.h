@@ -421,8 +421,8 @@ int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_s
  * not 0; NULL: none) has one, (b, eos), at its own score, and its logits are not read. A
  * beam whose score is -inf or NaN has none, nor has a row with a NaN or +inf; logits of
  * -inf are no candidates. The best first: within a beam by logits, the lowest token first
- * among equal ones; across beams by the candidates in 64 bits (lse_b to about 1e-7), the
- * lowest beam first among equals. Written, [R, K] each: out_scores (rounded to fp32 once);
+ * among equal ones; across beams by the candidates in 64 bits (lse_b to 1.6e-6 in any row,
+ * about 1e-7 in most, alike in rows that are), the lowest beam first among equals. Written, [R, K] each: out_scores (rounded to fp32 once);
  * parents, the row r B + b of each; tokens; out_finished, 1 where the parent had finished
  * or the token is eos (-1: none is). Where there are fewer than K candidates the rest is
  * -inf, r B, 0, 0. 0 <= R <= 4096, 1 <= B <= 64, 1 <= K <= min(64, B V), V <= 2^20.

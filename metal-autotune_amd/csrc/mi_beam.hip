@@ -12,10 +12,14 @@
 //
 // Beams are compared in 64 bits, since candidates of different beams lie close together
 // (fp32 scores near -100 are 8e-6 apart, and two beams' candidates that often): lse_b is
-// the fp32 sum of a row's 2^t, against a reference within 2 of the row's maximum so that
-// t is rounded finely, joined in 64 bits and freed of what log2 e lost in fp32. Its error
-// is that of the sum's largest terms, about 1e-7. Rows are cut the same wherever they lie,
-// so that rows of equal logits have equal lse, and equal candidates stay equal.
+// the sum of a row's 2^t in fp32, against a reference within 2 of the row's maximum so that
+// t is rounded finely, 16 terms of a lane in pairs and their sums, chunk after chunk, in 64
+// bits, and freed of what log2 e lost in fp32. In 2^-24 it is off by at most 2 of the
+// exponential, 4 of the pairs, 0.7 |t| for t's rounding and 0.23 |t| for what log2 e lacks
+// at terms below the maximum, |t| on average at most log2 V + 4: 26 2^-24 = 1.6e-6 (one
+// token over a long constant tail, whose roundings go the same way; random rows 1e-7, rows
+// of one value below 2e-7). Rows are cut the same wherever they lie, so that rows of equal
+// logits have equal lse, and equal candidates stay equal.
 //
 // Bound at many rows by HBM beside the VALU (exponentials; 2000 rows of 151936 bf16, 608 MB,
 // 126 us, 4.8 TB/s), at few by launch and trips to memory, one after another: pass, the
@@ -32,7 +36,8 @@ static_assert((BS_SPLIT_ROWS + BS_MAX_R) * 4 <= MI_BEAM_ZERO_BYTES, "a ticket a 
 
 // A part of a row's sum: the reference, the largest value, sum 2^(x log2 e - zero).
 struct Part3 {
-    float ref, top, s;
+    float ref, top;
+    double s;
 };
 
 // By how much, in units, sums against `from` have to be scaled for `to`: an integer where
@@ -40,6 +45,24 @@ struct Part3 {
 __device__ __forceinline__ float moved(float from, float to) {
     return far(from) || far(to) ? (from - to) * LP_LOG2E + (excess(from) - excess(to))
                                 : units(from) - units(to);
+}
+
+// The sum of 2^t(x) over a lane's 16 values, by pairs of pairs.
+template <typename T, typename F>
+__device__ __forceinline__ float sum_pairs(const Piece<T> (&pc)[Row<T>::PER], F t) {
+    constexpr int N = Row<T>::N;
+    static_assert(N * Row<T>::PER == 16, "a lane's values of a chunk");
+    float level[4];  // of 1, 2, 4, 8 terms each, until there are two
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float s = __builtin_amdgcn_exp2f(t(pc[i / N].f[i % N]));
+        int at = 0;
+#pragma unroll
+        for (; at < 4 && (i >> at & 1); ++at) s = level[at] + s;
+        if (i == 15) return s;
+        level[at] = s;
+    }
+    return 0.0f;  // (not reached)
 }
 
 // One chunk added to a wave's sum; the key of its maximum at maxima[c].
@@ -59,22 +82,12 @@ __device__ __forceinline__ void add_beam_chunk(Part3 &a, const Piece<T> (&pc)[Ro
         a.s *= __builtin_amdgcn_exp2f(moved(a.ref, cm));
         a.ref = cm;
     }
-    float s = 0.0f;
     if (far(a.ref)) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                s += __builtin_amdgcn_exp2f((pc[i].f[j] - a.ref) * LP_LOG2E);
+        a.s += sum_pairs<T>(pc, [&](float x) { return (x - a.ref) * LP_LOG2E; });
     } else {
         const float zero = units(a.ref);
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                s += __builtin_amdgcn_exp2f(__builtin_fmaf(pc[i].f[j], LP_LOG2E, -zero));
+        a.s += sum_pairs<T>(pc, [&](float x) { return __builtin_fmaf(x, LP_LOG2E, -zero); });
     }
-    a.s += s;
 }
 
 // The chunks c0, c0 + STEP, ... below c1 of a row, by one wave; the row's end last.
@@ -82,7 +95,7 @@ template <typename T, int STEP>
 __device__ __forceinline__ Part3 beam_pass(const Row<T, true> &row, int c0, int c1, int *maxima,
                                            int lane) {
     constexpr int PER = Row<T>::PER;
-    Part3 a = {-3.4028235e38f, -INFINITY, 0.0f};
+    Part3 a = {-3.4028235e38f, -INFINITY, 0.0};
     const int w1 = min(c1, row.V / LP_CHUNK);
     uint4 raw[PER];
     if (c0 < w1) row.template load<true>(c0, lane, raw);
@@ -110,13 +123,11 @@ struct Joined {
     double s;
 };
 __device__ __forceinline__ Joined join_parts(Part3 p, int n, int lane) {
-    if (lane >= n) p = {-3.4028235e38f, -INFINITY, 0.0f};
+    if (lane >= n) p = {-3.4028235e38f, -INFINITY, 0.0};
     Joined j;
     j.ref = wave_max(p.ref);
     j.top = wave_max(p.top);
-    j.s = (double)(p.s * __builtin_amdgcn_exp2f(moved(p.ref, j.ref)));
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) j.s += __shfl_xor(j.s, o, 64);
+    j.s = wave_add(p.s * (double)__builtin_amdgcn_exp2f(moved(p.ref, j.ref)));
     return j;
 }
 // log sum e^x of what was joined, in 64 bits; NaN where there was a NaN or +inf, or no
@@ -259,13 +270,13 @@ __global__ __launch_bounds__(64 * WAVES) void beam_kernel(BeamArgs a) {
                 float4 *sums = a.part + r * segments + blockIdx.x;
                 if (lane == 0) {
                     put_part((float2 *)sums, make_float2(j.ref, j.top));
-                    put_part((float2 *)sums + 1, make_float2((float)j.s, 0.0f));
+                    put_part((float2 *)sums + 1, __builtin_bit_cast(float2, j.s));
                 }
             }
             if (!last_of(a.row_tickets + r, segments)) return;
             const float2 *sums = (const float2 *)(a.part + r * segments + min(lane, segments - 1));
             const float2 u = get_part(sums);
-            mine = {u.x, u.y, get_part(sums + 1).x};
+            mine = {u.x, u.y, __builtin_bit_cast(double, get_part(sums + 1))};
             for (int c = threadIdx.x; c < nc; c += 64 * WAVES)
                 maxima[c] = __hip_atomic_load(all + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }

@@ -60,6 +60,26 @@ __device__ __forceinline__ float wave_add(float v) {
     v = row16_sum(v);
     return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
 }
+// The same in 64 bits, two moves a value.
+template <int CTRL> __device__ __forceinline__ double dpp_f64(double v) {
+    const uint2 b = __builtin_bit_cast(uint2, v);
+    const uint2 m = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)b.x, CTRL, 0xF, 0xF, false),
+                     (unsigned)__builtin_amdgcn_update_dpp(0, (int)b.y, CTRL, 0xF, 0xF, false)};
+    return __builtin_bit_cast(double, m);
+}
+__device__ __forceinline__ double readlane_d(double v, int l) {
+    const uint2 b = __builtin_bit_cast(uint2, v);
+    const uint2 m = {(unsigned)__builtin_amdgcn_readlane((int)b.x, l),
+                     (unsigned)__builtin_amdgcn_readlane((int)b.y, l)};
+    return __builtin_bit_cast(double, m);
+}
+__device__ __forceinline__ double wave_add(double v) {
+    v += dpp_f64<0xB1>(v);
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x141>(v);
+    v += dpp_f64<0x140>(v);
+    return (readlane_d(v, 0) + readlane_d(v, 16)) + (readlane_d(v, 32) + readlane_d(v, 48));
+}
 
 // What a wave sums is in units of log2: t = x log2 e - C with C = rint(ref log2 e) an
 // integer, p = 2^t, S = sum p, E = sum p t: one fma a value, rounded as finely as t
