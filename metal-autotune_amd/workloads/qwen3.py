@@ -394,9 +394,10 @@ def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
     """Beam search over several prompts at once (1-d int64 arrays), ``batch.beams`` beams
     each (an empty batch of as many requests as there are beams in all). Prompt i is
     prefilled once, as request i * beams; its beams share its pages from then on, and part
-    from each other's as they differ. A beam that has come to ``eos`` stays as it is. Nothing
-    waits for the GPU before the end, where a batch whose pages ran out raises. The batch's
-    requests are left as the last choice found them."""
+    from each other's as they differ. A beam that has come to ``eos`` stays as it is: its request
+    gives its pages back and brings no more tokens (nor does that of a beam of score -inf).
+    Nothing waits for the GPU before the end, where a batch whose pages ran out raises. The
+    batch's requests are left as the last choice found them."""
     dev, B = batch.lens.device, batch.beams
     lens = [p.numel() for p in prompts]
     R = len(lens)
@@ -407,7 +408,6 @@ def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
     q_lens = torch.tensor([n if b == 0 else 0 for n in lens for b in range(B)],
                           dtype=torch.int32, device=dev)
     refused = batch.step(q_lens, ids.numel(), max(lens)).refused.clone()
-    one = torch.ones_like(q_lens)
     # at first one beam of each prompt has a score, and the others come from it
     scores = torch.full((R, B), -math.inf, device=dev)
     scores[:, 0] = 0.0
@@ -419,9 +419,13 @@ def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
         steps.append(s)
         scores, done = s.scores, s.finished
         if i + 1 < n_tokens:
-            refused += batch.fork(s.parents.view(-1))
-            refused += batch.step(one, R * B, 1).refused
-            ids = s.tokens.view(-1).long()
+            live = (~done & (scores > -math.inf)).view(-1)
+            refused += batch.fork(torch.where(live, s.parents.view(-1), -1))
+            plan = batch.step(live.int(), R * B, 1)
+            refused += plan.refused
+            # their tokens, request after request (the others' to the row behind all)
+            at = torch.where(live, plan.cu_q[:-1], R * B).long()
+            ids = at.new_zeros(R * B + 1).scatter_(0, at, s.tokens.view(-1).long())[:-1]
     # every beam's tokens, from its last one back
     at = torch.arange(R * B, device=dev)
     tokens = []
