@@ -391,8 +391,8 @@ class Beams(NamedTuple):
 
 def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
                    eos: int | None = None) -> Beams:
-    """Beam search over several prompts at once (1-d int64 arrays), ``batch.beams`` beams
-    each (an empty batch of as many requests as there are beams in all). Prompt i is
+    """Beam search over several prompts at once (1-d int64 arrays), ``batch.beams`` (1 to 64)
+    beams each (an empty batch of as many requests as there are beams in all). Prompt i is
     prefilled once, as request i * beams; its beams share its pages from then on, and part
     from each other's as they differ. A beam that has come to ``eos`` stays as it is: its request
     gives its pages back and brings no more tokens (nor does that of a beam of score -inf).
@@ -404,6 +404,10 @@ def generate_beams(model: Qwen3Model, batch: PagedBatch, prompts, n_tokens: int,
     if n_tokens < 1 or not lens or min(lens) < 1 or batch.lens.shape[0] != R * B:
         raise ValueError(f"generate_beams: n_tokens={n_tokens}, prompts of {lens} tokens, "
                          f"{batch.lens.shape[0]} requests of {B} beams")
+    if not 1 <= B <= 64 or not (eos is None or 0 <= eos < model.cfg.vocab_size):
+        # (as the selection does, but before the prompts take pages)
+        raise ValueError(f"generate_beams: {B} beams (1 to 64), eos={eos} of "
+                         f"{model.cfg.vocab_size} tokens")
     ids = torch.cat([p.to(dev) for p in prompts])
     q_lens = torch.tensor([n if b == 0 else 0 for n in lens for b in range(B)],
                           dtype=torch.int32, device=dev)
