@@ -583,6 +583,9 @@ def beam_select(logits, scores, width: int | None = None, finished=None,
     return out
 
 
+FORK_MAX_PAGES = 1 << 20  # that paged_fork and paged_compact cover
+
+
 class PagePools(NamedTuple):
     """The pools of all layers as ``paged_fork`` and ``paged_compact`` take them
     (``page_pools``)."""
@@ -595,7 +598,7 @@ class PagePools(NamedTuple):
 def page_pools(pools) -> PagePools:
     """Pools [pages, heads, page size, head dim] of one shape and type on one device
     (every layer's k_pages and v_pages), made once and kept: whatever pages a fork or a
-    compaction moves, it moves in all of them."""
+    compaction moves, it moves in all of them. Both cover pools of FORK_MAX_PAGES pages."""
     pools = tuple(pools)
     if not pools:
         raise ValueError("page_pools: no pools")

@@ -157,6 +157,9 @@ class PagedBatch:
         def i32(*shape):
             return torch.zeros(shape, dtype=torch.int32, device=device)
 
+        if beams > 1 and n_pages > ops.FORK_MAX_PAGES:
+            raise ValueError(f"PagedBatch: beams fork, which covers {ops.FORK_MAX_PAGES} pages, not "
+                             f"{n_pages}")
         self.page_size = page_size
         self.block_table = i32(max_requests, -(-max_len // page_size))
         self.lens = i32(max_requests)
@@ -179,7 +182,7 @@ class PagedBatch:
         shape = (n_pages, cfg.num_key_value_heads, page_size, cfg.head_dim)
         self.caches = [PagedKVCache(self, shape, device, dtype) for _ in range(n_layers)]
         self._pools = None
-        if self.lens.is_cuda:
+        if n_layers and self.lens.is_cuda:
             self.pools()
 
     def step(self, q_lens, num_tokens: int, max_q_len: int | None = None) -> ops.PagedPlan:
@@ -237,7 +240,19 @@ class PagedBatch:
         """The request's pages go back, but for those that others hold too."""
         sources = torch.arange(self.lens.shape[0], dtype=torch.int32, device=self.lens.device)
         sources[r] = -1
-        self.fork(sources)
+        if self.caches and self.lens.is_cuda and self.free_pages.shape[0] <= ops.FORK_MAX_PAGES:
+            self.fork(sources)
+            return
+        # what a fork would do, where it has no pools or too many pages (this waits for the GPU)
+        n = ((self.lens + self.page_size - 1) // self.page_size)[:, None]
+        live = torch.arange(self.block_table.shape[1], device=self.lens.device) < n
+        held = self.block_table[live & (sources >= 0)[:, None]]
+        gone = self.block_table[r][live[r]].unique()
+        gone = gone[torch.isin(gone, held, invert=True)]
+        at = int(self.free_count)
+        self.free_pages[at:at + gone.shape[0]] = gone
+        self.free_count += gone.shape[0]
+        self.lens[r] = 0
 
 
 class Attention(nn.Module):
