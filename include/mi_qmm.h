@@ -488,7 +488,8 @@ int mi_paged_compact(int32_t *block_table, int64_t table_width, const int32_t *k
  *
  * mi_paged_shared_attention: mi_paged_attention's result for the step that the plan was
  * made for, within rounding: the same sums in another order, which depends on all requests'
- * lengths and groups, deterministic for them. A schedule of other sizes leaves out as it
+ * lengths and groups, deterministic for them; no row's probabilities have fewer bits (those
+ * of requests of 33 to 512 rows a kv head have more). A schedule of other sizes leaves out as it
  * was. workspace: mi_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no
  * initialization needed. Calls sharing one must not overlap. */
 int64_t mi_paged_shared_plan_ints(int64_t T, int64_t R, int64_t n_groups, int64_t table_width,

@@ -25,12 +25,11 @@
 // that its registers and LDS hold (either kind dealt among the other gained nothing). The
 // paged attention, which reads the prefix once a request, takes 12.2, 54 and 583 us.
 //
-// Probabilities enter the second product as T. No row has fewer bits of them than the paged
-// attention gives it: a request of at most 32 columns takes the product of what that rounding
-// left too, over its own keys and over a prefix, whoever shares it (so in all blocks of a
-// group that has such a request; and in a group's only block, where reading K and V bounds
-// it). What is off is then the result's own rounding (bf16 1.7e-3 of the norm, fp16 2.1e-4).
-// Requests of more columns, bound by these products, keep one rounding (2.3e-3, 2.7e-4).
+// Probabilities enter the second product as T, and the product of what that rounding left is
+// taken too: over prefixes in groups of any size, over a request's own keys up to REST_COLS
+// columns. What is off is then the result's own rounding (bf16 1.66e-3 of the norm, fp16
+// 2.1e-4). Prompts, bound by these products, keep one rounding (2.1e-3 to 2.3e-3, 2.8e-4), as
+// in the paged attention, which takes the rests of requests of at most 32 columns.
 #include <type_traits>
 
 #include "mi_paged_common.h"
@@ -49,6 +48,11 @@ constexpr int SP_THREADS = 1024;
 // requests behind 2048, in fours, of 64 columns each 27.7 / 32.7, of 128 42.4 / 43.1; eight
 // behind 4096 of 64 27.9 / 29.9, of 128 38.2 / 36.9, of 512 101 / 94.)
 constexpr int SP_MIN_KEYS = 128, SP_MAX_COLS = 64;
+// Columns up to which a request takes the probabilities' rests over its own keys: four wide
+// blocks, steps of some tokens and short questions. (us with / without: 16 requests of 40
+// tokens behind 960 keys 42 / 35, of 128 tokens behind 384 39 / 33, behind 1900 109 / 86;
+// for prompts the sums are longest and the product dearest: a third more MFMAs of 170 us.)
+constexpr int REST_COLS = 512;
 
 // A part of the work, for one kv head.
 enum { NARROW, WIDE_REST, WIDE };  // a block of 32 columns, or of 128
@@ -74,7 +78,6 @@ struct SharedGroup {
     int lead;      // the request whose pages are read
     int keys;      // keys shared, 0 where they are not worth it
     int t0, cols;  // its tokens' first and their columns
-    int rest;      // whether its blocks take the probabilities' rests
 };
 
 struct PlanArgs {
@@ -108,12 +111,12 @@ __device__ __forceinline__ Span span_of(const PlanArgs &a, int r) {
 // alike, as far as each one's keys from before the step fill them. Requests without
 // tokens or keys do not count.
 __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
-    __shared__ int lead, limit, most, least, others;
+    __shared__ int lead, limit, most, others;
     __shared__ bool part[SP_MAX_R];  // whether the request counts
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int first = min(max(a.cu_groups[g], 0), a.R);
     const int end = min(max(a.cu_groups[g + 1], first), a.R);
-    if (threadIdx.x == 0) lead = a.R, limit = a.W, most = 0, least = a.T, others = 0;
+    if (threadIdx.x == 0) lead = a.R, limit = a.W, most = 0, others = 0;
     __syncthreads();
     for (int r = first + (int)threadIdx.x; r < end; r += SP_THREADS) {
         const Span s = span_of(a, r);
@@ -122,7 +125,6 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
         atomicMax(&most, s.n);  // (of all: their rows are columns of the prefix's blocks)
         if (!part[r]) continue;
         atomicMin(&lead, r);
-        atomicMin(&least, s.n);
         atomicMin(&limit, max(s.len - s.n, 0) >> a.page_log2);
         atomicAdd(&others, 1);
     }
@@ -173,12 +175,11 @@ __global__ __launch_bounds__(SP_THREADS) void shared_keys_kernel(PlanArgs a) {
     if (threadIdx.x) return;
     const int keys = l < end ? limit << a.page_log2 : 0;
     a.keys[g] = keys;
-    SharedGroup o = {l < end ? l : 0, 0, 0, 0, 0};
+    SharedGroup o = {l < end ? l : 0, 0, 0, 0};
     if (first < end) {
         const Span s = span_of(a, first), e = span_of(a, end - 1);
         o.t0 = s.q0;
         o.cols = max(e.q0 + e.n - s.q0, 0) * a.G;
-        o.rest = least * a.G <= 32 || o.cols <= WIDE_COLS;
     }
     if (others > 1 && keys >= SP_MIN_KEYS && most * a.G <= SP_MAX_COLS) o.keys = keys;
     a.groups[g] = o;
@@ -190,7 +191,7 @@ struct Segment {
     int r, t0, cols, from, to;  // keys [from, to)
     int blocks, runs;
     bool alone;  // nothing else is joined with it
-    int rest;    // whether wide blocks take the probabilities' rests
+    bool rest;   // whether wide blocks take the probabilities' rests
 };
 // Runs a part that are wanted, of narrow and of wide blocks (parts_wanted).
 struct Each {
@@ -200,12 +201,13 @@ __device__ __forceinline__ Segment segment_of(const PlanArgs &a, int s) {
     Segment g;
     if (s < a.NG) {
         const SharedGroup o = a.groups[s];
-        g = {o.lead, o.t0, o.keys ? o.cols : 0, 0, o.keys, 0, 0, false, o.rest};
+        g = {o.lead, o.t0, o.keys ? o.cols : 0, 0, o.keys, 0, 0, false, true};
     } else {
         const int r = s - a.NG, of = a.group_of[r];
         const Span p = span_of(a, r);
         const int shared = (unsigned)of < (unsigned)a.NG ? a.groups[of].keys : 0;
-        g = {r, p.q0, p.n * a.G, min(shared, p.len), p.len, 0, 0, shared == 0, 0};
+        g = {r, p.q0, p.n * a.G, min(shared, p.len), p.len, 0, 0, shared == 0,
+             p.n * a.G <= REST_COLS};
         // (of a group's request without keys behind the prefix nothing is to be done)
         if (shared && g.from >= g.to) g.cols = 0;
     }

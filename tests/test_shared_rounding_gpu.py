@@ -44,6 +44,25 @@ def test_large_groups_round_once(R, few, H, HK, D, page, dtype):
     assert float((out - want).norm()) <= float(rounding) + 3e-5 * float(want.norm())
 
 
+@pytest.mark.parametrize("n_q,H,HK,D,page,dtype", [
+    ([40] * 6, 8, 2, 128, 64, BF), ([40, 9, 33, 1], 4, 4, 64, 16, FP), ([40, 40, 21], 16, 2, 64, 32, FP),
+    ([128, 100], 8, 2, 128, 16, BF), ([17, 16, 20], 16, 4, 64, 64, BF), ([512], 2, 2, 128, 128, FP),
+])
+def test_steps_of_some_tokens_round_once(n_q, H, HK, D, page, dtype):
+    """Requests by themselves of up to 512 columns: the bound above."""
+    assert max(n_q) * H // HK <= 512
+    R, T = len(n_q), sum(n_q)
+    kv = [1200 + 37 * r for r in range(R)]
+    g = gen_of(T + D)
+    kp, vp, table, ks, vs = make_cache(g, [(0, kv)], page, HK, D, dtype)
+    q, cu, lens = rnd(g, T, H, D, dtype=dtype), i32([0] + np.cumsum(n_q).tolist()), i32(kv)
+    plan = ops.paged_shared_plan(table, cu, lens, i32([0, R]), page, T, H, HK, D)
+    out = ops.paged_shared_attention(q, kp, vp, table, plan, D ** -0.5).double().cpu()
+    want, _ = attention_64(q, ks, vs, n_q, D ** -0.5)
+    rounding = (want.to(dtype).double() - want).norm()
+    assert float((out - want).norm()) <= float(rounding) + 3e-5 * float(want.norm())
+
+
 @pytest.mark.parametrize("R,n,D,dtype", [(40, 1, 128, BF), (40, 1, 64, FP), (20, 8, 128, FP),
                                          (20, 8, 64, BF), (5, 1, 64, BF)])
 def test_values_that_cancel(R, n, D, dtype):
