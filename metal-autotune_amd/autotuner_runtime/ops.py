@@ -649,10 +649,13 @@ def paged_fork(block_table, kv_lens, sources, free_pages, free_count,
 
 
 def paged_compact(block_table, kv_lens, free_pages, free_count, pools: PagePools) -> torch.Tensor:
-    """The pages that requests hold moved to the lowest ids, in every layer's pools, so
-    that the rest of the pools can go: block_table, free_pages (of as many entries as
-    there are pages) and free_count are changed in place; every page that no request
-    holds is free afterwards. Returns int32 [1]: how many are held."""
+    """The pages that requests hold moved to the lowest ids, in every layer's pools:
+    block_table, free_pages (of as many entries as there are pages) and free_count are
+    changed in place; every page that no request holds is free afterwards, the highest
+    first in the list. Returns int32 [1]: how many are held. To a step one free page is as
+    good as another; this is for caches that are to be stored or moved, which are then the
+    first pages of each pool, or cut: requests go on in copies of the pools' first P pages
+    of N with free_pages[N - P:] and free_count - (N - P)."""
     dev = _check_pages("paged_compact", pools, block_table, kv_lens, free_pages, free_count)
     live = kv_lens.new_empty(1)
     with _on(dev):
