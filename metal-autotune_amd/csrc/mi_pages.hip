@@ -20,7 +20,7 @@
 //
 // Bound by HBM where pages are moved (figures at pages_move_kernel); else by two launches and
 // the trips to memory in the first, one after another: lengths, rows, marks, ticket, bitmaps,
-// lists (four beams 10 us, of which the first launch takes 8).
+// lists (four beams 11 to 12 us, of which the first launch takes 8.5).
 #include "mi_common.h"
 
 namespace mi {

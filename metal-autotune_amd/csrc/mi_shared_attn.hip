@@ -16,14 +16,15 @@
 // part and kv head, then a kernel that joins a row's parts. A block whose keys are not cut
 // and that has no prefix writes its rows itself.
 //
-// What bounds it, on MI355X (32 q / 8 kv heads): four beams behind 960 keys 9.4 us, two
-// launches and a chain of trips to memory; 64 requests in five groups, heads of 64, 94 MB,
-// 28 us, HBM at 4.1 TB/s while the parts are read (23 us, of which about 6 are their starts
-// and ends); 96 requests of up to four tokens behind 16256 keys, 359 MB and 61 GFLOP, 119
-// us: the matrix cores over the prefix (65 us by themselves at 1 PFLOP/s), then HBM over
-// the requests' own keys (52 us), which overlap little, since two workgroups a CU is all
-// that its registers and LDS hold (either kind dealt among the other gained nothing). The
-// paged attention, which reads the prefix once a request, takes 12.2, 54 and 583 us.
+// What bounds it, on MI355X (32 q / 8 kv heads; calls back to back): four beams behind 960
+// keys 13 us, of which a graph takes 9.3, two launches and a chain of trips to memory; 64
+// requests in five groups, heads of 64, 94 MB, 27 us, HBM at 4.0 TB/s while the parts are read
+// (24 us, of which about 6 are their starts and ends); 96 requests of up to four tokens behind
+// 16256 keys, 359 MB and 61 GFLOP (92 with the rests' product), 133 us: the matrix cores over
+// the prefix, busy 49% of the cycles, then HBM over the requests' own keys (43 us by
+// themselves at 7 TB/s), which overlap little, since two workgroups a CU is all that its
+// registers and LDS hold. The paged attention, which reads the prefix once a request, takes
+// 12.1, 54 and 588 us in graphs, where these take 9.3, 27.5 and 137.
 //
 // Probabilities enter the second product as T, and the product of what that rounding left is
 // taken too: over prefixes in groups of any size, over a request's own keys up to REST_COLS
@@ -45,13 +46,13 @@ constexpr int SP_THREADS = 1024;
 // Keys that a group has to share, and the columns (rows of a kv head) that each of its
 // requests may have, for it to be worth parts of its own. (us with / without: 16 groups of
 // four sharing 64 keys 20.4 / 18.6, 128 21.0 / 22.3, 512 23.2 / 29.7, 1024 29.0 / 40.8; 16
-// requests behind 2048, in fours, of 64 columns each 27.7 / 32.7, of 128 42.4 / 43.1; eight
-// behind 4096 of 64 27.9 / 29.9, of 128 38.2 / 36.9, of 512 101 / 94.)
+// requests behind 2048, in fours, of 64 columns each 32.4 / 35.8, of 128 47.7 / 45.0; eight
+// behind 4096 of 64 31.3 / 35.1, of 128 43.8 / 43.2.)
 constexpr int SP_MIN_KEYS = 128, SP_MAX_COLS = 64;
 // Columns up to which a request takes the probabilities' rests over its own keys: four wide
 // blocks, steps of some tokens and short questions. (us with / without: 16 requests of 40
-// tokens behind 960 keys 42 / 35, of 128 tokens behind 384 39 / 33, behind 1900 109 / 86;
-// for prompts the sums are longest and the product dearest: a third more MFMAs of 170 us.)
+// tokens over 1000 keys 42 / 35, of 128 over 500 39 / 33, over 2000 109 / 86. Prompts, which
+// nothing but the products bounds, would take half as many MFMAs again.)
 constexpr int REST_COLS = 512;
 
 // A part of the work, for one kv head.
@@ -225,9 +226,9 @@ __device__ __forceinline__ int parts_of(const Segment &g, const Each &each, int 
 }
 // One round of workgroups for all blocks' runs; where it would be a long one, narrow blocks,
 // whose parts' states are small, are cut for one and a half: what waits for HBM at a part's
-// start and end is then hidden by others. (us, one round / one and a half: 96 requests of
-// up to 4000 keys behind 3968 147 / 140, 32 pairs behind 1984 62 / 57; but 8 requests
-// behind 8192, a short round, 16.2 / 22, and 96 wide requests behind 16256 120 / 133.)
+// start and end is then hidden by others. (us, one round / one and a half: 32 pairs behind
+// 1984 60.8 / 59.1; but 8 requests behind 8192, a short round, 16.4 / 21.7, and with the wide
+// blocks too 96 requests behind 16256 136 / 146.)
 __device__ __forceinline__ Each parts_wanted(unsigned long long runs, int slots) {
     const unsigned long long one = (runs + slots - 1) / slots;
     const unsigned long long more = (2 * runs + 3 * slots - 1) / (3 * slots);
