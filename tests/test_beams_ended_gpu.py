@@ -15,9 +15,9 @@ from test_beams_model_gpu import batch_of, consistent, prompts, small  # noqa: E
 
 
 def test_a_beam_that_ends_grows_no_longer():
-    """One beam a prompt: the first comes to its eos as its second token, and 20 tokens
-    more would pass the table's 96 keys and the pool's twelve pages (90 keys and one are
-    six pages of 16, seven and 20 two)."""
+    """One beam a prompt: the first comes to its eos as its second token at the latest, and
+    20 tokens would pass the table's 96 keys. The pool holds eight pages of 16: six for its
+    90 keys and one token, two for the other's 7 and 19."""
     model, ps = small(), prompts(90, 7)
     free = qwen3.generate_beams(model, batch_of(model, 2, 1), ps, 2)
     eos = int(free.sequences[0, 0, 1])
