@@ -422,9 +422,9 @@ int mi_token_logprobs(const void *logits, int64_t rows, int64_t V, int64_t row_s
  * beam whose score is -inf or NaN has none, nor has a row with a NaN or +inf; logits of
  * -inf are no candidates. The best first: within a beam by logits, the lowest token first
  * among equal ones; across beams by the candidates in 64 bits (lse_b to 1.6e-6 in any row,
- * about 1e-7 in most, alike in rows that are), the lowest beam first among equals. Written, [R, K] each: out_scores (rounded to fp32 once);
- * parents, the row r B + b of each; tokens; out_finished, 1 where the parent had finished
- * or the token is eos (-1: none is). Where there are fewer than K candidates the rest is
+ * about 1e-7 in most, alike in rows that are), the lowest beam first among equals. Written,
+ * [R, K] each: out_scores (rounded to fp32 once); parents, the row r B + b of each; tokens;
+ * out_finished, 1 where the parent had finished or the token is eos (-1: none is). Where there are fewer than K candidates the rest is
  * -inf, r B, 0, 0. 0 <= R <= 4096, 1 <= B <= 64, 1 <= K <= min(64, B V), V <= 2^20.
  * workspace: device memory of mi_beam_select_workspace_bytes(...) bytes, 16-byte aligned,
  * whose first MI_BEAM_ZERO_BYTES (a fixed prefix) are zero before its first use; every
@@ -489,8 +489,8 @@ int mi_paged_compact(int32_t *block_table, int64_t table_width, const int32_t *k
  * mi_paged_shared_attention: mi_paged_attention's result for the step that the plan was
  * made for, within rounding: the same sums in another order, which depends on all requests'
  * lengths and groups, deterministic for them; no row's probabilities have fewer bits (those
- * of requests of 33 to 512 rows a kv head have more). A schedule of other sizes leaves out as it
- * was. workspace: mi_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no
+ * of requests of 33 to 512 rows a kv head have more). A schedule of other sizes leaves out
+ * as it was. workspace: mi_paged_shared_attention_workspace_bytes(...) bytes, 16-byte aligned, no
  * initialization needed. Calls sharing one must not overlap. */
 int64_t mi_paged_shared_plan_ints(int64_t T, int64_t R, int64_t n_groups, int64_t table_width,
                                   int64_t H, int64_t HK, int64_t D, int64_t page_size);

@@ -15,16 +15,16 @@
 // the sum of a row's 2^t in fp32, against a reference within 2 of the row's maximum so that
 // t is rounded finely, 16 terms of a lane in pairs and their sums, chunk after chunk, in 64
 // bits, and freed of what log2 e lost in fp32. In 2^-24 it is off by at most 2 of the
-// exponential, 4 of the pairs, 0.7 |t| for t's rounding and 0.23 |t| for what log2 e lacks
+// exponential, 4 of the pairs, 0.7 |t| for t's rounding and 0.16 |t| for what log2 e lacks
 // at terms below the maximum, |t| on average at most log2 V + 4: 26 2^-24 = 1.6e-6 (one
 // token over a long constant tail, whose roundings go the same way; random rows 1e-7, rows
 // of one value below 2e-7). Rows are cut the same wherever they lie, so that rows of equal
 // logits have equal lse, and equal candidates stay equal.
 //
 // Bound at many rows by HBM beside the VALU (exponentials; 2000 rows of 151936 bf16, 608 MB,
-// 131 us, 4.6 TB/s; 256 rows of fp32, 156 MB, 37), at few by launch and trips to memory, one after another: pass, the
-// row's ticket, ranks, second reading, the prompt's ticket, the lists (four rows 13.2 us,
-// 240 rows, 73 MB, 24).
+// 131 us, 4.6 TB/s; 256 rows of fp32, 156 MB, 37), at few by launch and trips to memory, one
+// after another: pass, the row's ticket, ranks, second reading, the prompt's ticket, the
+// lists (four rows 13.2 us, 240 rows, 73 MB, 24).
 #include "mi_rows.h"
 
 namespace mi {
